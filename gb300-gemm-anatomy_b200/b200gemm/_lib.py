@@ -33,6 +33,14 @@ MODE_2CTA = 2
 MODE_2CTA_M512 = 3
 MODE_2CTA_N128 = 4
 
+VL_BF16 = 0
+VL_F16 = 1
+VL_F32 = 2
+
+VL_NONE = 0
+VL_MEAN = 1
+VL_SUM = 2
+
 STREAM_LDGSTS = 0
 STREAM_TMA = 1
 STREAM_TMA_SW128 = 2
@@ -111,6 +119,19 @@ UmmaConfig = _i64_struct(
     "B200UmmaConfig", ["cta_group", "n", "depth", "iterations", "timed", "num_ctas"]
 )
 
+VocabLossDesc = _i64_struct(
+    "B200VocabLossDesc",
+    ["rows", "vocab", "hidden", "ld_hidden", "ld_weight", "dtype", "top", "index_bytes", "ld_index",
+     "ld_teacher", "teacher_dtype", "ignore_index", "reduction"],
+    doubles=["temperature"],
+)
+
+VocabLossInfo = _i64_struct(
+    "B200VocabLossInfo",
+    ["cta_group", "tile_m", "vocab_tiles", "piece", "pieces", "splits", "workspace_forward",
+     "workspace_backward", "launches_forward", "launches_backward"],
+)
+
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _INT = ctypes.c_int
@@ -155,6 +176,12 @@ SIGNATURES = {
     "b200_stream_plan_result": (_INT, [_P, _P, ctypes.POINTER(StreamResult)]),
     "b200_stream_plan_destroy": (_INT, [_P]),
     "b200_umma_probe": (_INT, [ctypes.POINTER(UmmaConfig), _P, _P, _P, _P, _P, _P]),
+    "b200_vocab_loss_desc_size": (ctypes.c_size_t, []),
+    "b200_vocab_loss_info_size": (ctypes.c_size_t, []),
+    "b200_vocab_loss_info": (_INT, [ctypes.POINTER(VocabLossDesc), _INT, ctypes.POINTER(VocabLossInfo)]),
+    "b200_vocab_loss_forward": (_INT, [ctypes.POINTER(VocabLossDesc), _P, _P, _P, _P, _P, _P, _P, _I64, _P]),
+    "b200_vocab_loss_backward": (_INT, [ctypes.POINTER(VocabLossDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P,
+                                        _I64, _P]),
     "b200_selftest_bounded_wait": (_INT, [ctypes.c_ulonglong, _P, _P]),
     "b200_selftest_occupy": (_INT, [_INT, _INT, ctypes.c_ulonglong, _P]),
     "b200_shard_range": (_INT, [_I64, _I64, _I64, _I64, ctypes.POINTER(_I64),
@@ -166,6 +193,8 @@ _STRUCT_SIZES = {
     "b200_device_info_size": DeviceInfo,
     "b200_stream_result_size": StreamResult,
     "b200_policy_info_size": PolicyInfo,
+    "b200_vocab_loss_desc_size": VocabLossDesc,
+    "b200_vocab_loss_info_size": VocabLossInfo,
 }
 
 _lib = None

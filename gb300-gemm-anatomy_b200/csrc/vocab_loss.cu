@@ -1,0 +1,1668 @@
+// Losses at the vocabulary projection (sm_100a): cross entropy and top-k
+// distillation over logits z = H * W^T that are never kept, with the gradients
+// of H and W.
+//
+// Mathematics. Row t of H (T x D) has the logits z_v = h_t . w_v. With
+// p = softmax(z / tau) over the vocabulary and a sparse target distribution q
+// (one token for the cross entropy, the softmax of a teacher's kept logits for
+// the distillation; entries of one index add up)
+//   loss_t = tau^2 * sum_k q_k (log q_k + lse_t - z_{i_k} / tau),
+//   lse_t  = log sum_v exp(z_v / tau),
+//   dloss_t / dz_v = tau * (p_v - q_v).
+//
+// Forward: one pass over W. A persistent tcgen05 GEMM computes 256-column
+// tiles of z in TMEM; its epilogue keeps, for every row and tile, the running
+// maximum m and s = sum exp((z - m) / tau) and copies out the logits at the
+// row's targets. 8 bytes per (row, tile) leave the SM instead of 1024. A small
+// kernel merges the tiles in order and forms the loss.
+//
+// Backward: the vocabulary is walked in pieces. For each piece, the logits are
+// recomputed and turned into G = g_t (p - q) in 16 bits (T x piece), then
+//   dH += G W_piece     (fp32, added piece after piece in stream order)
+//   dW_piece = G^T H    (rounded once)
+// G is the operand both products read, so it stays the operands' type: with
+// |G| <= 1 (the factor common to all rows is applied after the products) its
+// rounding is half a step of the type for each term, no more than the
+// operands' own.
+//
+// Rows without a target are gathered out first: they cost nothing, and what
+// they hold (padding, infinities, NaN) meets no other row. W and H keep their
+// row-major layout in all three products; where the contraction runs down the
+// rows, the operand tile goes to the tensor cores in its MN-major form.
+#include <algorithm>
+#include <climits>
+#include <cmath>
+#include <cstring>
+#include <mutex>
+
+#include <cuda_fp16.h>
+
+#include "internal.h"
+#include "ptx.cuh"
+
+namespace b200 {
+namespace vl {
+
+constexpr int kBK = 64;
+constexpr int kBN = 256;
+constexpr int kRowsPerCta = 128;
+constexpr int kThreads = 192;
+constexpr int kEpiWarps = 4;
+constexpr int kEpiBufBytes = 32 * 128;
+constexpr int kTmemCols = 2 * kBN;
+constexpr int kQueue = 4;
+constexpr int kNoCol = INT_MAX;
+constexpr int kMaxTop = 256;      // teacher logits per row
+constexpr int kMaxSplits = 16;    // runs of the contraction of dH
+constexpr float kLog2e = 1.4426950408889634f;
+
+// The four products. Operands: Stats, Grad: A = H, B = W (both K-major);
+// Dh: A = G (K-major), B = W (MN-major); Dw: A = G, B = H (both MN-major).
+enum Op { kStats = 0, kGrad = 1, kDh = 2, kDw = 3 };
+
+// What the first kernels of a call leave in the workspace for the others.
+struct Head {
+    int status;       // device status word
+    int counter[2];   // tile scheduler: next tile, finished clusters
+    int ticket;       // finished blocks of the merge kernel
+    int n_rows;       // rows that the products run over
+    int n_valid;      // rows with a loss
+    int compact;      // 1: the rows are those of the gathered copy of H
+    float alpha;      // factor common to all rows of G, applied after the products
+};
+
+template <int kCtaGroup>
+struct Cfg {
+    static constexpr int kStages = kCtaGroup == 1 ? 4 : 6;
+    static constexpr int kABytes = kRowsPerCta * kBK * 2;
+    static constexpr int kBRows = kBN / kCtaGroup;
+    static constexpr int kBBytes = kBRows * kBK * 2;
+    static constexpr int kStageBytes = kABytes + kBBytes;
+    static constexpr int kTileM = kRowsPerCta * kCtaGroup;
+    static constexpr int kEpiOffset = kStages * kStageBytes;
+    static constexpr int kEpiBytes = kEpiWarps * 2 * kEpiBufBytes;
+    static constexpr int kBarOffset = kEpiOffset + kEpiBytes;
+    static constexpr int kBarCount = 2 * kStages + 4 + 2 * kQueue;
+    static constexpr int kBarBytes = kBarCount * 8 + 16 + 4 * kQueue;
+    static constexpr int kSmemBytes = kBarOffset + kBarBytes + 1024;
+    static_assert(kStageBytes % 1024 == 0, "ring slots must keep 1024-byte alignment");
+    static_assert(kSmemBytes <= 232448, "exceeds the 227 KB opt-in shared memory");
+};
+
+struct Params {
+    Head* head;
+    unsigned long long timeout_ns;
+    int fp16;             // operand type: 1 fp16, 0 bf16
+    int rows;             // rows of the call
+    int m;                // Dw: rows of the piece; otherwise from the head
+    int n;                // columns of the product: piece (Stats, Grad) or D
+    int k;                // contraction: D (Stats, Grad) or piece (Dh); Dw: from the head
+    int v0;               // first vocabulary row of the piece
+    int group_m;          // m-blocks per raster group
+    int splits;           // Dh: runs of the contraction
+    int rows_pad;         // Dh: rows between two splits' partial sums
+    int accumulate;       // Dh: 1 add to the partial sums, 0 write them
+    // Stats, Grad: per row of the call (not of the gathered copy)
+    const int* rowmap;    // gathered row -> row
+    const int* ecol;      // [rows][top] ascending target columns, kNoCol behind the last
+    const float* eq;      // [rows][top] their probabilities; null: 1
+    float* zsel;          // Stats: [rows][top] logits at the targets
+    float2* part;         // Stats: [tile][part_ld] (maximum, sum of exponentials)
+    long long part_ld;
+    const float* lse;     // Grad
+    const float* rscale;  // Grad: g_t
+    int top;
+    float c2;             // log2(e) / tau
+};
+
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+    __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+}
+
+// Shared-memory descriptor of an MN-major operand tile written by TMA in
+// 64-column x 64-row boxes with 128-byte swizzle: atoms of 64 columns x 8 rows
+// (1024 bytes) follow each other down the contraction (stride-dimension
+// offset 1024), the next 64 columns start one box later (leading-dimension
+// offset 8192).
+__device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t smem_addr) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu);
+    d |= static_cast<uint64_t>(8192u >> 4) << 16;
+    d |= static_cast<uint64_t>(1024u >> 4) << 32;
+    d |= static_cast<uint64_t>(1u) << 46;
+    d |= static_cast<uint64_t>(2u) << 61;
+    return d;
+}
+
+// One TMEM column of the warp's 32 lanes.
+__device__ __forceinline__ float tmem_ld_col(uint32_t taddr) {
+    uint32_t r;
+    __syncwarp();
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
+    tmem_ld_wait();
+    return __uint_as_float(r);
+}
+
+// Adds a staged fp32 box to global memory (each element once per launch, so
+// the order of additions is the order of the launches).
+__device__ __forceinline__ void tma_reduce_add_2d(const void* tmap, uint32_t src, int32_t x, int32_t y) {
+    asm volatile(
+        "cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];"
+        ::"l"(reinterpret_cast<uint64_t>(tmap)), "r"(src), "r"(x), "r"(y)
+        : "memory");
+}
+
+// 2^x by the hardware's approximation (absolute error about 2^-22 of the
+// result): every use is a term of a sum of exponentials or a probability.
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// The reference point of a sum of exponentials: the maximum, or 0 where it is
+// infinite (all terms are then 0, or one is infinite, without a NaN from
+// inf - inf).
+__device__ __forceinline__ float finite_or_zero(float m) { return fabsf(m) == INFINITY ? 0.0f : m; }
+
+template <int kCtaGroup, int kOp>
+__global__ void __launch_bounds__(kThreads, 1)
+vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmA1,
+                  const __grid_constant__ CUtensorMap tmB0, const __grid_constant__ CUtensorMap tmB1,
+                  const __grid_constant__ CUtensorMap tmD, const Params p) {
+    using C = Cfg<kCtaGroup>;
+    constexpr int kStages = C::kStages;
+    constexpr bool kPair = kCtaGroup == 2;
+    constexpr bool kAMn = kOp == kDw;
+    constexpr bool kBMn = kOp == kDh || kOp == kDw;
+    constexpr int kBoxBytes = 64 * kBK * 2;  // an MN-major box
+
+    int* const status = &p.head->status;
+    // Launch contract: uniform across the grid, checked before any barrier.
+    if (blockDim.x != kThreads || blockDim.y != 1 || blockDim.z != 1 ||
+        (kPair && cluster_nctarank() != 2) || (gridDim.x % kCtaGroup) != 0) {
+        if (threadIdx.x == 0) report_status(status, B200_DEV_BAD_LAUNCH);
+        return;
+    }
+
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                               ~static_cast<uintptr_t>(1023));
+    const uint32_t sbase = smem_u32(smem);
+    const uint32_t full0 = sbase + C::kBarOffset;
+    const uint32_t empty0 = full0 + 8 * kStages;
+    const uint32_t tfull0 = empty0 + 8 * kStages;
+    const uint32_t tempty0 = tfull0 + 16;
+    const uint32_t qfull0 = tempty0 + 16;
+    const uint32_t qempty0 = qfull0 + 8 * kQueue;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kBarOffset + C::kBarCount * 8);
+    volatile int* ring = reinterpret_cast<volatile int*>(smem + C::kBarOffset + C::kBarCount * 8 + 16);
+    const uint32_t ring_addr = smem_u32(const_cast<int*>(ring));
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const uint32_t rank = kPair ? cluster_ctarank() : 0;
+    const int num_clusters = gridDim.x / kCtaGroup;
+    const int cluster = blockIdx.x / kCtaGroup;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(full0 + 8 * s, 1);
+            mbar_init(empty0 + 8 * s, 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(tfull0 + 8 * a, 1);
+            mbar_init(tempty0 + 8 * a, kEpiWarps * kCtaGroup);
+        }
+        // A queued tile id is read by the MMA issuer and 4 epilogue warps of the
+        // leader, and in pair mode also by the peer's producer and 4 epilogue warps.
+        for (int q = 0; q < kQueue; ++q) {
+            mbar_init(qfull0 + 8 * q, 1);
+            mbar_init(qempty0 + 8 * q, kPair ? 10 : 5);
+        }
+        fence_barrier_init();
+    }
+    if (warp == 0 && lane == 0) {
+        tma_prefetch_desc(&tmA0);
+        tma_prefetch_desc(&tmB0);
+        if (kOp != kStats) tma_prefetch_desc(&tmD);
+    }
+    if (warp == 1) {
+        tmem_alloc<kCtaGroup>(smem_u32(tmem_slot), kTmemCols);
+        tmem_relinquish<kCtaGroup>();
+    }
+    tc_fence_before();
+    if constexpr (kPair) cluster_sync(); else __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+    // Nothing in global memory is touched before the previous kernel is done.
+    griddep_wait();
+
+    const int n_rows = p.head->n_rows;
+    const bool compact = p.head->compact != 0;
+    // Of H, the gathered copy where rows were left out. Without a single row the
+    // products still run over one block of zero rows: dW is then written as zeros.
+    const CUtensorMap* tmA = ((kOp == kStats || kOp == kGrad) && compact) ? &tmA1 : &tmA0;
+    const CUtensorMap* tmB = (kOp == kDw && compact) ? &tmB1 : &tmB0;
+    const int m_ext = kOp == kDw ? p.m : (kOp == kStats ? n_rows : max(n_rows, 1));
+    const int k_ext = kOp == kDw ? max(n_rows, 1) : p.k;
+    const int num_m = (m_ext + C::kTileM - 1) / C::kTileM;
+    const int num_n = (p.n + kBN - 1) / kBN;
+    const int num_k = (k_ext + kBK - 1) / kBK;
+    const int tiles_mn = num_m * num_n;
+    const int num_tiles = kOp == kDh ? tiles_mn * p.splits : tiles_mn;
+
+    // Tile id -> blocks and k-slices. Groups of m-blocks walk all n-blocks, so
+    // the tiles in flight share rows of both operands in L2.
+    struct Tile {
+        int mb, nb, kb0, kb1, split;
+    };
+    auto tile_of = [&](int t) {
+        Tile w;
+        w.split = 0;
+        w.kb0 = 0;
+        w.kb1 = num_k;
+        if constexpr (kOp == kDh) {
+            w.split = t / tiles_mn;
+            t -= w.split * tiles_mn;
+            w.kb0 = static_cast<int>(static_cast<long long>(num_k) * w.split / p.splits);
+            w.kb1 = static_cast<int>(static_cast<long long>(num_k) * (w.split + 1) / p.splits);
+        }
+        const int per_group = p.group_m * num_n;
+        const int g = t / per_group;
+        const int first = g * p.group_m;
+        const int gsize = min(p.group_m, num_m - first);
+        const int r = t - g * per_group;
+        w.mb = first + r % gsize;
+        w.nb = r / gsize;
+        return w;
+    };
+    auto queue_wait = [&](uint32_t qs, uint32_t qph, int code) -> bool {
+        return mbar_wait<kPair>(qfull0 + 8 * qs, qph, status, p.timeout_ns, code);
+    };
+    auto queue_release = [&](uint32_t qs) {
+        if constexpr (kPair) mbar_arrive_cluster(mapa_shared(qempty0 + 8 * qs, 0));
+        else mbar_arrive(qempty0 + 8 * qs);
+    };
+
+    if (warp == 0) {
+        // ------------------------------------------------------------ producer
+        if (elect_one()) {
+            uint32_t stage = 0, phase = 0, qs = 0, qph = 0;
+            long long issued = 0;
+            bool ok = true;
+            // The first tile is the cluster's own number, later ones come from the
+            // launch-wide counter.
+            int next = cluster;
+            while (ok) {
+                int t;
+                if (rank == 0) {
+                    if (!mbar_wait(qempty0 + 8 * qs, qph ^ 1, status, p.timeout_ns,
+                                   B200_DEV_TIMEOUT_PRODUCER)) {
+                        break;
+                    }
+                    t = next;
+                    if (t >= num_tiles) {
+                        t = -1;
+                        __threadfence();
+                        if (atomicAdd(&p.head->counter[1], 1) == num_clusters - 1) {
+                            // Every cluster has made its last fetch: ready for the next launch.
+                            atomicExch(&p.head->counter[0], 0);
+                            atomicExch(&p.head->counter[1], 0);
+                        }
+                    }
+                    ring[qs] = t;
+                    if constexpr (kPair) {
+                        st_shared_cluster_u32(mapa_shared(ring_addr + 4 * qs, 1), static_cast<uint32_t>(t));
+                        mbar_arrive_cluster(mapa_shared(qfull0 + 8 * qs, 1));
+                    }
+                    mbar_arrive(qfull0 + 8 * qs);
+                } else {
+                    if (!queue_wait(qs, qph, B200_DEV_TIMEOUT_PRODUCER)) break;
+                    t = ring[qs];
+                    queue_release(qs);
+                }
+                if (++qs == kQueue) { qs = 0; qph ^= 1; }
+                if (t < 0) {
+                    griddep_launch_dependents();
+                    break;
+                }
+                const Tile w = tile_of(t);
+                const int a_m = w.mb * C::kTileM + static_cast<int>(rank) * kRowsPerCta;
+                const int b_n = w.nb * kBN + static_cast<int>(rank) * C::kBRows;
+                // The next tile id is fetched two ring depths before the last k-slice:
+                // early enough to hide the round trip, late enough that a fast cluster
+                // does not take two tiles while a slow one has none.
+                const int fetch_kb = max(w.kb0, w.kb1 - 2 * kStages);
+                if (rank == 0 && w.kb0 == w.kb1) next = atomicAdd(&p.head->counter[0], 1) + num_clusters;
+                for (int kb = w.kb0; kb < w.kb1; ++kb) {
+                    if (rank == 0 && kb == fetch_kb) next = atomicAdd(&p.head->counter[0], 1) + num_clusters;
+                    if (!mbar_wait(empty0 + 8 * stage, phase ^ 1, status, p.timeout_ns,
+                                   B200_DEV_TIMEOUT_PRODUCER)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t sa = sbase + stage * C::kStageBytes;
+                    const uint32_t sb = sa + C::kABytes;
+                    const uint32_t fb = full0 + 8 * stage;
+                    const uint32_t bar = kPair ? mapa_shared(fb, 0) : fb;
+                    if (rank == 0) mbar_arrive_expect_tx(fb, kCtaGroup * C::kStageBytes);
+                    auto load = [&](uint32_t dst, const CUtensorMap* map, int x, int y) {
+                        if constexpr (kPair) tma_load_2d_pair(dst, map, bar, x, y);
+                        else tma_load_2d(dst, map, bar, x, y);
+                    };
+                    const int kc = kb * kBK;
+                    if constexpr (kAMn) {
+#pragma unroll
+                        for (int i = 0; i < kRowsPerCta / 64; ++i)
+                            load(sa + i * kBoxBytes, tmA, a_m + 64 * i, kc);
+                    } else {
+                        load(sa, tmA, kc, a_m);
+                    }
+                    if constexpr (kBMn) {
+                        const int y = kOp == kDh ? p.v0 + kc : kc;
+#pragma unroll
+                        for (int i = 0; i < C::kBRows / 64; ++i)
+                            load(sb + i * kBoxBytes, tmB, b_n + 64 * i, y);
+                    } else {
+                        load(sb, tmB, kc, p.v0 + b_n);
+                    }
+                    ++issued;
+                    if (++stage == kStages) { stage = 0; phase ^= 1; }
+                }
+            }
+            if (status_failed(status) && rank == 0) {
+                // The launch is being abandoned: before this CTA (pair) exits, wait
+                // (bounded) for the loads it still has in flight into its ring.
+                const unsigned long long drain_ns = min(p.timeout_ns, 100000000ull);
+                for (int s = 0; s < kStages; ++s) {
+                    if (issued <= s) continue;
+                    const long long last = ((issued - 1 - s) / kStages) * kStages + s;
+                    mbar_wait(full0 + 8 * s, static_cast<uint32_t>((last / kStages) & 1), nullptr,
+                              drain_ns, 0);
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // --------------------------------------------------------- MMA issuer
+        if (rank == 0 && elect_one()) {
+            const uint32_t fmt = p.fp16 ? 0u : 1u;
+            const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((kAMn ? 1u : 0u) << 15) |
+                                   ((kBMn ? 1u : 0u) << 16) | ((kBN >> 3) << 17) |
+                                   (((kRowsPerCta * kCtaGroup) >> 4) << 24);
+            uint32_t stage = 0, phase = 0, unit = 0, qs = 0, qph = 0;
+            bool ok = true;
+            while (ok) {
+                if (!queue_wait(qs, qph, B200_DEV_TIMEOUT_MMA_FULL)) break;
+                const int t = ring[qs];
+                queue_release(qs);
+                if (++qs == kQueue) { qs = 0; qph ^= 1; }
+                if (t < 0) break;
+                const Tile w = tile_of(t);
+                if (w.kb0 == w.kb1) continue;
+                const uint32_t slot = unit & 1;
+                if (!mbar_wait<kPair>(tempty0 + 8 * slot, ((unit >> 1) & 1) ^ 1, status, p.timeout_ns,
+                                      B200_DEV_TIMEOUT_MMA_TMEM)) {
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t d_tmem = tmem_base + slot * kBN;
+                for (int kb = w.kb0; kb < w.kb1; ++kb) {
+                    if (!mbar_wait(full0 + 8 * stage, phase, status, p.timeout_ns,
+                                   B200_DEV_TIMEOUT_MMA_FULL)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t sa = sbase + stage * C::kStageBytes;
+                    const uint32_t sb = sa + C::kABytes;
+#pragma unroll
+                    for (int k = 0; k < kBK / 16; ++k) {
+                        // 16 elements down the contraction: 32 bytes inside a K-major row,
+                        // 16 rows of 128 bytes in an MN-major box.
+                        const uint64_t da = kAMn ? smem_desc_mn_sw128(sa + 2048 * k) : smem_desc_sw128(sa + 32 * k);
+                        const uint64_t db = kBMn ? smem_desc_mn_sw128(sb + 2048 * k) : smem_desc_sw128(sb + 32 * k);
+                        umma_bf16<kCtaGroup>(d_tmem, da, db, idesc, (kb != w.kb0 || k != 0) ? 1u : 0u);
+                    }
+                    const uint32_t eb = empty0 + 8 * stage;
+                    if constexpr (!kPair) {
+                        umma_commit<1>(eb);
+                    } else {
+                        umma_commit<2>(mapa_shared(eb, 0));
+                        umma_commit<2>(mapa_shared(eb, 1));
+                    }
+                    if (++stage == kStages) { stage = 0; phase ^= 1; }
+                }
+                if (!ok) break;
+                const uint32_t tb = tfull0 + 8 * slot;
+                if constexpr (!kPair) {
+                    umma_commit<1>(tb);
+                } else {
+                    umma_commit<2>(mapa_shared(tb, 0));
+                    umma_commit<2>(mapa_shared(tb, 1));
+                }
+                ++unit;
+            }
+        }
+        __syncwarp();
+    } else {
+        // ----------------------------------------------------------- epilogue
+        const int q = warp & 3;  // TMEM lane quadrant this warp may access
+        const uint32_t stage_buf0 = sbase + C::kEpiOffset + q * 2 * kEpiBufBytes;
+        uint32_t unit = 0, buf = 0, qs = 0, qph = 0;
+        const float alpha = kOp == kDw ? p.head->alpha : 1.0f;
+        while (true) {
+            // The warp leaves as a whole: what follows is warp-wide.
+            if (!__all_sync(0xffffffffu, queue_wait(qs, qph, B200_DEV_TIMEOUT_EPILOGUE))) break;
+            const int t = ring[qs];
+            __syncwarp();
+            if (lane == 0) queue_release(qs);
+            if (++qs == kQueue) { qs = 0; qph ^= 1; }
+            if (t < 0) break;
+            const Tile w = tile_of(t);
+            if (w.kb0 == w.kb1) continue;
+            const uint32_t slot = unit & 1;
+            const int row0 = w.mb * C::kTileM + static_cast<int>(rank) * kRowsPerCta + q * 32;
+            const int col0 = w.nb * kBN;
+            const uint32_t t_row = tmem_base + slot * kBN + (static_cast<uint32_t>(q * 32) << 16);
+
+            // The row's targets: position of the first one at or behind the tile's
+            // first column, and that column.
+            const int grow = row0 + lane;  // row of the products
+            const bool active = grow < n_rows;
+            int pos = 0, cur = kNoCol;
+            long long ebase = 0;
+            float rs = 0.0f, neg_lse2 = 0.0f;
+            auto col_at = [&](int i) { return i < p.top ? __ldg(p.ecol + ebase + i) : kNoCol; };
+            if constexpr (kOp == kStats || kOp == kGrad) {
+                if (active) {
+                    const int r = __ldg(p.rowmap + grow);
+                    ebase = static_cast<long long>(r) * p.top;
+                    if constexpr (kOp == kGrad) {
+                        rs = __ldg(p.rscale + r);
+                        neg_lse2 = -__ldg(p.lse + r) * kLog2e;
+                    }
+                    int hi = p.top;
+                    const int first = p.v0 + col0;
+                    while (pos < hi) {
+                        const int mid = (pos + hi) >> 1;
+                        if (__ldg(p.ecol + ebase + mid) < first) pos = mid + 1;
+                        else hi = mid;
+                    }
+                    cur = col_at(pos);
+                    if (cur != kNoCol) cur -= p.v0;
+                }
+            }
+            auto advance = [&]() {
+                ++pos;
+                cur = col_at(pos);
+                if (cur != kNoCol) cur -= p.v0;
+            };
+
+            if (!__all_sync(0xffffffffu, mbar_wait<kPair, true>(tfull0 + 8 * slot, (unit >> 1) & 1, status,
+                                                                p.timeout_ns, B200_DEV_TIMEOUT_EPILOGUE))) {
+                break;
+            }
+            ++unit;
+            tc_fence_after();
+            auto release_tmem = [&]() {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if constexpr (!kPair) mbar_arrive(tempty0 + 8 * slot);
+                    else mbar_arrive_cluster(mapa_shared(tempty0 + 8 * slot, 0));
+                }
+            };
+
+            if constexpr (kOp == kStats) {
+                float m = -INFINITY, s = 0.0f;
+#pragma unroll 1
+                for (int c = 0; c < kBN / 32; ++c) {
+                    const int left = p.n - (col0 + c * 32);  // columns of the vocabulary in this chunk
+                    if (left <= 0) break;
+                    uint32_t r[32];
+                    tmem_ld_32x32b_x32(t_row + c * 32, r);
+                    tmem_ld_wait();
+                    if (left < 32) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (i >= left) r[i] = __float_as_uint(-INFINITY);
+                    }
+                    float mx = m;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(r[i]));
+                    const float ref = -finite_or_zero(mx) * p.c2;
+                    s *= exp2_approx(fmaf(finite_or_zero(m), p.c2, ref));
+                    float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        s0 += exp2_approx(fmaf(__uint_as_float(r[i]), p.c2, ref));
+                        s1 += exp2_approx(fmaf(__uint_as_float(r[i + 1]), p.c2, ref));
+                    }
+                    s += s0 + s1;
+                    m = mx;
+                    // Logits at the targets: all lanes read the column, the lanes that
+                    // want it keep it.
+                    while (true) {
+                        const int col = __reduce_min_sync(0xffffffffu, cur);
+                        if (col >= col0 + (c + 1) * 32) break;
+                        const float z = tmem_ld_col(t_row + (col - col0));
+                        if (cur == col) {
+                            p.zsel[ebase + pos] = z;
+                            advance();
+                        }
+                    }
+                }
+                release_tmem();
+                if (active) p.part[static_cast<long long>(w.nb) * p.part_ld + grow] = make_float2(m, s);
+            } else if constexpr (kOp == kGrad) {
+#pragma unroll 1
+                for (int c = 0; c < kBN / 64; ++c) {
+                    uint32_t r0[32], r1[32], pk[32];
+                    tmem_ld_32x32b_x32(t_row + c * 64, r0);
+                    tmem_ld_32x32b_x32(t_row + c * 64 + 32, r1);
+                    tmem_ld_wait();
+                    const int left = p.n - (col0 + c * 64);
+                    auto grad = [&](uint32_t z, int i) {
+                        const float g = rs * exp2_approx(fmaf(__uint_as_float(z), p.c2, neg_lse2));
+                        // Rows and columns beyond the ends are zeros of the products that
+                        // contract over them, whatever the accumulator holds.
+                        return active && i < left ? g : 0.0f;
+                    };
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float a0 = grad(r0[2 * i], 2 * i), a1 = grad(r0[2 * i + 1], 2 * i + 1);
+                        const float b0 = grad(r1[2 * i], 32 + 2 * i), b1 = grad(r1[2 * i + 1], 33 + 2 * i);
+                        pk[i] = p.fp16 ? pack_half2(a0, a1) : pack_bf16x2(a0, a1);
+                        pk[16 + i] = p.fp16 ? pack_half2(b0, b1) : pack_bf16x2(b0, b1);
+                    }
+                    if (row0 >= p.rows) {  // nothing of the call in these rows
+                        if (c == kBN / 64 - 1) release_tmem();
+                        continue;
+                    }
+                    const uint32_t sbuf = stage_buf0 + buf * kEpiBufBytes;
+                    if (lane == 0) bulk_wait_group_read<1>();
+                    __syncwarp();
+                    const uint32_t row_addr = sbuf + lane * 128;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        st_shared_v4(row_addr + ((j ^ (lane & 7)) << 4), pk[4 * j], pk[4 * j + 1],
+                                     pk[4 * j + 2], pk[4 * j + 3]);
+                    }
+                    // The targets' columns again, from the unrounded logit: p - q.
+                    while (true) {
+                        const int col = __reduce_min_sync(0xffffffffu, cur);
+                        if (col >= col0 + (c + 1) * 64) break;
+                        const float z = tmem_ld_col(t_row + (col - col0));
+                        if (cur == col) {
+                            const float qv = p.eq == nullptr ? 1.0f : __ldg(p.eq + ebase + pos);
+                            const float g = rs * (exp2_approx(fmaf(z, p.c2, neg_lse2)) - qv);
+                            const uint32_t bits = p.fp16 ? pack_half2(g, 0.0f) : pack_bf16x2(g, 0.0f);
+                            const int i = col - col0 - c * 64;
+                            asm volatile("st.shared.u16 [%0], %1;"
+                                         ::"r"(row_addr + (((i >> 3) ^ (lane & 7)) << 4) + (i & 7) * 2),
+                                         "h"(static_cast<uint16_t>(bits & 0xffffu)) : "memory");
+                            advance();
+                        }
+                    }
+                    if (c == kBN / 64 - 1) release_tmem();
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tma_store_2d(&tmD, sbuf, col0 + c * 64, row0);
+                        bulk_commit_group();
+                    }
+                    buf ^= 1;
+                }
+            } else if constexpr (kOp == kDh) {
+#pragma unroll 1
+                for (int c = 0; c < kBN / 32; ++c) {
+                    uint32_t r[32];
+                    tmem_ld_32x32b_x32(t_row + c * 32, r);
+                    tmem_ld_wait();
+                    if (c == kBN / 32 - 1) release_tmem();
+                    const int col = col0 + c * 32;
+                    if (col >= p.n) continue;
+                    const uint32_t sbuf = stage_buf0 + buf * kEpiBufBytes;
+                    if (lane == 0) bulk_wait_group_read<1>();
+                    __syncwarp();
+                    const uint32_t row_addr = sbuf + lane * 128;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        st_shared_v4(row_addr + ((j ^ (lane & 7)) << 4), r[4 * j], r[4 * j + 1],
+                                     r[4 * j + 2], r[4 * j + 3]);
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        const int y = w.split * p.rows_pad + row0;
+                        if (p.accumulate) tma_reduce_add_2d(&tmD, sbuf, col, y);
+                        else tma_store_2d(&tmD, sbuf, col, y);
+                        bulk_commit_group();
+                    }
+                    buf ^= 1;
+                }
+            } else {
+#pragma unroll 1
+                for (int c = 0; c < kBN / 64; ++c) {
+                    uint32_t r0[32], r1[32], pk[32];
+                    tmem_ld_32x32b_x32(t_row + c * 64, r0);
+                    tmem_ld_32x32b_x32(t_row + c * 64 + 32, r1);
+                    tmem_ld_wait();
+                    if (c == kBN / 64 - 1) release_tmem();
+                    const int col = col0 + c * 64;
+                    if (col >= p.n || row0 >= p.m) continue;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float a0 = alpha * __uint_as_float(r0[2 * i]), a1 = alpha * __uint_as_float(r0[2 * i + 1]);
+                        const float b0 = alpha * __uint_as_float(r1[2 * i]), b1 = alpha * __uint_as_float(r1[2 * i + 1]);
+                        pk[i] = p.fp16 ? pack_half2(a0, a1) : pack_bf16x2(a0, a1);
+                        pk[16 + i] = p.fp16 ? pack_half2(b0, b1) : pack_bf16x2(b0, b1);
+                    }
+                    const uint32_t sbuf = stage_buf0 + buf * kEpiBufBytes;
+                    if (lane == 0) bulk_wait_group_read<1>();
+                    __syncwarp();
+                    const uint32_t row_addr = sbuf + lane * 128;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        st_shared_v4(row_addr + ((j ^ (lane & 7)) << 4), pk[4 * j], pk[4 * j + 1],
+                                     pk[4 * j + 2], pk[4 * j + 3]);
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tma_store_2d(&tmD, sbuf, col, p.v0 + row0);
+                        bulk_commit_group();
+                    }
+                    buf ^= 1;
+                }
+            }
+        }
+        if (lane == 0) bulk_wait_group<0>();
+        __syncwarp();
+    }
+
+    // Teardown: every role is done with TMEM and with the peer's barriers.
+    tc_fence_before();
+    if constexpr (kPair) cluster_sync(); else __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc<kCtaGroup>(tmem_base, kTmemCols);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Rows, targets, teachers
+// ---------------------------------------------------------------------------
+enum RowFlag { kNoLoss = 0, kLoss = 1, kBad = 2 };  // kBad: a target outside the vocabulary
+
+__device__ __forceinline__ long long index_at(const void* idx, int bytes, long long i) {
+    return bytes == 8 ? __ldg(static_cast<const long long*>(idx) + i)
+                      : static_cast<long long>(__ldg(static_cast<const int*>(idx) + i));
+}
+
+__device__ __forceinline__ float teacher_at(const void* t, int dtype, long long i) {
+    if (dtype == B200_VL_F32) return __ldg(static_cast<const float*>(t) + i);
+    const unsigned short u = __ldg(static_cast<const unsigned short*>(t) + i);
+    if (dtype == B200_VL_BF16) return __uint_as_float(static_cast<uint32_t>(u) << 16);
+    return __half2float(__ushort_as_half(u));
+}
+
+struct TeacherParams {
+    const void* index;
+    const void* teacher;
+    int index_bytes, teacher_dtype;
+    long long ld_index, ld_teacher;
+    int rows, vocab, top;
+    float inv_tau;
+    int* ecol;
+    float* eq;
+    int* flag;
+};
+
+// A warp turns one row of a teacher's logits into its target distribution:
+// softmax over the entries that are there, sorted by column, entries of one
+// column added up in the order given. 2 x 8 bytes per entry in, 8 out.
+constexpr int kTeacherWarps = 8;
+__global__ void __launch_bounds__(kTeacherWarps * 32) teacher_kernel(const TeacherParams p, int pad) {
+    extern __shared__ unsigned long long teacher_smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    unsigned long long* key = teacher_smem + static_cast<size_t>(warp) * pad;
+    float* prob = reinterpret_cast<float*>(teacher_smem + static_cast<size_t>(kTeacherWarps) * pad) +
+                  static_cast<size_t>(warp) * pad;
+    const int t = blockIdx.x * kTeacherWarps + warp;
+    if (t >= p.rows) return;
+    float mx = -INFINITY;
+    bool any = false, bad = false, nan = false;
+    for (int k = lane; k < pad; k += 32) {
+        float l = -INFINITY;
+        unsigned col = kNoCol;
+        if (k < p.top) {
+            const long long c = index_at(p.index, p.index_bytes, t * p.ld_index + k);
+            if (c >= p.vocab) bad = true;
+            else if (c >= 0) {
+                l = teacher_at(p.teacher, p.teacher_dtype, t * p.ld_teacher + k) * p.inv_tau;
+                if (l != -INFINITY) {
+                    col = static_cast<unsigned>(c);
+                    any = true;
+                    if (!(l < INFINITY)) nan = true;  // NaN or +inf: no distribution
+                }
+            }
+        }
+        key[k] = (static_cast<unsigned long long>(col) << 32) | static_cast<unsigned>(k);
+        prob[k] = l;
+        mx = fmaxf(mx, l);
+    }
+    any = __any_sync(0xffffffffu, any);
+    bad = __any_sync(0xffffffffu, bad);
+    nan = __any_sync(0xffffffffu, nan);
+    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    float sum = 0.0f;
+    for (int k = lane; k < pad; k += 32) {
+        const float e = prob[k] == -INFINITY ? 0.0f : expf(prob[k] - mx);
+        prob[k] = e;
+        sum += e;
+    }
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const float inv = nan ? NAN : 1.0f / sum;
+    __syncwarp();
+    // Bitonic sort of (column, position).
+    for (int size = 2; size <= pad; size <<= 1) {
+        for (int stride = size >> 1; stride; stride >>= 1) {
+            for (int i = lane; i < pad / 2; i += 32) {
+                const int lo = 2 * i - (i & (stride - 1));
+                const int hi = lo + stride;
+                const unsigned long long a = key[lo], b = key[hi];
+                if ((a > b) == ((lo & size) == 0)) {
+                    key[lo] = b;
+                    key[hi] = a;
+                }
+            }
+            __syncwarp();
+        }
+    }
+    int out = 0;
+    int* ecol = p.ecol + static_cast<long long>(t) * p.top;
+    float* eq = p.eq + static_cast<long long>(t) * p.top;
+    for (int base = 0; base < pad; base += 32) {
+        const int i = base + lane;
+        unsigned col = kNoCol;
+        bool first = false;
+        if (i < pad) {
+            col = static_cast<unsigned>(key[i] >> 32);
+            first = col != kNoCol && (i == 0 || static_cast<unsigned>(key[i - 1] >> 32) != col);
+        }
+        const unsigned heads = __ballot_sync(0xffffffffu, first);
+        if (first) {
+            float v = 0.0f;
+            for (int j = i; j < pad && static_cast<unsigned>(key[j] >> 32) == col; ++j)
+                v += prob[static_cast<unsigned>(key[j])];
+            const int o = out + __popc(heads & ((1u << lane) - 1));
+            ecol[o] = static_cast<int>(col);
+            eq[o] = v * inv;
+        }
+        out += __popc(heads);
+    }
+    for (int i = out + lane; i < p.top; i += 32) {
+        ecol[i] = kNoCol;
+        eq[i] = 0.0f;
+    }
+    if (lane == 0) p.flag[t] = bad ? kBad : (any ? kLoss : kNoLoss);
+}
+
+struct RowsParams {
+    Head* head;
+    const void* target;   // cross entropy; null: the flags are the teachers'
+    int index_bytes;
+    long long ignore;
+    int rows, vocab;
+    int gather;           // 0: the products run over all rows
+    int reduction;
+    int* flag;
+    int* ecol;            // cross entropy: written here
+    int* rowmap;
+    int* inv;             // row -> gathered row, -1 without a loss
+    const float* grad;    // backward: what comes from above
+    float* rscale;
+    float tau;
+};
+
+// One block numbers the rows that have a loss, in order, and leaves the
+// factors of the backward pass. 1024 rows per step.
+__global__ void __launch_bounds__(1024) rows_kernel(const RowsParams p) {
+    __shared__ int warp_sum[32];
+    __shared__ float warp_max[32];
+    __shared__ int base;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) base = 0;
+    float gmax = 0.0f;
+    __syncthreads();
+    for (int r0 = 0; r0 < p.rows; r0 += 1024) {
+        const int t = r0 + tid;
+        int f = kNoLoss;
+        if (t < p.rows) {
+            if (p.target != nullptr) {
+                const long long c = index_at(p.target, p.index_bytes, t);
+                f = c == p.ignore ? kNoLoss : (c >= 0 && c < p.vocab ? kLoss : kBad);
+                p.ecol[t] = f == kLoss ? static_cast<int>(c) : kNoCol;
+                p.flag[t] = f;
+            } else {
+                f = p.flag[t];
+            }
+        }
+        const bool in = f != kNoLoss;
+        const unsigned b = __ballot_sync(0xffffffffu, in);
+        if (lane == 0) warp_sum[warp] = __popc(b);
+        __syncthreads();
+        if (warp == 0) {
+            int v = warp_sum[lane];
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, v, o);
+                if (lane >= o) v += u;
+            }
+            warp_sum[lane] = v;
+        }
+        __syncthreads();
+        const int at = base + (warp ? warp_sum[warp - 1] : 0) + __popc(b & ((1u << lane) - 1));
+        if (t < p.rows) {
+            p.inv[t] = in ? (p.gather ? at : t) : -1;
+            if (!p.gather) p.rowmap[t] = t;
+            else if (in) p.rowmap[at] = t;
+            if (p.rscale != nullptr && in && p.reduction == B200_VL_NONE) {
+                const float g = fabsf(p.grad[t]);
+                gmax = g > gmax || g != g ? g : gmax;  // a NaN stays
+            }
+        }
+        __syncthreads();
+        if (tid == 0) base += warp_sum[31];
+        __syncthreads();
+    }
+    const int n_valid = base;
+    if (p.rscale != nullptr && p.reduction == B200_VL_NONE) {
+        for (int o = 16; o; o >>= 1) {
+            const float u = __shfl_xor_sync(0xffffffffu, gmax, o);
+            gmax = u > gmax || u != u ? u : gmax;
+        }
+        if (lane == 0) warp_max[warp] = gmax;
+        __syncthreads();
+        for (int i = 0; i < 32; ++i) gmax = warp_max[i] > gmax || warp_max[i] != warp_max[i] ? warp_max[i] : gmax;
+    }
+    if (p.rscale != nullptr) {
+        const float unit = gmax > 0.0f ? gmax : 1.0f;
+        for (int t = tid; t < p.rows; t += 1024) {
+            const float g = p.reduction == B200_VL_NONE ? p.grad[t] / unit : 1.0f;
+            p.rscale[t] = p.flag[t] == kBad ? NAN : g;
+        }
+    }
+    if (tid == 0) {
+        Head h;
+        h.status = 0;
+        h.counter[0] = h.counter[1] = 0;
+        h.ticket = 0;
+        h.n_valid = n_valid;
+        h.n_rows = p.gather ? n_valid : p.rows;
+        h.compact = h.n_rows != p.rows;
+        h.alpha = 1.0f;
+        if (p.rscale != nullptr) {
+            if (p.reduction == B200_VL_NONE) h.alpha = gmax > 0.0f || gmax != gmax ? gmax * p.tau : p.tau;
+            else h.alpha = p.grad[0] * p.tau / (p.reduction == B200_VL_MEAN ? static_cast<float>(max(n_valid, 1)) : 1.0f);
+        }
+        *p.head = h;
+    }
+    griddep_launch_dependents();
+}
+
+// Gathers the rows that have a loss; a block of rows of zeros follows the last
+// one. Nothing to do where every row has one.
+__global__ void __launch_bounds__(256) gather_kernel(const Head* head, const int* rowmap, const uint4* src,
+                                                     long long ld, uint4* dst, int rows, int vecs) {
+    griddep_wait();
+    griddep_launch_dependents();
+    if (!head->compact) return;
+    const int n = head->n_rows;
+    const int end = min(rows, (max(n, 1) + 255) / 256 * 256);
+    for (int i = blockIdx.x; i < end; i += gridDim.x) {
+        const uint4* s = i < n ? src + rowmap[i] * ld : nullptr;
+        uint4* d = dst + static_cast<long long>(i) * vecs;
+        for (int v = threadIdx.x; v < vecs; v += 256) d[v] = s != nullptr ? __ldg(s + v) : make_uint4(0, 0, 0, 0);
+    }
+}
+
+struct MergeParams {
+    Head* head;
+    const float2* part;
+    long long part_ld;
+    int tiles, rows, top, reduction;
+    const int* inv;
+    const int* flag;
+    const float* eq;
+    const float* zsel;
+    float c2, inv_tau, tau2;
+    float* lse;
+    float* row_loss;   // reduction none: the result
+    float* loss;
+};
+
+// 32 rows per block: eight warps take an eighth of the tiles each (lane = row,
+// so the reads are contiguous), join in order, then a warp forms four rows'
+// losses. The last block to finish adds the rows in order.
+__global__ void __launch_bounds__(256) merge_kernel(const MergeParams p) {
+    __shared__ float sm[8][32], ss[8][32], slse[32];
+    __shared__ double sums[8];
+    __shared__ int last;
+    griddep_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int t0 = blockIdx.x * 32;
+    const int t = t0 + lane;
+    const int i = t < p.rows ? p.inv[t] : -1;
+    float m = -INFINITY, s = 0.0f;
+    if (i >= 0) {
+        const int b = p.tiles * warp / 8, e = p.tiles * (warp + 1) / 8;
+#pragma unroll 4
+        for (int j = b; j < e; ++j) {
+            const float2 v = p.part[j * p.part_ld + i];
+            const float mx = fmaxf(m, v.x);
+            const float ref = -finite_or_zero(mx) * p.c2;
+            s = s * exp2_approx(fmaf(finite_or_zero(m), p.c2, ref)) + v.y * exp2_approx(fmaf(finite_or_zero(v.x), p.c2, ref));
+            m = mx;
+        }
+    }
+    sm[warp][lane] = m;
+    ss[warp][lane] = s;
+    __syncthreads();
+    if (warp == 0) {
+        for (int w = 1; w < 8; ++w) {
+            const float mx = fmaxf(m, sm[w][lane]);
+            const float ref = -finite_or_zero(mx) * p.c2;
+            s = s * exp2_approx(fmaf(finite_or_zero(m), p.c2, ref)) + ss[w][lane] * exp2_approx(fmaf(finite_or_zero(sm[w][lane]), p.c2, ref));
+            m = mx;
+        }
+        const float l = i >= 0 ? logf(s) + finite_or_zero(m) * p.inv_tau : 0.0f;
+        slse[lane] = l;
+        if (t < p.rows) p.lse[t] = l;
+    }
+    __syncthreads();
+    const bool failed = p.head->status != 0;
+    for (int r = warp; r < 32 && t0 + r < p.rows; r += 8) {
+        const int row = t0 + r;
+        const int f = p.flag[row];
+        float v = 0.0f;
+        if (f == kLoss) {
+            const long long e = static_cast<long long>(row) * p.top;
+            for (int k = lane; k < p.top; k += 32) {
+                const float qv = p.eq == nullptr ? 1.0f : p.eq[e + k];
+                if (qv != 0.0f) v += qv * ((p.eq == nullptr ? 0.0f : logf(qv)) + (slse[r] - p.zsel[e + k] * p.inv_tau));
+            }
+            for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+            v *= p.tau2;
+        }
+        // A target outside the vocabulary, or a launch that was given up, is no number.
+        if (f == kBad || failed) v = NAN;
+        if (lane == 0) p.row_loss[row] = v;
+    }
+    if (p.reduction == B200_VL_NONE) return;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) last = atomicAdd(&p.head->ticket, 1) == static_cast<int>(gridDim.x) - 1;
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    // In 64 bits: the sum over many rows keeps the rows' own precision.
+    double sum = 0.0;
+    for (int r = threadIdx.x; r < p.rows; r += 256) sum += static_cast<double>(__ldcg(p.row_loss + r));
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) sums[warp] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 8; ++w) sum += sums[w];
+        if (p.reduction == B200_VL_MEAN) sum /= max(p.head->n_valid, 1);
+        *p.loss = static_cast<float>(sum);
+    }
+}
+
+struct FinishParams {
+    const Head* head;
+    const int* inv;
+    const float* part;    // [splits][rows_pad][hidden]
+    long long split_stride;
+    int splits, rows, hidden, vocab, fp16;
+    void* d_hidden;
+    void* d_weight;
+};
+
+// dH: adds the splits in order, applies the common factor, rounds, and puts the
+// rows back in their places; rows without a loss get zeros. 4 bytes read per
+// split and 2 written for each element.
+__global__ void __launch_bounds__(256) finish_kernel(const FinishParams p) {
+    griddep_wait();
+    const bool failed = p.head->status != 0;
+    const float alpha = p.head->alpha;
+    const int vecs = p.hidden / 8;
+    if (p.d_hidden != nullptr) {
+        for (int t = blockIdx.x; t < p.rows; t += gridDim.x) {
+            const int i = p.inv[t];
+            uint4* out = static_cast<uint4*>(p.d_hidden) + static_cast<long long>(t) * vecs;
+            for (int v = threadIdx.x; v < vecs; v += 256) {
+                float x[8] = {};
+                if (i >= 0) {
+                    const float* src = p.part + static_cast<long long>(i) * p.hidden + v * 8;
+                    for (int s = 0; s < p.splits; ++s) {
+                        const float4 a = __ldcs(reinterpret_cast<const float4*>(src + s * p.split_stride));
+                        const float4 b = __ldcs(reinterpret_cast<const float4*>(src + s * p.split_stride) + 1);
+                        x[0] += a.x; x[1] += a.y; x[2] += a.z; x[3] += a.w;
+                        x[4] += b.x; x[5] += b.y; x[6] += b.z; x[7] += b.w;
+                    }
+                }
+                uint32_t o[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float lo = failed ? NAN : (i >= 0 ? alpha * x[2 * j] : 0.0f);
+                    const float hi = failed ? NAN : (i >= 0 ? alpha * x[2 * j + 1] : 0.0f);
+                    o[j] = p.fp16 ? pack_half2(lo, hi) : pack_bf16x2(lo, hi);
+                }
+                out[v] = make_uint4(o[0], o[1], o[2], o[3]);
+            }
+        }
+    }
+    if (failed && p.d_weight != nullptr) {
+        // Never a silent half of a gradient: a launch that was given up leaves NaN.
+        const long long n = static_cast<long long>(p.vocab) * vecs;
+        const uint4 nan4 = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+        for (long long v = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; v < n; v += static_cast<long long>(gridDim.x) * 256)
+            static_cast<uint4*>(p.d_weight)[v] = nan4;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+static int64_t align_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
+
+// Room for G: this, or as much as H itself takes (one 256-column block at least).
+constexpr int64_t kPieceBytes = int64_t(256) << 20;
+constexpr int64_t kPartialBytes = int64_t(256) << 20;
+
+struct Layout {
+    int cta_group;
+    int64_t tile_m, piece, pieces, splits, rows_pad;
+    int64_t n_tiles;
+    // Offsets in the workspace.
+    int64_t flag, rowmap, inv, ecol, eq;                 // both directions
+    int64_t zsel, part, row_loss, gathered_forward;
+    int64_t rscale, gathered_backward, g, partial;
+    int64_t bytes_forward, bytes_backward;
+    bool gather_forward;
+};
+
+static int check_desc(const B200VocabLossDesc* d) {
+    if (d == nullptr) {
+        set_error("desc must not be NULL");
+        return B200_ERR_INVALID_ARGUMENT;
+    }
+    const int64_t kMax = (int64_t(1) << 31) - 1;
+    if (d->rows < 0 || d->vocab < 1 || d->hidden < 1) {
+        set_error("(rows,vocab,hidden)=(%lld,%lld,%lld): rows must be >= 0, vocab and hidden >= 1",
+                  (long long)d->rows, (long long)d->vocab, (long long)d->hidden);
+        return B200_ERR_INVALID_ARGUMENT;
+    }
+    // Tile arithmetic is in 32 bits: leave room for a block behind the end.
+    if (d->rows > kMax - 1024 || d->vocab > kMax - 1024 || d->hidden > kMax - 1024) {
+        set_error("(rows,vocab,hidden)=(%lld,%lld,%lld): every extent must be below 2^31 - 1024",
+                  (long long)d->rows, (long long)d->vocab, (long long)d->hidden);
+        return B200_ERR_UNSUPPORTED;
+    }
+    if (d->hidden % 8 != 0) {
+        set_error("hidden=%lld: rows must be whole 16-byte units for TMA (hidden %% 8 == 0)", (long long)d->hidden);
+        return B200_ERR_UNSUPPORTED;
+    }
+    if (d->dtype != B200_VL_BF16 && d->dtype != B200_VL_F16) {
+        set_error("dtype=%lld is neither B200_VL_BF16 nor B200_VL_F16", (long long)d->dtype);
+        return B200_ERR_INVALID_ARGUMENT;
+    }
+    if (d->ld_hidden < d->hidden || d->ld_weight < d->hidden) {
+        set_error("row pitches %lld, %lld are smaller than hidden=%lld", (long long)d->ld_hidden,
+                  (long long)d->ld_weight, (long long)d->hidden);
+        return B200_ERR_INVALID_ARGUMENT;
+    }
+    if (d->ld_hidden % 8 != 0 || d->ld_weight % 8 != 0) {
+        set_error("row pitches %lld, %lld must be multiples of 8 elements (16 bytes)", (long long)d->ld_hidden,
+                  (long long)d->ld_weight);
+        return B200_ERR_UNSUPPORTED;
+    }
+    if (d->index_bytes != 4 && d->index_bytes != 8) {
+        set_error("index_bytes=%lld is neither 4 nor 8", (long long)d->index_bytes);
+        return B200_ERR_INVALID_ARGUMENT;
+    }
+    if (d->reduction != B200_VL_NONE && d->reduction != B200_VL_MEAN && d->reduction != B200_VL_SUM) {
+        set_error("reduction=%lld is not one of NONE(0), MEAN(1), SUM(2)", (long long)d->reduction);
+        return B200_ERR_INVALID_ARGUMENT;
+    }
+    if (d->top < 0 || d->top > kMaxTop) {
+        set_error("top=%lld: a teacher's row holds 1 to %d logits (0: cross entropy)", (long long)d->top, kMaxTop);
+        return B200_ERR_UNSUPPORTED;
+    }
+    if (d->top > 0) {
+        if (d->teacher_dtype != B200_VL_F32 && d->teacher_dtype != B200_VL_BF16 && d->teacher_dtype != B200_VL_F16) {
+            set_error("teacher_dtype=%lld is not one of BF16(0), F16(1), F32(2)", (long long)d->teacher_dtype);
+            return B200_ERR_INVALID_ARGUMENT;
+        }
+        if (d->ld_index < d->top || d->ld_teacher < d->top) {
+            set_error("row pitches %lld, %lld of the teacher are smaller than top=%lld", (long long)d->ld_index,
+                      (long long)d->ld_teacher, (long long)d->top);
+            return B200_ERR_INVALID_ARGUMENT;
+        }
+        if (!(d->temperature > 0.0) || !std::isfinite(d->temperature)) {
+            set_error("temperature=%g must be positive and finite", d->temperature);
+            return B200_ERR_INVALID_ARGUMENT;
+        }
+    } else if (d->temperature != 1.0) {
+        set_error("temperature=%g: the cross entropy has temperature 1", d->temperature);
+        return B200_ERR_INVALID_ARGUMENT;
+    }
+    return B200_OK;
+}
+
+// The host's choices for a call: a function of the sizes and the SM count alone.
+static Layout layout_for(const B200VocabLossDesc& d, int64_t sms) {
+    Layout l{};
+    const int64_t T = std::max<int64_t>(d.rows, 1), K = std::max<int64_t>(d.top, 1);
+    l.cta_group = T <= kRowsPerCta ? 1 : 2;
+    l.tile_m = kRowsPerCta * l.cta_group;
+    l.rows_pad = align_up(T, l.tile_m);
+    l.n_tiles = ceil_div(d.vocab, kBN);
+    l.gather_forward = T > kRowsPerCta;
+    const int64_t slots = std::max<int64_t>(sms / l.cta_group, 1), pairs = std::max<int64_t>(sms / 2, 1);
+    const int64_t mb = l.rows_pad / l.tile_m, nb = ceil_div(d.hidden, kBN);
+    const int64_t kd = ceil_div(d.hidden, kBK), kt = ceil_div(T, kBK);
+    // Piece of the vocabulary (in blocks of 256) and runs of dH's contraction: the
+    // least k-slices on the longest cluster, over the three products of all
+    // pieces, with eight k-slices for each launch's start and end. One piece where
+    // G has room; otherwise up to 64 widths between half the room and all of it.
+    // More than one run only where dH's tiles leave clusters idle.
+    const int64_t most = std::max<int64_t>(1, std::min(l.n_tiles, std::max(kPieceBytes, 2 * l.rows_pad * d.hidden) / (2 * kBN * l.rows_pad)));
+    const int64_t least = most == l.n_tiles ? most : std::max<int64_t>(1, most / 2);
+    const int64_t step = std::max<int64_t>(1, (most - least) / 64);
+    int64_t max_splits = 1;
+    if (mb * nb < 2 * slots)
+        max_splits = std::max<int64_t>(1, std::min<int64_t>(kMaxSplits, kPartialBytes / (4 * l.rows_pad * d.hidden)));
+    max_splits = std::min(max_splits, ceil_div(d.vocab, kBK));
+    int64_t best = -1;
+    for (int64_t b = least; b <= most; b += step) {
+        const int64_t pieces = ceil_div(l.n_tiles, b), rest = l.n_tiles - (pieces - 1) * b;
+        auto cost_of = [&](int64_t blocks, int64_t s) {
+            return ceil_div(mb * blocks, slots) * kd + ceil_div(blocks * nb, pairs) * kt +
+                   ceil_div(mb * nb * s, slots) * ceil_div(blocks * (kBN / kBK), s) + 24;
+        };
+        for (int64_t s = 1; s <= max_splits && s <= b * (kBN / kBK); ++s) {
+            const int64_t cost = (pieces - 1) * cost_of(b, s) + cost_of(rest, s) + 2 * (s - 1);
+            if (best < 0 || cost < best) {
+                best = cost;
+                l.piece = b * kBN;
+                l.pieces = pieces;
+                l.splits = s;
+            }
+        }
+    }
+    int64_t at = 256;
+    auto take = [&](int64_t bytes) {
+        const int64_t here = at;
+        at = align_up(at + bytes, 256);
+        return here;
+    };
+    l.flag = take(4 * T);
+    l.rowmap = take(4 * T);
+    l.inv = take(4 * T);
+    l.ecol = take(4 * T * K);
+    l.eq = take(d.top > 0 ? 4 * T * K : 0);
+    const int64_t common = at;
+    l.zsel = take(4 * T * K);
+    l.part = take(8 * l.n_tiles * T);
+    l.row_loss = take(4 * T);
+    l.gathered_forward = take(l.gather_forward ? 2 * T * d.hidden : 0);
+    l.bytes_forward = at;
+    at = common;
+    l.rscale = take(4 * T);
+    l.gathered_backward = take(2 * T * d.hidden);
+    l.g = take(2 * T * l.piece);
+    l.partial = take(4 * l.splits * l.rows_pad * d.hidden);
+    l.bytes_backward = at;
+    return l;
+}
+
+using KernelFn = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, Params);
+
+template <int G>
+static KernelFn kernel_of(int op) {
+    switch (op) {
+        case kStats: return vocab_gemm_kernel<G, kStats>;
+        case kGrad: return vocab_gemm_kernel<G, kGrad>;
+        case kDh: return vocab_gemm_kernel<G, kDh>;
+        default: return vocab_gemm_kernel<2, kDw>;
+    }
+}
+
+struct DeviceState {
+    bool ready = false;
+    int sms = 0;
+    int pairs = 0;
+};
+
+static int device_state(DeviceState* out) {
+    constexpr int kMaxDevices = 64;
+    static DeviceState cache[kMaxDevices];
+    static std::mutex mu;
+    int device = 0;
+    B200_CUDA_TRY(cudaGetDevice(&device));
+    // Binds the device's context to a thread that has not called the runtime yet
+    // (autograd's backward threads): the tensor maps are encoded by the driver.
+    B200_CUDA_TRY(cudaSetDevice(device));
+    DeviceProps props;
+    int rc = device_props(device, &props);
+    if (rc != B200_OK) return rc;
+    if (props.cc_major != 10 || props.cc_minor != 0) {
+        set_error("device %d has compute capability %d.%d; this library is built for sm_100a (10.0)", device,
+                  props.cc_major, props.cc_minor);
+        return B200_ERR_UNSUPPORTED;
+    }
+    std::lock_guard<std::mutex> lock(mu);
+    DeviceState& s = cache[device];
+    if (!s.ready) {
+        for (int op = 0; op < 4; ++op) {
+            const void* one = reinterpret_cast<const void*>(kernel_of<1>(op));
+            const void* two = reinterpret_cast<const void*>(kernel_of<2>(op));
+            if (op != kDw)
+                B200_CUDA_TRY(cudaFuncSetAttribute(one, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<1>::kSmemBytes));
+            B200_CUDA_TRY(cudaFuncSetAttribute(two, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<2>::kSmemBytes));
+        }
+        cudaLaunchConfig_t cfg = {};
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 2;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.gridDim = dim3(props.sm_count & ~1, 1, 1);
+        cfg.blockDim = dim3(kThreads, 1, 1);
+        cfg.dynamicSmemBytes = Cfg<2>::kSmemBytes;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        int clusters = 0;
+        const cudaError_t err = cudaOccupancyMaxActiveClusters(&clusters, reinterpret_cast<const void*>(kernel_of<2>(kStats)), &cfg);
+        if (err != cudaSuccess || clusters <= 0) {
+            cudaGetLastError();
+            clusters = props.sm_count / 2;
+        }
+        s.sms = props.sm_count;
+        s.pairs = std::max(clusters, 1);
+        s.ready = true;
+    }
+    *out = s;
+    return B200_OK;
+}
+
+// Launches that follow another kernel of the same call start their set-up while
+// it ends (programmatic dependent launch); each waits for it before it touches
+// global memory.
+template <typename... KArgs, typename... Args>
+static int launch(void (*fn)(KArgs...), int grid, int block, int smem, int cluster, bool dependent, cudaStream_t stream,
+                  Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (cluster > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = cluster;
+        attr[n].val.clusterDim.y = 1;
+        attr[n++].val.clusterDim.z = 1;
+    }
+    if (dependent) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    cfg.gridDim = dim3(grid, 1, 1);
+    cfg.blockDim = dim3(block, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = n;
+    B200_CUDA_TRY(cudaLaunchKernelEx(&cfg, fn, static_cast<KArgs>(args)...));
+    return B200_OK;
+}
+
+struct Call {
+    const B200VocabLossDesc* d;
+    Layout l;
+    DeviceState dev;
+    uint8_t* ws;
+    cudaStream_t stream;
+    CUtensorMapDataType type;
+    template <typename T>
+    T* at(int64_t offset) const { return reinterpret_cast<T*>(ws + offset); }
+    Head* head() const { return reinterpret_cast<Head*>(ws); }
+};
+
+static int check_pointers(std::initializer_list<std::pair<const void*, const char*>> ptrs) {
+    for (const auto& p : ptrs) {
+        if (p.first == nullptr) {
+            set_error("%s must be a device pointer", p.second);
+            return B200_ERR_INVALID_ARGUMENT;
+        }
+    }
+    return B200_OK;
+}
+
+static int check_aligned(std::initializer_list<std::pair<const void*, const char*>> ptrs) {
+    for (const auto& p : ptrs) {
+        if (reinterpret_cast<uintptr_t>(p.first) % 16 != 0) {
+            set_error("%s %p is not 16-byte aligned (TMA requirement)", p.second, p.first);
+            return B200_ERR_UNSUPPORTED;
+        }
+    }
+    return B200_OK;
+}
+
+static int map_2d(const Call& c, CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld,
+                  int box_rows, int box_cols) {
+    return encode_tmap_2d(map, c.type, 2, base, rows, cols, ld, box_rows, box_cols, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// Targets, row numbers and the gathered copy of H.
+static int launch_rows(const Call& c, const void* index, const void* teacher, const void* hidden, bool gather,
+                       int64_t gathered, const float* grad) {
+    const B200VocabLossDesc& d = *c.d;
+    const Layout& l = c.l;
+    if (d.top > 0) {
+        TeacherParams t{};
+        t.index = index;
+        t.teacher = teacher;
+        t.index_bytes = static_cast<int>(d.index_bytes);
+        t.teacher_dtype = static_cast<int>(d.teacher_dtype);
+        t.ld_index = d.ld_index;
+        t.ld_teacher = d.ld_teacher;
+        t.rows = static_cast<int>(d.rows);
+        t.vocab = static_cast<int>(d.vocab);
+        t.top = static_cast<int>(d.top);
+        t.inv_tau = static_cast<float>(1.0 / d.temperature);
+        t.ecol = c.at<int>(l.ecol);
+        t.eq = c.at<float>(l.eq);
+        t.flag = c.at<int>(l.flag);
+        int pad = 2;
+        while (pad < t.top) pad *= 2;
+        const int rc = launch(teacher_kernel, static_cast<int>(ceil_div(d.rows, kTeacherWarps)), kTeacherWarps * 32,
+                              kTeacherWarps * pad * 12, 1, false, c.stream, t, pad);
+        if (rc != B200_OK) return rc;
+    }
+    RowsParams r{};
+    r.head = c.head();
+    r.target = d.top > 0 ? nullptr : index;
+    r.index_bytes = static_cast<int>(d.index_bytes);
+    r.ignore = d.ignore_index;
+    r.rows = static_cast<int>(d.rows);
+    r.vocab = static_cast<int>(d.vocab);
+    r.gather = gather;
+    r.reduction = static_cast<int>(d.reduction);
+    r.flag = c.at<int>(l.flag);
+    r.ecol = c.at<int>(l.ecol);
+    r.rowmap = c.at<int>(l.rowmap);
+    r.inv = c.at<int>(l.inv);
+    r.grad = grad;
+    r.rscale = grad != nullptr ? c.at<float>(l.rscale) : nullptr;
+    r.tau = static_cast<float>(d.temperature);
+    int rc = launch(rows_kernel, 1, 1024, 0, 1, false, c.stream, r);
+    if (rc != B200_OK || !gather) return rc;
+    const int vecs = static_cast<int>(d.hidden / 8);
+    return launch(gather_kernel, static_cast<int>(std::min<int64_t>(d.rows, 8 * c.dev.sms)), 256, 0, 1, true, c.stream,
+                  static_cast<const Head*>(c.head()), static_cast<const int*>(c.at<int>(l.rowmap)),
+                  static_cast<const uint4*>(hidden), static_cast<long long>(d.ld_hidden / 8), c.at<uint4>(gathered),
+                  static_cast<int>(d.rows), vecs);
+}
+
+static Params base_params(const Call& c) {
+    const B200VocabLossDesc& d = *c.d;
+    Params p{};
+    p.head = c.head();
+    p.timeout_ns = wait_timeout_ns();
+    p.fp16 = d.dtype == B200_VL_F16;
+    p.rows = static_cast<int>(d.rows);
+    p.splits = 1;
+    p.rowmap = c.at<int>(c.l.rowmap);
+    p.ecol = c.at<int>(c.l.ecol);
+    p.eq = d.top > 0 ? c.at<float>(c.l.eq) : nullptr;
+    p.top = static_cast<int>(std::max<int64_t>(d.top, 1));
+    p.c2 = static_cast<float>(1.4426950408889634 / d.temperature);
+    return p;
+}
+
+// Raster groups of about 4096 rows of A whose panel stays within 64 MiB.
+static int group_for(int64_t tile_m, int64_t k) {
+    const double rows = std::min(4096.0, 64.0 * 1024 * 1024 / (2.0 * std::max<int64_t>(k, 64)));
+    return std::max(2, std::min(32, static_cast<int>(rows / tile_m + 0.5)));
+}
+
+static int launch_gemm(const Call& c, int op, int cta_group, int64_t tiles, const CUtensorMap& a0, const CUtensorMap& a1,
+                       const CUtensorMap& b0, const CUtensorMap& b1, const CUtensorMap& dmap, const Params& p) {
+    const int64_t slots = cta_group == 2 ? c.dev.pairs : c.dev.sms;
+    const int grid = static_cast<int>(std::max<int64_t>(1, std::min(tiles, slots))) * cta_group;
+    return launch(cta_group == 2 ? kernel_of<2>(op) : kernel_of<1>(op), grid, kThreads,
+                  cta_group == 2 ? Cfg<2>::kSmemBytes : Cfg<1>::kSmemBytes, cta_group, true, c.stream, a0, a1, b0, b1, dmap, p);
+}
+
+static int begin(const B200VocabLossDesc* d, void* workspace, int64_t bytes, bool backward, void* stream, Call* c) {
+    int rc = device_state(&c->dev);
+    if (rc != B200_OK) return rc;
+    c->d = d;
+    c->l = layout_for(*d, c->dev.sms);
+    c->ws = static_cast<uint8_t*>(workspace);
+    c->stream = static_cast<cudaStream_t>(stream);
+    c->type = d->dtype == B200_VL_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const int64_t need = backward ? c->l.bytes_backward : c->l.bytes_forward;
+    if (bytes < need) {
+        set_error("workspace of %lld bytes is smaller than the %lld needed", (long long)bytes, (long long)need);
+        return B200_ERR_INVALID_ARGUMENT;
+    }
+    if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0) {
+        set_error("workspace %p is not 256-byte aligned", workspace);
+        return B200_ERR_INVALID_ARGUMENT;
+    }
+    return B200_OK;
+}
+
+static int forward(const B200VocabLossDesc* d, const void* hidden, const void* weight, const void* index,
+                   const void* teacher, float* loss, float* lse, void* workspace, int64_t bytes, void* stream) {
+    int rc = check_desc(d);
+    if (rc != B200_OK) return rc;
+    if (d->rows == 0) {
+        set_error("rows=0: there is nothing to launch");
+        return B200_ERR_UNSUPPORTED;
+    }
+    rc = check_pointers({{hidden, "hidden"}, {weight, "weight"}, {index, "index"}, {loss, "loss"}, {lse, "lse"},
+                         {workspace, "workspace"}});
+    if (rc == B200_OK && d->top > 0) rc = check_pointers({{teacher, "teacher"}});
+    if (rc == B200_OK) rc = check_aligned({{hidden, "hidden"}, {weight, "weight"}});
+    if (rc != B200_OK) return rc;
+    Call c{};
+    rc = begin(d, workspace, bytes, false, stream, &c);
+    if (rc != B200_OK) return rc;
+    const Layout& l = c.l;
+    CUtensorMap a0, a1, b;
+    const int box_n = kBN / l.cta_group;
+    rc = map_2d(c, &a0, hidden, d->rows, d->hidden, d->ld_hidden, kRowsPerCta, kBK);
+    if (rc == B200_OK)
+        rc = l.gather_forward ? map_2d(c, &a1, c.at<void>(l.gathered_forward), d->rows, d->hidden, d->hidden, kRowsPerCta, kBK)
+                              : (a1 = a0, B200_OK);
+    if (rc == B200_OK) rc = map_2d(c, &b, weight, d->vocab, d->hidden, d->ld_weight, box_n, kBK);
+    if (rc != B200_OK) return rc;
+    rc = launch_rows(c, index, teacher, hidden, l.gather_forward, l.gathered_forward, nullptr);
+    if (rc != B200_OK) return rc;
+    Params p = base_params(c);
+    p.n = static_cast<int>(d->vocab);
+    p.k = static_cast<int>(d->hidden);
+    p.group_m = group_for(l.tile_m, d->hidden);
+    p.zsel = c.at<float>(l.zsel);
+    p.part = c.at<float2>(l.part);
+    p.part_ld = d->rows;
+    rc = launch_gemm(c, kStats, l.cta_group, l.rows_pad / l.tile_m * l.n_tiles, a0, a1, b, b, b, p);
+    if (rc != B200_OK) return rc;
+    MergeParams m{};
+    m.head = c.head();
+    m.part = p.part;
+    m.part_ld = p.part_ld;
+    m.tiles = static_cast<int>(l.n_tiles);
+    m.rows = static_cast<int>(d->rows);
+    m.top = p.top;
+    m.reduction = static_cast<int>(d->reduction);
+    m.inv = c.at<int>(l.inv);
+    m.flag = c.at<int>(l.flag);
+    m.eq = p.eq;
+    m.zsel = p.zsel;
+    m.c2 = p.c2;
+    m.inv_tau = static_cast<float>(1.0 / d->temperature);
+    m.tau2 = static_cast<float>(d->temperature * d->temperature);
+    m.lse = lse;
+    m.row_loss = d->reduction == B200_VL_NONE ? loss : c.at<float>(l.row_loss);
+    m.loss = loss;
+    return launch(merge_kernel, static_cast<int>(ceil_div(d->rows, 32)), 256, 0, 1, true, c.stream, m);
+}
+
+static int backward(const B200VocabLossDesc* d, const void* hidden, const void* weight, const void* index,
+                    const void* teacher, const float* lse, const float* grad_loss, void* d_hidden, void* d_weight,
+                    void* workspace, int64_t bytes, void* stream) {
+    int rc = check_desc(d);
+    if (rc != B200_OK) return rc;
+    if (d->rows == 0 || (d_hidden == nullptr && d_weight == nullptr)) {
+        set_error("rows=%lld with %s: there is nothing to launch", (long long)d->rows,
+                  d_hidden == nullptr && d_weight == nullptr ? "no gradient asked for" : "gradients to write");
+        return B200_ERR_UNSUPPORTED;
+    }
+    rc = check_pointers({{hidden, "hidden"}, {weight, "weight"}, {index, "index"}, {lse, "lse"},
+                         {grad_loss, "grad_loss"}, {workspace, "workspace"}});
+    if (rc == B200_OK && d->top > 0) rc = check_pointers({{teacher, "teacher"}});
+    if (rc == B200_OK)
+        rc = check_aligned({{hidden, "hidden"}, {weight, "weight"}, {d_hidden, "d_hidden"}, {d_weight, "d_weight"}});
+    if (rc != B200_OK) return rc;
+    Call c{};
+    rc = begin(d, workspace, bytes, true, stream, &c);
+    if (rc != B200_OK) return rc;
+    const Layout& l = c.l;
+    void* hg = c.at<void>(l.gathered_backward);
+    void* g = c.at<void>(l.g);
+    CUtensorMap h_k, hg_k, h_mn, hg_mn, w_k, w_mn, g_st, g_k, g_mn, part_st, dw_st;
+    std::memset(&part_st, 0, sizeof(part_st));
+    std::memset(&dw_st, 0, sizeof(dw_st));
+    const int64_t T = d->rows, V = d->vocab, D = d->hidden;
+    rc = map_2d(c, &h_k, hidden, T, D, d->ld_hidden, kRowsPerCta, kBK);
+    if (rc == B200_OK) rc = map_2d(c, &hg_k, hg, T, D, D, kRowsPerCta, kBK);
+    if (rc == B200_OK) rc = map_2d(c, &h_mn, hidden, T, D, d->ld_hidden, kBK, 64);
+    if (rc == B200_OK) rc = map_2d(c, &hg_mn, hg, T, D, D, kBK, 64);
+    if (rc == B200_OK) rc = map_2d(c, &w_k, weight, V, D, d->ld_weight, kBN / l.cta_group, kBK);
+    if (rc == B200_OK) rc = map_2d(c, &w_mn, weight, V, D, d->ld_weight, kBK, 64);
+    if (rc == B200_OK) rc = map_2d(c, &g_st, g, T, l.piece, l.piece, 32, 64);
+    if (rc == B200_OK) rc = map_2d(c, &g_k, g, T, l.piece, l.piece, kRowsPerCta, kBK);
+    if (rc == B200_OK) rc = map_2d(c, &g_mn, g, T, l.piece, l.piece, kBK, 64);
+    if (rc == B200_OK)
+        rc = encode_tmap_2d(&part_st, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, c.at<void>(l.partial), l.splits * l.rows_pad, D,
+                            D, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc == B200_OK && d_weight != nullptr) rc = map_2d(c, &dw_st, d_weight, V, D, D, 32, 64);
+    if (rc != B200_OK) return rc;
+    rc = launch_rows(c, index, teacher, hidden, true, l.gathered_backward, grad_loss);
+    for (int64_t v0 = 0; rc == B200_OK && v0 < V; v0 += l.piece) {
+        const int64_t vp = std::min(l.piece, V - v0);
+        Params p = base_params(c);
+        p.v0 = static_cast<int>(v0);
+        p.lse = lse;
+        p.rscale = c.at<float>(l.rscale);
+        p.n = static_cast<int>(vp);
+        p.k = static_cast<int>(D);
+        p.group_m = group_for(l.tile_m, D);
+        rc = launch_gemm(c, kGrad, l.cta_group, l.rows_pad / l.tile_m * ceil_div(vp, kBN), h_k, hg_k, w_k, w_k, g_st, p);
+        if (rc == B200_OK && d_hidden != nullptr) {
+            Params q = p;
+            q.n = static_cast<int>(D);
+            q.k = static_cast<int>(vp);
+            q.group_m = group_for(l.tile_m, l.piece);
+            q.splits = static_cast<int>(l.splits);
+            q.rows_pad = static_cast<int>(l.rows_pad);
+            q.accumulate = v0 > 0;
+            rc = launch_gemm(c, kDh, l.cta_group, l.rows_pad / l.tile_m * ceil_div(D, kBN) * l.splits, g_k, g_k, w_mn,
+                             w_mn, part_st, q);
+        }
+        if (rc == B200_OK && d_weight != nullptr) {
+            Params q = p;
+            q.m = static_cast<int>(vp);
+            q.n = static_cast<int>(D);
+            q.group_m = group_for(2 * kRowsPerCta, T);
+            rc = launch_gemm(c, kDw, 2, ceil_div(vp, 2 * kRowsPerCta) * ceil_div(D, kBN), g_mn, g_mn, h_mn, hg_mn, dw_st, q);
+        }
+    }
+    if (rc != B200_OK) return rc;
+    FinishParams f{};
+    f.head = c.head();
+    f.inv = c.at<int>(l.inv);
+    f.part = c.at<float>(l.partial);
+    f.split_stride = l.rows_pad * D;
+    f.splits = static_cast<int>(l.splits);
+    f.rows = static_cast<int>(T);
+    f.hidden = static_cast<int>(D);
+    f.vocab = static_cast<int>(V);
+    f.fp16 = d->dtype == B200_VL_F16;
+    f.d_hidden = d_hidden;
+    f.d_weight = d_weight;
+    return launch(finish_kernel, static_cast<int>(std::min<int64_t>(T, 8 * c.dev.sms)), 256, 0, 1, true, c.stream, f);
+}
+
+}  // namespace vl
+}  // namespace b200
+
+extern "C" {
+
+size_t b200_vocab_loss_desc_size(void) { return sizeof(B200VocabLossDesc); }
+size_t b200_vocab_loss_info_size(void) { return sizeof(B200VocabLossInfo); }
+
+int b200_vocab_loss_info(const B200VocabLossDesc* desc, int sm_count, B200VocabLossInfo* out) {
+    B200_ABI_GUARD_BEGIN
+    b200::clear_error();
+    if (out == nullptr || sm_count < 1) {
+        b200::set_error("out must not be NULL and sm_count=%d must be positive", sm_count);
+        return B200_ERR_INVALID_ARGUMENT;
+    }
+    std::memset(out, 0, sizeof(*out));
+    const int rc = b200::vl::check_desc(desc);
+    if (rc != B200_OK) return rc;
+    const b200::vl::Layout l = b200::vl::layout_for(*desc, sm_count);
+    out->cta_group = l.cta_group;
+    out->tile_m = l.tile_m;
+    out->vocab_tiles = l.n_tiles;
+    out->piece = l.piece;
+    out->pieces = l.pieces;
+    out->splits = l.splits;
+    out->workspace_forward = l.bytes_forward;
+    out->workspace_backward = l.bytes_backward;
+    const int64_t teacher = desc->top > 0 ? 1 : 0;
+    out->launches_forward = desc->rows == 0 ? 0 : 3 + teacher + (l.gather_forward ? 1 : 0);
+    out->launches_backward = desc->rows == 0 ? 0 : 3 + teacher + 3 * l.pieces;
+    return B200_OK;
+    B200_ABI_GUARD_END
+}
+
+int b200_vocab_loss_forward(const B200VocabLossDesc* desc, const void* hidden, const void* weight,
+                            const void* index, const void* teacher, float* loss, float* lse, void* workspace,
+                            int64_t workspace_bytes, void* stream) {
+    B200_ABI_GUARD_BEGIN
+    b200::clear_error();
+    return b200::vl::forward(desc, hidden, weight, index, teacher, loss, lse, workspace, workspace_bytes, stream);
+    B200_ABI_GUARD_END
+}
+
+int b200_vocab_loss_backward(const B200VocabLossDesc* desc, const void* hidden, const void* weight,
+                             const void* index, const void* teacher, const float* lse, const float* grad_loss,
+                             void* d_hidden, void* d_weight, void* workspace, int64_t workspace_bytes, void* stream) {
+    B200_ABI_GUARD_BEGIN
+    b200::clear_error();
+    return b200::vl::backward(desc, hidden, weight, index, teacher, lse, grad_loss, d_hidden, d_weight, workspace,
+                              workspace_bytes, stream);
+    B200_ABI_GUARD_END
+}
+
+}  // extern "C"

@@ -389,6 +389,84 @@ int b200_umma_probe(const B200UmmaConfig* cfg, const void* a, const void* b, flo
                     unsigned long long* cycles, int* status, void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* Losses at the vocabulary projection                                       */
+/* ------------------------------------------------------------------------ */
+
+/* Cross entropy and distillation over the logits z = hidden * weight^T of a
+ * projection onto a vocabulary, without keeping z, and the gradients of hidden
+ * and weight. No counterpart in the reference.
+ *
+ * hidden is rows x hidden and weight vocab x hidden, both row-major with the
+ * given row pitches, bf16 or fp16 (the same), 16-byte aligned. Row t's loss is
+ *   tau^2 * sum_k q_k (log q_k + log sum_v exp(z_v / tau) - z_{i_k} / tau)
+ * top = 0, cross entropy: one target index[t] with q = 1 and tau = 1; rows with
+ *   index[t] == ignore_index have no loss.
+ * top > 0, distillation: index and teacher are rows x top (any order); q is the
+ *   softmax of teacher / tau over the row's entries with index >= 0 and a logit
+ *   above -inf; entries of one index add up; rows without an entry have no loss.
+ * Rows without a loss count 0, get zero gradients and meet no other row,
+ * whatever hidden holds there. An index outside the vocabulary (other than the
+ * above) makes its row's loss NaN, and the gradients that it reaches.
+ * reduction: NONE (a loss per row), MEAN over the rows with a loss (0 without
+ * any) or SUM. */
+enum { B200_VL_BF16 = 0, B200_VL_F16 = 1, B200_VL_F32 = 2 };
+enum { B200_VL_NONE = 0, B200_VL_MEAN = 1, B200_VL_SUM = 2 };
+
+typedef struct B200VocabLossDesc {
+    int64_t rows;
+    int64_t vocab;
+    int64_t hidden;        /* a multiple of 8 */
+    int64_t ld_hidden;     /* row pitch in elements, a multiple of 8 */
+    int64_t ld_weight;
+    int64_t dtype;         /* B200_VL_BF16 or B200_VL_F16 */
+    int64_t top;           /* 0: cross entropy; 1..256: teacher logits per row */
+    int64_t index_bytes;   /* 4 or 8 */
+    int64_t ld_index;      /* distillation: row pitches in elements */
+    int64_t ld_teacher;
+    int64_t teacher_dtype; /* B200_VL_BF16, B200_VL_F16 or B200_VL_F32 */
+    int64_t ignore_index;  /* cross entropy */
+    int64_t reduction;
+    double temperature;    /* distillation; 1 otherwise */
+} B200VocabLossDesc;
+
+/* The host's choices for a call, a function of the sizes and the SM count. */
+typedef struct B200VocabLossInfo {
+    int64_t cta_group;     /* CTAs per tile of the logits: 1 up to 128 rows, else 2 */
+    int64_t tile_m;
+    int64_t vocab_tiles;
+    int64_t piece;         /* columns of the vocabulary per step of the backward pass */
+    int64_t pieces;
+    int64_t splits;        /* runs of the contraction over the vocabulary in d_hidden */
+    int64_t workspace_forward;  /* bytes, 256-byte aligned */
+    int64_t workspace_backward;
+    int64_t launches_forward;
+    int64_t launches_backward;  /* with both gradients */
+} B200VocabLossInfo;
+
+size_t b200_vocab_loss_desc_size(void);
+size_t b200_vocab_loss_info_size(void);
+
+/* Checks *desc and fills *out; needs no device. */
+int b200_vocab_loss_info(const B200VocabLossDesc* desc, int sm_count, B200VocabLossInfo* out);
+
+/* Asynchronous on `stream`, on the current device. loss: fp32, rows values
+ * (NONE) or one; lse: fp32, rows values (log sum exp(z / tau)) for the backward
+ * pass. The workspace is scratch for this call alone. A wait that runs out in a
+ * kernel leaves NaN in loss. */
+int b200_vocab_loss_forward(const B200VocabLossDesc* desc, const void* hidden, const void* weight,
+                            const void* index, const void* teacher, float* loss, float* lse,
+                            void* workspace, int64_t workspace_bytes, void* stream);
+
+/* grad_loss: fp32, the gradient of the loss (rows values for NONE, else one).
+ * d_hidden (rows x hidden) and d_weight (vocab x hidden): contiguous, of the
+ * operands' type, 16-byte aligned; either may be NULL. Every element is
+ * written. A wait that runs out in a kernel leaves NaN in both. */
+int b200_vocab_loss_backward(const B200VocabLossDesc* desc, const void* hidden, const void* weight,
+                             const void* index, const void* teacher, const float* lse,
+                             const float* grad_loss, void* d_hidden, void* d_weight,
+                             void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Multi-GPU N-sharding (host arithmetic; the collective runs in the caller) */
 /* ------------------------------------------------------------------------ */
 
