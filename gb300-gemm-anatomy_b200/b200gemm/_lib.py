@@ -63,6 +63,7 @@ DEV_STATUS_NAMES = {
 
 LIB_NAME = "libb200gemm.so"
 LIB_PATH = Path(os.environ.get("B200GEMM_LIB", Path(__file__).resolve().parent / LIB_NAME))
+TORCH_LIB_PATH = Path(__file__).resolve().parent / "libb200gemm_torch.so"
 
 
 class BridgeError(RuntimeError):
@@ -198,6 +199,7 @@ _STRUCT_SIZES = {
 }
 
 _lib = None
+_torch_ops = None
 
 
 def load(path: Path | None = None):
@@ -233,6 +235,25 @@ def load(path: Path | None = None):
     if path is None:
         _lib = lib
     return lib
+
+
+def torch_ops():
+    """The torch operators over the C ABI (``torch.ops.b200gemm``), bound once to ``load()``'s library."""
+    global _torch_ops
+    if _torch_ops is None:
+        import torch
+        lib = load()
+        if not TORCH_LIB_PATH.is_file():
+            raise BridgeError(f"{TORCH_LIB_PATH} is missing: build it with `make -C gb300-gemm-anatomy_b200/csrc` "
+                              "(or __graft_entry__.build()); there is no fallback path", ERR_INTERNAL)
+        try:
+            torch.ops.load_library(str(TORCH_LIB_PATH))
+        except OSError as exc:
+            raise BridgeError(f"cannot load {TORCH_LIB_PATH}: {exc}") from exc
+        names = ("b200_vocab_loss_info", "b200_vocab_loss_forward", "b200_vocab_loss_backward", "b200_last_error")
+        torch.ops.b200gemm.bind(*(ctypes.cast(getattr(lib, n), _P).value for n in names))
+        _torch_ops = torch.ops.b200gemm
+    return _torch_ops
 
 
 def last_error(lib=None) -> str:

@@ -32,6 +32,7 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <cstdlib>
 #include <cstring>
 #include <mutex>
 
@@ -1302,6 +1303,12 @@ static int device_state(DeviceState* out) {
     return B200_OK;
 }
 
+// Programmatic dependent launch is on unless B200_PDL=0, as for the GEMM's plans.
+static bool pdl_on() {
+    const char* e = std::getenv("B200_PDL");
+    return e == nullptr || e[0] != '0';
+}
+
 // Launches that follow another kernel of the same call start their set-up while
 // it ends (programmatic dependent launch); each waits for it before it touches
 // global memory.
@@ -1317,7 +1324,7 @@ static int launch(void (*fn)(KArgs...), int grid, int block, int smem, int clust
         attr[n].val.clusterDim.y = 1;
         attr[n++].val.clusterDim.z = 1;
     }
-    if (dependent) {
+    if (dependent && pdl_on()) {
         attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[n++].val.programmaticStreamSerializationAllowed = 1;
     }
