@@ -47,9 +47,19 @@ namespace vl {
 constexpr int kBK = 64;
 constexpr int kBN = 256;
 constexpr int kRowsPerCta = 128;
-constexpr int kThreads = 192;
-constexpr int kEpiWarps = 4;
+// Eight epilogue warps, two for each TMEM quadrant (32 rows), each with half of
+// the tile's columns. Four warps left the exponentials and the staging of a tile
+// exposed up to D = 1024 (768 x 32000 x 64: 28 us for the statistics, 36 us for
+// G).
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = 64 + 32 * kEpiWarps;
+constexpr int kHalfN = kBN / 2;
 constexpr int kEpiBufBytes = 32 * 128;
+// k-slices between two drains of the statistics' accumulators. The tensor cores
+// add to a 32-bit accumulator without rounding to nearest: over D = 4096 the lost
+// bits add up to 5e-6 of a logit. Sums of 512 products are added up in registers
+// instead, rounded to nearest.
+constexpr int kDrain = 8;
 constexpr int kTmemCols = 2 * kBN;
 constexpr int kQueue = 4;
 constexpr int kNoCol = INT_MAX;
@@ -81,7 +91,7 @@ struct Cfg {
     static constexpr int kStageBytes = kABytes + kBBytes;
     static constexpr int kTileM = kRowsPerCta * kCtaGroup;
     static constexpr int kEpiOffset = kStages * kStageBytes;
-    static constexpr int kEpiBytes = kEpiWarps * 2 * kEpiBufBytes;
+    static constexpr int kEpiBytes = kEpiWarps * kEpiBufBytes;
     static constexpr int kBarOffset = kEpiOffset + kEpiBytes;
     static constexpr int kBarCount = 2 * kStages + 4 + 2 * kQueue;
     static constexpr int kBarBytes = kBarCount * 8 + 16 + 4 * kQueue;
@@ -93,7 +103,7 @@ struct Cfg {
 struct Params {
     Head* head;
     unsigned long long timeout_ns;
-    int fp16;             // operand type: 1 fp16, 0 bf16
+    int fp16;             // operand type: 1 fp16, 0 bf16 (kHalf where it is packed)
     int rows;             // rows of the call
     int m;                // Dw: rows of the piece; otherwise from the head
     int n;                // columns of the product: piece (Stats, Grad) or D
@@ -108,7 +118,7 @@ struct Params {
     const int* ecol;      // [rows][top] ascending target columns, kNoCol behind the last
     const float* eq;      // [rows][top] their probabilities; null: 1
     float* zsel;          // Stats: [rows][top] logits at the targets
-    float2* part;         // Stats: [tile][part_ld] (maximum, sum of exponentials)
+    float2* part;         // Stats: [half tile][part_ld] (maximum, sum of exponentials)
     long long part_ld;
     const float* lse;     // Grad
     const float* rscale;  // Grad: g_t
@@ -136,6 +146,21 @@ __device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t smem_addr) {
     return d;
 }
 
+// Arrival on a barrier of either CTA of the pair, ordered within the own CTA
+// only: it hands back something that was read (a tile id, an accumulator), no
+// written data. The cluster-scope release waits for every earlier store to
+// global memory, about 1400 cycles per tile and warp.
+__device__ __forceinline__ void mbar_arrive_pair(uint32_t cluster_bar) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+
+// Four bytes into the peer's shared memory; they and the count on the peer's
+// barrier arrive together, so the peer waits as for a TMA load.
+__device__ __forceinline__ void st_async_u32(uint32_t cluster_addr, uint32_t v, uint32_t cluster_bar) {
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];"
+                 ::"r"(cluster_addr), "r"(v), "r"(cluster_bar) : "memory");
+}
+
 // One TMEM column of the warp's 32 lanes.
 __device__ __forceinline__ float tmem_ld_col(uint32_t taddr) {
     uint32_t r;
@@ -154,6 +179,29 @@ __device__ __forceinline__ void tma_reduce_add_2d(const void* tmap, uint32_t src
         : "memory");
 }
 
+// a[i], the index uniform in the warp: a branch for the group of 32, then five
+// levels of selects.
+__device__ __forceinline__ float pick_32(const float* a, int i) {
+    float v[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = (i & 16) ? a[j + 16] : a[j];
+#pragma unroll
+    for (int w = 8; w; w >>= 1) {
+#pragma unroll
+        for (int j = 0; j < w; ++j) v[j] = (i & w) ? v[j + w] : v[j];
+    }
+    return v[0];
+}
+
+__device__ __forceinline__ float pick(const float (&a)[kHalfN], int i) {
+    switch (i >> 5) {
+        case 0: return pick_32(a, i);
+        case 1: return pick_32(a + 32, i);
+        case 2: return pick_32(a + 64, i);
+        default: return pick_32(a + 96, i);
+    }
+}
+
 // 2^x by the hardware's approximation (absolute error about 2^-22 of the
 // result): every use is a term of a sum of exponentials or a probability.
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -167,7 +215,7 @@ __device__ __forceinline__ float exp2_approx(float x) {
 // inf - inf).
 __device__ __forceinline__ float finite_or_zero(float m) { return fabsf(m) == INFINITY ? 0.0f : m; }
 
-template <int kCtaGroup, int kOp>
+template <int kCtaGroup, int kOp, bool kHalf>
 __global__ void __launch_bounds__(kThreads, 1)
 vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmA1,
                   const __grid_constant__ CUtensorMap tmB0, const __grid_constant__ CUtensorMap tmB1,
@@ -216,13 +264,17 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
             mbar_init(tfull0 + 8 * a, 1);
             mbar_init(tempty0 + 8 * a, kEpiWarps * kCtaGroup);
         }
-        // A queued tile id is read by the MMA issuer and 4 epilogue warps of the
-        // leader, and in pair mode also by the peer's producer and 4 epilogue warps.
+        // A queued tile id is read by the MMA issuer and the epilogue warps of the
+        // leader, and in pair mode also by the peer's producer and epilogue warps.
         for (int q = 0; q < kQueue; ++q) {
             mbar_init(qfull0 + 8 * q, 1);
-            mbar_init(qempty0 + 8 * q, kPair ? 10 : 5);
+            mbar_init(qempty0 + 8 * q, (kEpiWarps + 1) * kCtaGroup);
         }
         fence_barrier_init();
+        // The peer's slots are filled by asynchronous stores, each armed before the
+        // leader may write it.
+        if (rank == 1)
+            for (int q = 0; q < kQueue; ++q) mbar_arrive_expect_tx(qfull0 + 8 * q, 4);
     }
     if (warp == 0 && lane == 0) {
         tma_prefetch_desc(&tmA0);
@@ -280,10 +332,10 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
         return w;
     };
     auto queue_wait = [&](uint32_t qs, uint32_t qph, int code) -> bool {
-        return mbar_wait<kPair>(qfull0 + 8 * qs, qph, status, p.timeout_ns, code);
+        return mbar_wait(qfull0 + 8 * qs, qph, status, p.timeout_ns, code);
     };
     auto queue_release = [&](uint32_t qs) {
-        if constexpr (kPair) mbar_arrive_cluster(mapa_shared(qempty0 + 8 * qs, 0));
+        if constexpr (kPair) mbar_arrive_pair(mapa_shared(qempty0 + 8 * qs, 0));
         else mbar_arrive(qempty0 + 8 * qs);
     };
 
@@ -314,14 +366,15 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
                         }
                     }
                     ring[qs] = t;
-                    if constexpr (kPair) {
-                        st_shared_cluster_u32(mapa_shared(ring_addr + 4 * qs, 1), static_cast<uint32_t>(t));
-                        mbar_arrive_cluster(mapa_shared(qfull0 + 8 * qs, 1));
-                    }
+                    if constexpr (kPair)
+                        st_async_u32(mapa_shared(ring_addr + 4 * qs, 1), static_cast<uint32_t>(t),
+                                     mapa_shared(qfull0 + 8 * qs, 1));
                     mbar_arrive(qfull0 + 8 * qs);
                 } else {
                     if (!queue_wait(qs, qph, B200_DEV_TIMEOUT_PRODUCER)) break;
                     t = ring[qs];
+                    // Armed for the slot's next turn before the slot is handed back.
+                    if (t >= 0) mbar_arrive_expect_tx(qfull0 + 8 * qs, 4);
                     queue_release(qs);
                 }
                 if (++qs == kQueue) { qs = 0; qph ^= 1; }
@@ -403,14 +456,20 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
                 if (t < 0) break;
                 const Tile w = tile_of(t);
                 if (w.kb0 == w.kb1) continue;
-                const uint32_t slot = unit & 1;
-                if (!mbar_wait<kPair>(tempty0 + 8 * slot, ((unit >> 1) & 1) ^ 1, status, p.timeout_ns,
-                                      B200_DEV_TIMEOUT_MMA_TMEM)) {
-                    break;
-                }
-                tc_fence_after();
-                const uint32_t d_tmem = tmem_base + slot * kBN;
                 for (int kb = w.kb0; kb < w.kb1; ++kb) {
+                    // A unit is what one accumulator sums up: the whole contraction, or
+                    // kDrain k-slices of it for the statistics.
+                    const int in_unit = kOp == kStats ? (kb - w.kb0) % kDrain : kb - w.kb0;
+                    const uint32_t slot = unit & 1;
+                    const uint32_t d_tmem = tmem_base + slot * kBN;
+                    if (in_unit == 0) {
+                        if (!mbar_wait(tempty0 + 8 * slot, ((unit >> 1) & 1) ^ 1, status, p.timeout_ns,
+                                              B200_DEV_TIMEOUT_MMA_TMEM)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                    }
                     if (!mbar_wait(full0 + 8 * stage, phase, status, p.timeout_ns,
                                    B200_DEV_TIMEOUT_MMA_FULL)) {
                         ok = false;
@@ -425,7 +484,7 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
                         // 16 rows of 128 bytes in an MN-major box.
                         const uint64_t da = kAMn ? smem_desc_mn_sw128(sa + 2048 * k) : smem_desc_sw128(sa + 32 * k);
                         const uint64_t db = kBMn ? smem_desc_mn_sw128(sb + 2048 * k) : smem_desc_sw128(sb + 32 * k);
-                        umma_bf16<kCtaGroup>(d_tmem, da, db, idesc, (kb != w.kb0 || k != 0) ? 1u : 0u);
+                        umma_bf16<kCtaGroup>(d_tmem, da, db, idesc, (in_unit != 0 || k != 0) ? 1u : 0u);
                     }
                     const uint32_t eb = empty0 + 8 * stage;
                     if constexpr (!kPair) {
@@ -435,27 +494,70 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
                         umma_commit<2>(mapa_shared(eb, 1));
                     }
                     if (++stage == kStages) { stage = 0; phase ^= 1; }
+                    if (kb + 1 == w.kb1 || (kOp == kStats && in_unit == kDrain - 1)) {
+                        const uint32_t tb = tfull0 + 8 * slot;
+                        if constexpr (!kPair) {
+                            umma_commit<1>(tb);
+                        } else {
+                            umma_commit<2>(mapa_shared(tb, 0));
+                            umma_commit<2>(mapa_shared(tb, 1));
+                        }
+                        ++unit;
+                    }
                 }
-                if (!ok) break;
-                const uint32_t tb = tfull0 + 8 * slot;
-                if constexpr (!kPair) {
-                    umma_commit<1>(tb);
-                } else {
-                    umma_commit<2>(mapa_shared(tb, 0));
-                    umma_commit<2>(mapa_shared(tb, 1));
-                }
-                ++unit;
             }
         }
         __syncwarp();
     } else {
         // ----------------------------------------------------------- epilogue
         const int q = warp & 3;  // TMEM lane quadrant this warp may access
-        const uint32_t stage_buf0 = sbase + C::kEpiOffset + q * 2 * kEpiBufBytes;
-        uint32_t unit = 0, buf = 0, qs = 0, qph = 0;
+        const int half = (warp - 2) >> 2;
+        const uint32_t sbuf = sbase + C::kEpiOffset + (warp - 2) * kEpiBufBytes;
+        const uint32_t row_addr = sbuf + lane * 128;
+        uint32_t unit = 0, qs = 0, qph = 0;
         const float alpha = kOp == kDw ? p.head->alpha : 1.0f;
+        // The warp leaves as a whole: what follows a wait is warp-wide.
+        auto wait_unit = [&]() -> bool {
+            const bool got = mbar_wait<false, true>(tfull0 + 8 * (unit & 1), (unit >> 1) & 1, status, p.timeout_ns,
+                                                    B200_DEV_TIMEOUT_EPILOGUE);
+            if (!__all_sync(0xffffffffu, got)) return false;
+            tc_fence_after();
+            return true;
+        };
+        // Accumulator fully read: hand it back to the MMA issuer.
+        auto release_unit = [&]() {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                const uint32_t bar = tempty0 + 8 * (unit & 1);
+                if constexpr (!kPair) mbar_arrive(bar);
+                else mbar_arrive_pair(mapa_shared(bar, 0));
+            }
+            ++unit;
+        };
+        // One 32-row x 128-byte chunk of the warp into its staging buffer, once the
+        // last store has read it; `store` sends it off.
+        auto stage_chunk = [&](const uint32_t (&pk)[32]) {
+            if (lane == 0) bulk_wait_group_read<0>();
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                st_shared_v4(row_addr + ((j ^ (lane & 7)) << 4), pk[4 * j], pk[4 * j + 1], pk[4 * j + 2],
+                             pk[4 * j + 3]);
+            }
+        };
+        auto store_chunk = [&](int x, int y, bool add) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                if (add) tma_reduce_add_2d(&tmD, sbuf, x, y);
+                else tma_store_2d(&tmD, sbuf, x, y);
+                bulk_commit_group();
+            }
+        };
+        auto pack = [](float lo, float hi) { return kHalf ? pack_half2(lo, hi) : pack_bf16x2(lo, hi); };
+
         while (true) {
-            // The warp leaves as a whole: what follows is warp-wide.
             if (!__all_sync(0xffffffffu, queue_wait(qs, qph, B200_DEV_TIMEOUT_EPILOGUE))) break;
             const int t = ring[qs];
             __syncwarp();
@@ -464,19 +566,21 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
             if (t < 0) break;
             const Tile w = tile_of(t);
             if (w.kb0 == w.kb1) continue;
-            const uint32_t slot = unit & 1;
             const int row0 = w.mb * C::kTileM + static_cast<int>(rank) * kRowsPerCta + q * 32;
-            const int col0 = w.nb * kBN;
-            const uint32_t t_row = tmem_base + slot * kBN + (static_cast<uint32_t>(q * 32) << 16);
+            const int col0 = w.nb * kBN + half * kHalfN;  // first column of this warp
+            const uint32_t t_lane = tmem_base + half * kHalfN + (static_cast<uint32_t>(q * 32) << 16);
 
-            // The row's targets: position of the first one at or behind the tile's
+            // The row's targets: position of the first one at or behind the warp's
             // first column, and that column.
             const int grow = row0 + lane;  // row of the products
             const bool active = grow < n_rows;
             int pos = 0, cur = kNoCol;
             long long ebase = 0;
             float rs = 0.0f, neg_lse2 = 0.0f;
-            auto col_at = [&](int i) { return i < p.top ? __ldg(p.ecol + ebase + i) : kNoCol; };
+            auto load_cur = [&]() {
+                const int c = pos < p.top ? __ldg(p.ecol + ebase + pos) : kNoCol;
+                cur = c == kNoCol ? kNoCol : c - p.v0;
+            };
             if constexpr (kOp == kStats || kOp == kGrad) {
                 if (active) {
                     const int r = __ldg(p.rowmap + grow);
@@ -492,193 +596,145 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
                         if (__ldg(p.ecol + ebase + mid) < first) pos = mid + 1;
                         else hi = mid;
                     }
-                    cur = col_at(pos);
-                    if (cur != kNoCol) cur -= p.v0;
+                    load_cur();
                 }
             }
-            auto advance = [&]() {
-                ++pos;
-                cur = col_at(pos);
-                if (cur != kNoCol) cur -= p.v0;
-            };
 
-            if (!__all_sync(0xffffffffu, mbar_wait<kPair, true>(tfull0 + 8 * slot, (unit >> 1) & 1, status,
-                                                                p.timeout_ns, B200_DEV_TIMEOUT_EPILOGUE))) {
-                break;
-            }
-            ++unit;
-            tc_fence_after();
-            auto release_tmem = [&]() {
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) {
-                    if constexpr (!kPair) mbar_arrive(tempty0 + 8 * slot);
-                    else mbar_arrive_cluster(mapa_shared(tempty0 + 8 * slot, 0));
-                }
-            };
-
+            if (!wait_unit()) break;
+            const uint32_t t_row = t_lane + (unit & 1) * kBN;
             if constexpr (kOp == kStats) {
-                float m = -INFINITY, s = 0.0f;
+                float acc[kHalfN];
+#pragma unroll
+                for (int g = 0; g < kHalfN / 32; ++g) tmem_ld_32x32b_x32(t_row + 32 * g, reinterpret_cast<uint32_t(&)[32]>(acc[32 * g]));
+                tmem_ld_wait();
+                release_unit();
+                bool ok = true;
 #pragma unroll 1
-                for (int c = 0; c < kBN / 32; ++c) {
-                    const int left = p.n - (col0 + c * 32);  // columns of the vocabulary in this chunk
-                    if (left <= 0) break;
-                    uint32_t r[32];
-                    tmem_ld_32x32b_x32(t_row + c * 32, r);
-                    tmem_ld_wait();
-                    if (left < 32) {
+                for (int kb = w.kb0 + kDrain; kb < w.kb1; kb += kDrain) {
+                    ok = wait_unit();
+                    if (!ok) break;
+                    const uint32_t t_next = t_lane + (unit & 1) * kBN;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (i >= left) r[i] = __float_as_uint(-INFINITY);
+                    for (int g = 0; g < kHalfN / 32; ++g) {
+                        uint32_t r[32];
+                        tmem_ld_32x32b_x32(t_next + 32 * g, r);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) acc[32 * g + i] += __uint_as_float(r[i]);
                     }
-                    float mx = m;
+                    release_unit();
+                }
+                if (!ok) break;
+                const int left = p.n - col0;  // columns of the vocabulary in this half
+                if (left <= 0) continue;
+                if (left < kHalfN) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(r[i]));
-                    const float ref = -finite_or_zero(mx) * p.c2;
-                    s *= exp2_approx(fmaf(finite_or_zero(m), p.c2, ref));
-                    float s0 = 0.0f, s1 = 0.0f;
+                    for (int i = 0; i < kHalfN; ++i)
+                        if (i >= left) acc[i] = -INFINITY;
+                }
+                float m4[4] = {acc[0], acc[1], acc[2], acc[3]};
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        s0 += exp2_approx(fmaf(__uint_as_float(r[i]), p.c2, ref));
-                        s1 += exp2_approx(fmaf(__uint_as_float(r[i + 1]), p.c2, ref));
-                    }
-                    s += s0 + s1;
-                    m = mx;
-                    // Logits at the targets: all lanes read the column, the lanes that
-                    // want it keep it.
-                    while (true) {
-                        const int col = __reduce_min_sync(0xffffffffu, cur);
-                        if (col >= col0 + (c + 1) * 32) break;
-                        const float z = tmem_ld_col(t_row + (col - col0));
-                        if (cur == col) {
-                            p.zsel[ebase + pos] = z;
-                            advance();
-                        }
+                for (int i = 4; i < kHalfN; ++i) m4[i & 3] = fmaxf(m4[i & 3], acc[i]);
+                const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+                const float ref = -finite_or_zero(m) * p.c2;
+                // Logits at the targets, before the exponentials take their place: the
+                // column is the same for all lanes, the lanes that want it keep it.
+                while (true) {
+                    const int col = __reduce_min_sync(0xffffffffu, cur);
+                    if (col >= col0 + kHalfN) break;
+                    const float z = pick(acc, col - col0);
+                    if (cur == col) {
+                        p.zsel[ebase + pos] = z;
+                        ++pos;
+                        load_cur();
                     }
                 }
-                release_tmem();
-                if (active) p.part[static_cast<long long>(w.nb) * p.part_ld + grow] = make_float2(m, s);
+                float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int i = 0; i < kHalfN; ++i) s4[i & 3] += exp2_approx(fmaf(acc[i], p.c2, ref));
+                if (active)
+                    p.part[static_cast<long long>(2 * w.nb + half) * p.part_ld + grow] =
+                        make_float2(m, (s4[0] + s4[1]) + (s4[2] + s4[3]));
             } else if constexpr (kOp == kGrad) {
 #pragma unroll 1
-                for (int c = 0; c < kBN / 64; ++c) {
+                for (int c = 0; c < kHalfN / 64; ++c) {
                     uint32_t r0[32], r1[32], pk[32];
                     tmem_ld_32x32b_x32(t_row + c * 64, r0);
                     tmem_ld_32x32b_x32(t_row + c * 64 + 32, r1);
                     tmem_ld_wait();
-                    const int left = p.n - (col0 + c * 64);
-                    auto grad = [&](uint32_t z, int i) {
-                        const float g = rs * exp2_approx(fmaf(__uint_as_float(z), p.c2, neg_lse2));
-                        // Rows and columns beyond the ends are zeros of the products that
-                        // contract over them, whatever the accumulator holds.
-                        return active && i < left ? g : 0.0f;
+                    const int x = col0 + c * 64;
+                    const int left = p.n - x;
+                    auto grad = [&](uint32_t z) {
+                        return rs * exp2_approx(fmaf(__uint_as_float(z), p.c2, neg_lse2));
                     };
+                    if (left < 64) {
+                        // Columns beyond the piece are zeros of the product that contracts
+                        // over them, whatever the accumulator holds: logits of -inf.
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            if (i >= left) r0[i] = __float_as_uint(-INFINITY);
+                            if (i + 32 >= left) r1[i] = __float_as_uint(-INFINITY);
+                        }
+                    }
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const float a0 = grad(r0[2 * i], 2 * i), a1 = grad(r0[2 * i + 1], 2 * i + 1);
-                        const float b0 = grad(r1[2 * i], 32 + 2 * i), b1 = grad(r1[2 * i + 1], 33 + 2 * i);
-                        pk[i] = p.fp16 ? pack_half2(a0, a1) : pack_bf16x2(a0, a1);
-                        pk[16 + i] = p.fp16 ? pack_half2(b0, b1) : pack_bf16x2(b0, b1);
+                        pk[i] = pack(grad(r0[2 * i]), grad(r0[2 * i + 1]));
+                        pk[16 + i] = pack(grad(r1[2 * i]), grad(r1[2 * i + 1]));
                     }
-                    if (row0 >= p.rows) {  // nothing of the call in these rows
-                        if (c == kBN / 64 - 1) release_tmem();
-                        continue;
-                    }
-                    const uint32_t sbuf = stage_buf0 + buf * kEpiBufBytes;
-                    if (lane == 0) bulk_wait_group_read<1>();
-                    __syncwarp();
-                    const uint32_t row_addr = sbuf + lane * 128;
+                    // So are rows without a loss.
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        st_shared_v4(row_addr + ((j ^ (lane & 7)) << 4), pk[4 * j], pk[4 * j + 1],
-                                     pk[4 * j + 2], pk[4 * j + 3]);
-                    }
+                    for (int i = 0; i < 32; ++i) pk[i] = active ? pk[i] : 0u;
+                    if (row0 >= p.rows) continue;  // nothing of the call in these rows
+                    stage_chunk(pk);
                     // The targets' columns again, from the unrounded logit: p - q.
                     while (true) {
                         const int col = __reduce_min_sync(0xffffffffu, cur);
-                        if (col >= col0 + (c + 1) * 64) break;
+                        if (col >= x + 64) break;
                         const float z = tmem_ld_col(t_row + (col - col0));
                         if (cur == col) {
                             const float qv = p.eq == nullptr ? 1.0f : __ldg(p.eq + ebase + pos);
                             const float g = rs * (exp2_approx(fmaf(z, p.c2, neg_lse2)) - qv);
-                            const uint32_t bits = p.fp16 ? pack_half2(g, 0.0f) : pack_bf16x2(g, 0.0f);
-                            const int i = col - col0 - c * 64;
+                            const int i = col - x;
                             asm volatile("st.shared.u16 [%0], %1;"
                                          ::"r"(row_addr + (((i >> 3) ^ (lane & 7)) << 4) + (i & 7) * 2),
-                                         "h"(static_cast<uint16_t>(bits & 0xffffu)) : "memory");
-                            advance();
+                                         "h"(static_cast<uint16_t>(pack(g, 0.0f) & 0xffffu)) : "memory");
+                            ++pos;
+                            load_cur();
                         }
                     }
-                    if (c == kBN / 64 - 1) release_tmem();
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) {
-                        tma_store_2d(&tmD, sbuf, col0 + c * 64, row0);
-                        bulk_commit_group();
-                    }
-                    buf ^= 1;
+                    store_chunk(x, row0, false);
                 }
+                release_unit();
             } else if constexpr (kOp == kDh) {
 #pragma unroll 1
-                for (int c = 0; c < kBN / 32; ++c) {
+                for (int c = 0; c < kHalfN / 32; ++c) {
                     uint32_t r[32];
                     tmem_ld_32x32b_x32(t_row + c * 32, r);
                     tmem_ld_wait();
-                    if (c == kBN / 32 - 1) release_tmem();
-                    const int col = col0 + c * 32;
-                    if (col >= p.n) continue;
-                    const uint32_t sbuf = stage_buf0 + buf * kEpiBufBytes;
-                    if (lane == 0) bulk_wait_group_read<1>();
-                    __syncwarp();
-                    const uint32_t row_addr = sbuf + lane * 128;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        st_shared_v4(row_addr + ((j ^ (lane & 7)) << 4), r[4 * j], r[4 * j + 1],
-                                     r[4 * j + 2], r[4 * j + 3]);
-                    }
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) {
-                        const int y = w.split * p.rows_pad + row0;
-                        if (p.accumulate) tma_reduce_add_2d(&tmD, sbuf, col, y);
-                        else tma_store_2d(&tmD, sbuf, col, y);
-                        bulk_commit_group();
-                    }
-                    buf ^= 1;
+                    const int x = col0 + c * 32;
+                    if (x >= p.n) break;
+                    stage_chunk(r);
+                    store_chunk(x, w.split * p.rows_pad + row0, p.accumulate != 0);
                 }
+                release_unit();
             } else {
 #pragma unroll 1
-                for (int c = 0; c < kBN / 64; ++c) {
+                for (int c = 0; c < kHalfN / 64; ++c) {
                     uint32_t r0[32], r1[32], pk[32];
                     tmem_ld_32x32b_x32(t_row + c * 64, r0);
                     tmem_ld_32x32b_x32(t_row + c * 64 + 32, r1);
                     tmem_ld_wait();
-                    if (c == kBN / 64 - 1) release_tmem();
-                    const int col = col0 + c * 64;
-                    if (col >= p.n || row0 >= p.m) continue;
+                    const int x = col0 + c * 64;
+                    if (x >= p.n || row0 >= p.m) break;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const float a0 = alpha * __uint_as_float(r0[2 * i]), a1 = alpha * __uint_as_float(r0[2 * i + 1]);
-                        const float b0 = alpha * __uint_as_float(r1[2 * i]), b1 = alpha * __uint_as_float(r1[2 * i + 1]);
-                        pk[i] = p.fp16 ? pack_half2(a0, a1) : pack_bf16x2(a0, a1);
-                        pk[16 + i] = p.fp16 ? pack_half2(b0, b1) : pack_bf16x2(b0, b1);
+                        pk[i] = pack(alpha * __uint_as_float(r0[2 * i]), alpha * __uint_as_float(r0[2 * i + 1]));
+                        pk[16 + i] = pack(alpha * __uint_as_float(r1[2 * i]), alpha * __uint_as_float(r1[2 * i + 1]));
                     }
-                    const uint32_t sbuf = stage_buf0 + buf * kEpiBufBytes;
-                    if (lane == 0) bulk_wait_group_read<1>();
-                    __syncwarp();
-                    const uint32_t row_addr = sbuf + lane * 128;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        st_shared_v4(row_addr + ((j ^ (lane & 7)) << 4), pk[4 * j], pk[4 * j + 1],
-                                     pk[4 * j + 2], pk[4 * j + 3]);
-                    }
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) {
-                        tma_store_2d(&tmD, sbuf, col, p.v0 + row0);
-                        bulk_commit_group();
-                    }
-                    buf ^= 1;
+                    stage_chunk(pk);
+                    store_chunk(x, p.v0 + row0, false);
                 }
+                release_unit();
             }
         }
         if (lane == 0) bulk_wait_group<0>();
@@ -831,8 +887,9 @@ struct RowsParams {
 };
 
 // One block numbers the rows that have a loss, in order, and leaves the
-// factors of the backward pass. 1024 rows per step.
+// factors of the backward pass. Four rows per thread and step.
 __global__ void __launch_bounds__(1024) rows_kernel(const RowsParams p) {
+    constexpr int kPer = 4;
     __shared__ int warp_sum[32];
     __shared__ float warp_max[32];
     __shared__ int base;
@@ -840,22 +897,33 @@ __global__ void __launch_bounds__(1024) rows_kernel(const RowsParams p) {
     if (tid == 0) base = 0;
     float gmax = 0.0f;
     __syncthreads();
-    for (int r0 = 0; r0 < p.rows; r0 += 1024) {
-        const int t = r0 + tid;
-        int f = kNoLoss;
-        if (t < p.rows) {
-            if (p.target != nullptr) {
-                const long long c = index_at(p.target, p.index_bytes, t);
-                f = c == p.ignore ? kNoLoss : (c >= 0 && c < p.vocab ? kLoss : kBad);
-                p.ecol[t] = f == kLoss ? static_cast<int>(c) : kNoCol;
-                p.flag[t] = f;
-            } else {
-                f = p.flag[t];
+    for (int r0 = 0; r0 < p.rows; r0 += 1024 * kPer) {
+        const int t0 = r0 + tid * kPer;
+        int f[kPer], count = 0;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            const int t = t0 + j;
+            f[j] = kNoLoss;
+            if (t < p.rows) {
+                if (p.target != nullptr) {
+                    const long long c = index_at(p.target, p.index_bytes, t);
+                    f[j] = c == p.ignore ? kNoLoss : (c >= 0 && c < p.vocab ? kLoss : kBad);
+                    p.ecol[t] = f[j] == kLoss ? static_cast<int>(c) : kNoCol;
+                    p.flag[t] = f[j];
+                } else {
+                    f[j] = p.flag[t];
+                }
             }
+            count += f[j] != kNoLoss;
         }
-        const bool in = f != kNoLoss;
-        const unsigned b = __ballot_sync(0xffffffffu, in);
-        if (lane == 0) warp_sum[warp] = __popc(b);
+        // Rows with a loss before this thread's first one: scan in the warp, then
+        // over the warps.
+        int upto = count;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += u;
+        }
+        if (lane == 31) warp_sum[warp] = upto;
         __syncthreads();
         if (warp == 0) {
             int v = warp_sum[lane];
@@ -866,11 +934,16 @@ __global__ void __launch_bounds__(1024) rows_kernel(const RowsParams p) {
             warp_sum[lane] = v;
         }
         __syncthreads();
-        const int at = base + (warp ? warp_sum[warp - 1] : 0) + __popc(b & ((1u << lane) - 1));
-        if (t < p.rows) {
+        int at = base + (warp ? warp_sum[warp - 1] : 0) + upto - count;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            const int t = t0 + j;
+            if (t >= p.rows) break;
+            const bool in = f[j] != kNoLoss;
             p.inv[t] = in ? (p.gather ? at : t) : -1;
             if (!p.gather) p.rowmap[t] = t;
             else if (in) p.rowmap[at] = t;
+            at += in;
             if (p.rscale != nullptr && in && p.reduction == B200_VL_NONE) {
                 const float g = fabsf(p.grad[t]);
                 gmax = g > gmax || g != g ? g : gmax;  // a NaN stays
@@ -891,6 +964,7 @@ __global__ void __launch_bounds__(1024) rows_kernel(const RowsParams p) {
         for (int i = 0; i < 32; ++i) gmax = warp_max[i] > gmax || warp_max[i] != warp_max[i] ? warp_max[i] : gmax;
     }
     if (p.rscale != nullptr) {
+        __syncthreads();  // the flags are other threads'
         const float unit = gmax > 0.0f ? gmax : 1.0f;
         for (int t = tid; t < p.rows; t += 1024) {
             const float g = p.reduction == B200_VL_NONE ? p.grad[t] / unit : 1.0f;
@@ -935,7 +1009,8 @@ struct MergeParams {
     Head* head;
     const float2* part;
     long long part_ld;
-    int tiles, rows, top, reduction;
+    int tiles;            // half tiles
+    int rows, top, reduction;
     const int* inv;
     const int* flag;
     const float* eq;
@@ -946,12 +1021,13 @@ struct MergeParams {
     float* loss;
 };
 
-// 32 rows per block: eight warps take an eighth of the tiles each (lane = row,
-// so the reads are contiguous), join in order, then a warp forms four rows'
-// losses. The last block to finish adds the rows in order.
-__global__ void __launch_bounds__(256) merge_kernel(const MergeParams p) {
-    __shared__ float sm[8][32], ss[8][32], slse[32];
-    __shared__ double sums[8];
+// 32 rows per block: each of the warps takes an equal run of the half tiles
+// (lane = row, so the reads are contiguous), one joins them in order, then each
+// forms a row's loss. The last block to finish adds the rows in order.
+constexpr int kMergeWarps = 32;
+__global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const MergeParams p) {
+    __shared__ float sm[kMergeWarps][32], ss[kMergeWarps][32], slse[32];
+    __shared__ double sums[kMergeWarps];
     __shared__ int last;
     griddep_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -960,8 +1036,9 @@ __global__ void __launch_bounds__(256) merge_kernel(const MergeParams p) {
     const int i = t < p.rows ? p.inv[t] : -1;
     float m = -INFINITY, s = 0.0f;
     if (i >= 0) {
-        const int b = p.tiles * warp / 8, e = p.tiles * (warp + 1) / 8;
-#pragma unroll 4
+        const int b = static_cast<int>(static_cast<long long>(p.tiles) * warp / kMergeWarps);
+        const int e = static_cast<int>(static_cast<long long>(p.tiles) * (warp + 1) / kMergeWarps);
+#pragma unroll 8
         for (int j = b; j < e; ++j) {
             const float2 v = p.part[j * p.part_ld + i];
             const float mx = fmaxf(m, v.x);
@@ -974,7 +1051,7 @@ __global__ void __launch_bounds__(256) merge_kernel(const MergeParams p) {
     ss[warp][lane] = s;
     __syncthreads();
     if (warp == 0) {
-        for (int w = 1; w < 8; ++w) {
+        for (int w = 1; w < kMergeWarps; ++w) {
             const float mx = fmaxf(m, sm[w][lane]);
             const float ref = -finite_or_zero(mx) * p.c2;
             s = s * exp2_approx(fmaf(finite_or_zero(m), p.c2, ref)) + ss[w][lane] * exp2_approx(fmaf(finite_or_zero(sm[w][lane]), p.c2, ref));
@@ -986,7 +1063,7 @@ __global__ void __launch_bounds__(256) merge_kernel(const MergeParams p) {
     }
     __syncthreads();
     const bool failed = p.head->status != 0;
-    for (int r = warp; r < 32 && t0 + r < p.rows; r += 8) {
+    for (int r = warp; r < 32 && t0 + r < p.rows; r += kMergeWarps) {
         const int row = t0 + r;
         const int f = p.flag[row];
         float v = 0.0f;
@@ -1012,12 +1089,12 @@ __global__ void __launch_bounds__(256) merge_kernel(const MergeParams p) {
     __threadfence();
     // In 64 bits: the sum over many rows keeps the rows' own precision.
     double sum = 0.0;
-    for (int r = threadIdx.x; r < p.rows; r += 256) sum += static_cast<double>(__ldcg(p.row_loss + r));
+    for (int r = threadIdx.x; r < p.rows; r += 32 * kMergeWarps) sum += static_cast<double>(__ldcg(p.row_loss + r));
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) sums[warp] = sum;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int w = 1; w < 8; ++w) sum += sums[w];
+        for (int w = 1; w < kMergeWarps; ++w) sum += sums[w];
         if (p.reduction == B200_VL_MEAN) sum /= max(p.head->n_valid, 1);
         *p.loss = static_cast<float>(sum);
     }
@@ -1220,7 +1297,7 @@ static Layout layout_for(const B200VocabLossDesc& d, int64_t sms) {
     l.eq = take(d.top > 0 ? 4 * T * K : 0);
     const int64_t common = at;
     l.zsel = take(4 * T * K);
-    l.part = take(8 * l.n_tiles * T);
+    l.part = take(8 * ceil_div(d.vocab, kHalfN) * T);
     l.row_loss = take(4 * T);
     l.gathered_forward = take(l.gather_forward ? 2 * T * d.hidden : 0);
     l.bytes_forward = at;
@@ -1236,12 +1313,12 @@ static Layout layout_for(const B200VocabLossDesc& d, int64_t sms) {
 using KernelFn = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, Params);
 
 template <int G>
-static KernelFn kernel_of(int op) {
+static KernelFn kernel_of(int op, bool fp16) {
     switch (op) {
-        case kStats: return vocab_gemm_kernel<G, kStats>;
-        case kGrad: return vocab_gemm_kernel<G, kGrad>;
-        case kDh: return vocab_gemm_kernel<G, kDh>;
-        default: return vocab_gemm_kernel<2, kDw>;
+        case kStats: return vocab_gemm_kernel<G, kStats, false>;
+        case kGrad: return fp16 ? vocab_gemm_kernel<G, kGrad, true> : vocab_gemm_kernel<G, kGrad, false>;
+        case kDh: return vocab_gemm_kernel<G, kDh, false>;
+        default: return fp16 ? vocab_gemm_kernel<2, kDw, true> : vocab_gemm_kernel<2, kDw, false>;
     }
 }
 
@@ -1271,9 +1348,10 @@ static int device_state(DeviceState* out) {
     std::lock_guard<std::mutex> lock(mu);
     DeviceState& s = cache[device];
     if (!s.ready) {
-        for (int op = 0; op < 4; ++op) {
-            const void* one = reinterpret_cast<const void*>(kernel_of<1>(op));
-            const void* two = reinterpret_cast<const void*>(kernel_of<2>(op));
+        for (int i = 0; i < 8; ++i) {
+            const int op = i / 2;
+            const void* one = reinterpret_cast<const void*>(kernel_of<1>(op, i % 2));
+            const void* two = reinterpret_cast<const void*>(kernel_of<2>(op, i % 2));
             if (op != kDw)
                 B200_CUDA_TRY(cudaFuncSetAttribute(one, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<1>::kSmemBytes));
             B200_CUDA_TRY(cudaFuncSetAttribute(two, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<2>::kSmemBytes));
@@ -1290,7 +1368,7 @@ static int device_state(DeviceState* out) {
         cfg.attrs = attr;
         cfg.numAttrs = 1;
         int clusters = 0;
-        const cudaError_t err = cudaOccupancyMaxActiveClusters(&clusters, reinterpret_cast<const void*>(kernel_of<2>(kStats)), &cfg);
+        const cudaError_t err = cudaOccupancyMaxActiveClusters(&clusters, reinterpret_cast<const void*>(kernel_of<2>(kStats, false)), &cfg);
         if (err != cudaSuccess || clusters <= 0) {
             cudaGetLastError();
             clusters = props.sm_count / 2;
@@ -1452,7 +1530,7 @@ static int launch_gemm(const Call& c, int op, int cta_group, int64_t tiles, cons
                        const CUtensorMap& b0, const CUtensorMap& b1, const CUtensorMap& dmap, const Params& p) {
     const int64_t slots = cta_group == 2 ? c.dev.pairs : c.dev.sms;
     const int grid = static_cast<int>(std::max<int64_t>(1, std::min(tiles, slots))) * cta_group;
-    return launch(cta_group == 2 ? kernel_of<2>(op) : kernel_of<1>(op), grid, kThreads,
+    return launch(cta_group == 2 ? kernel_of<2>(op, p.fp16) : kernel_of<1>(op, p.fp16), grid, kThreads,
                   cta_group == 2 ? Cfg<2>::kSmemBytes : Cfg<1>::kSmemBytes, cta_group, true, c.stream, a0, a1, b0, b1, dmap, p);
 }
 
@@ -1516,7 +1594,7 @@ static int forward(const B200VocabLossDesc* d, const void* hidden, const void* w
     m.head = c.head();
     m.part = p.part;
     m.part_ld = p.part_ld;
-    m.tiles = static_cast<int>(l.n_tiles);
+    m.tiles = static_cast<int>(ceil_div(d->vocab, kHalfN));
     m.rows = static_cast<int>(d->rows);
     m.top = p.top;
     m.reduction = static_cast<int>(d->reduction);
@@ -1530,7 +1608,8 @@ static int forward(const B200VocabLossDesc* d, const void* hidden, const void* w
     m.lse = lse;
     m.row_loss = d->reduction == B200_VL_NONE ? loss : c.at<float>(l.row_loss);
     m.loss = loss;
-    return launch(merge_kernel, static_cast<int>(ceil_div(d->rows, 32)), 256, 0, 1, true, c.stream, m);
+    return launch(merge_kernel, static_cast<int>(ceil_div(d->rows, 32)), 32 * kMergeWarps, 0, 1, true,
+                  c.stream, m);
 }
 
 static int backward(const B200VocabLossDesc* d, const void* hidden, const void* weight, const void* index,
