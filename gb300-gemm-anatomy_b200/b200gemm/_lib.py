@@ -129,8 +129,8 @@ VocabLossDesc = _i64_struct(
 
 VocabLossInfo = _i64_struct(
     "B200VocabLossInfo",
-    ["cta_group", "tile_m", "vocab_tiles", "piece", "pieces", "splits", "workspace_forward",
-     "workspace_backward", "launches_forward", "launches_backward"],
+    ["cta_group", "tile_m", "tile_n", "piece", "pieces", "splits_hidden", "splits_weight",
+     "workspace_forward", "workspace_backward", "launches_forward", "launches_backward"],
 )
 
 _P = ctypes.c_void_p

@@ -45,7 +45,7 @@ namespace b200 {
 namespace vl {
 
 constexpr int kBK = 64;
-constexpr int kBN = 256;
+constexpr int kBN = 256;          // columns of a tile; 128 where wider ones leave SMs idle
 constexpr int kRowsPerCta = 128;
 // Eight epilogue warps, two for each TMEM quadrant (32 rows), each with half of
 // the tile's columns. Four warps left the exponentials and the staging of a tile
@@ -53,23 +53,25 @@ constexpr int kRowsPerCta = 128;
 // G).
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 64 + 32 * kEpiWarps;
-constexpr int kHalfN = kBN / 2;
 constexpr int kEpiBufBytes = 32 * 128;
 // k-slices between two drains of the statistics' accumulators. The tensor cores
 // add to a 32-bit accumulator without rounding to nearest: over D = 4096 the lost
 // bits add up to 5e-6 of a logit. Sums of 512 products are added up in registers
 // instead, rounded to nearest.
 constexpr int kDrain = 8;
-constexpr int kTmemCols = 2 * kBN;
 constexpr int kQueue = 4;
 constexpr int kNoCol = INT_MAX;
 constexpr int kMaxTop = 256;      // teacher logits per row
 constexpr int kMaxSplits = 16;    // runs of the contraction of dH
 constexpr float kLog2e = 1.4426950408889634f;
 
-// The four products. Operands: Stats, Grad: A = H, B = W (both K-major);
-// Dh: A = G (K-major), B = W (MN-major); Dw: A = G, B = H (both MN-major).
-enum Op { kStats = 0, kGrad = 1, kDh = 2, kDw = 3 };
+// The products. Operands: Stats, Grad: A = H, B = W (both K-major); Dh: A = G
+// (K-major), B = W (MN-major); Dw: A = G, B = H (both MN-major). StatsShort is
+// Stats over at most kDrain k-slices, DwParts leaves runs of Dw's contraction
+// as partial sums.
+enum Op { kStats = 0, kStatsShort = 1, kGrad = 2, kDh = 3, kDw = 4, kDwParts = 5 };
+__host__ __device__ constexpr bool is_stats(int op) { return op == kStats || op == kStatsShort; }
+__host__ __device__ constexpr bool is_dw(int op) { return op == kDw || op == kDwParts; }
 
 // What the first kernels of a call leave in the workspace for the others.
 struct Head {
@@ -82,11 +84,12 @@ struct Head {
     float alpha;      // factor common to all rows of G, applied after the products
 };
 
-template <int kCtaGroup>
+template <int kCtaGroup, int kTileN>
 struct Cfg {
-    static constexpr int kStages = kCtaGroup == 1 ? 4 : 6;
+    static_assert(kTileN == kBN || (kTileN == 128 && kCtaGroup == 1), "unsupported tile width");
+    static constexpr int kStages = kCtaGroup == 1 && kTileN == kBN ? 4 : 6;
     static constexpr int kABytes = kRowsPerCta * kBK * 2;
-    static constexpr int kBRows = kBN / kCtaGroup;
+    static constexpr int kBRows = kTileN / kCtaGroup;
     static constexpr int kBBytes = kBRows * kBK * 2;
     static constexpr int kStageBytes = kABytes + kBBytes;
     static constexpr int kTileM = kRowsPerCta * kCtaGroup;
@@ -110,15 +113,16 @@ struct Params {
     int k;                // contraction: D (Stats, Grad) or piece (Dh); Dw: from the head
     int v0;               // first vocabulary row of the piece
     int group_m;          // m-blocks per raster group
-    int splits;           // Dh: runs of the contraction
-    int rows_pad;         // Dh: rows between two splits' partial sums
+    int a_bytes;          // bytes of an A tile: rows beyond the call's are not loaded
+    int splits;           // Dh, DwParts: runs of the contraction
+    int rows_pad;         // Dh, DwParts: rows between two splits' partial sums
     int accumulate;       // Dh: 1 add to the partial sums, 0 write them
     // Stats, Grad: per row of the call (not of the gathered copy)
     const int* rowmap;    // gathered row -> row
     const int* ecol;      // [rows][top] ascending target columns, kNoCol behind the last
     const float* eq;      // [rows][top] their probabilities; null: 1
     float* zsel;          // Stats: [rows][top] logits at the targets
-    float2* part;         // Stats: [half tile][part_ld] (maximum, sum of exponentials)
+    float2* part;         // Stats: [gathered row][part_ld half tiles] (maximum, sum of exponentials)
     long long part_ld;
     const float* lse;     // Grad
     const float* rscale;  // Grad: g_t
@@ -193,13 +197,13 @@ __device__ __forceinline__ float pick_32(const float* a, int i) {
     return v[0];
 }
 
-__device__ __forceinline__ float pick(const float (&a)[kHalfN], int i) {
-    switch (i >> 5) {
-        case 0: return pick_32(a, i);
-        case 1: return pick_32(a + 32, i);
-        case 2: return pick_32(a + 64, i);
-        default: return pick_32(a + 96, i);
+template <int kN>
+__device__ __forceinline__ float pick(const float (&a)[kN], int i) {
+    if constexpr (kN == 128) {
+        if (i >= 96) return pick_32(a + 96, i);
+        if (i >= 64) return pick_32(a + 64, i);
     }
+    return i >= 32 ? pick_32(a + 32, i) : pick_32(a, i);
 }
 
 // 2^x by the hardware's approximation (absolute error about 2^-22 of the
@@ -215,16 +219,18 @@ __device__ __forceinline__ float exp2_approx(float x) {
 // inf - inf).
 __device__ __forceinline__ float finite_or_zero(float m) { return fabsf(m) == INFINITY ? 0.0f : m; }
 
-template <int kCtaGroup, int kOp, bool kHalf>
+template <int kCtaGroup, int kTileN, int kOp, bool kHalf>
 __global__ void __launch_bounds__(kThreads, 1)
 vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmA1,
                   const __grid_constant__ CUtensorMap tmB0, const __grid_constant__ CUtensorMap tmB1,
                   const __grid_constant__ CUtensorMap tmD, const Params p) {
-    using C = Cfg<kCtaGroup>;
+    using C = Cfg<kCtaGroup, kTileN>;
     constexpr int kStages = C::kStages;
+    constexpr int kHalfN = kTileN / 2;
+    constexpr int kTmemCols = 2 * kTileN;  // two accumulators
     constexpr bool kPair = kCtaGroup == 2;
-    constexpr bool kAMn = kOp == kDw;
-    constexpr bool kBMn = kOp == kDh || kOp == kDw;
+    constexpr bool kAMn = is_dw(kOp);
+    constexpr bool kBMn = kOp == kDh || is_dw(kOp);
     constexpr int kBoxBytes = 64 * kBK * 2;  // an MN-major box
 
     int* const status = &p.head->status;
@@ -279,7 +285,7 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
     if (warp == 0 && lane == 0) {
         tma_prefetch_desc(&tmA0);
         tma_prefetch_desc(&tmB0);
-        if (kOp != kStats) tma_prefetch_desc(&tmD);
+        if (!is_stats(kOp)) tma_prefetch_desc(&tmD);
     }
     if (warp == 1) {
         tmem_alloc<kCtaGroup>(smem_u32(tmem_slot), kTmemCols);
@@ -296,15 +302,16 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
     const bool compact = p.head->compact != 0;
     // Of H, the gathered copy where rows were left out. Without a single row the
     // products still run over one block of zero rows: dW is then written as zeros.
-    const CUtensorMap* tmA = ((kOp == kStats || kOp == kGrad) && compact) ? &tmA1 : &tmA0;
-    const CUtensorMap* tmB = (kOp == kDw && compact) ? &tmB1 : &tmB0;
-    const int m_ext = kOp == kDw ? p.m : (kOp == kStats ? n_rows : max(n_rows, 1));
-    const int k_ext = kOp == kDw ? max(n_rows, 1) : p.k;
+    const CUtensorMap* tmA = ((is_stats(kOp) || kOp == kGrad) && compact) ? &tmA1 : &tmA0;
+    const CUtensorMap* tmB = (is_dw(kOp) && compact) ? &tmB1 : &tmB0;
+    const int m_ext = is_dw(kOp) ? p.m : (is_stats(kOp) ? n_rows : max(n_rows, 1));
+    const int k_ext = is_dw(kOp) ? max(n_rows, 1) : p.k;
     const int num_m = (m_ext + C::kTileM - 1) / C::kTileM;
-    const int num_n = (p.n + kBN - 1) / kBN;
+    const int num_n = (p.n + kTileN - 1) / kTileN;
     const int num_k = (k_ext + kBK - 1) / kBK;
     const int tiles_mn = num_m * num_n;
-    const int num_tiles = kOp == kDh ? tiles_mn * p.splits : tiles_mn;
+    constexpr bool kSplit = kOp == kDh || kOp == kDwParts;
+    const int num_tiles = kSplit ? tiles_mn * p.splits : tiles_mn;
 
     // Tile id -> blocks and k-slices. Groups of m-blocks walk all n-blocks, so
     // the tiles in flight share rows of both operands in L2.
@@ -316,7 +323,7 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
         w.split = 0;
         w.kb0 = 0;
         w.kb1 = num_k;
-        if constexpr (kOp == kDh) {
+        if constexpr (kSplit) {
             w.split = t / tiles_mn;
             t -= w.split * tiles_mn;
             w.kb0 = static_cast<int>(static_cast<long long>(num_k) * w.split / p.splits);
@@ -384,7 +391,7 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
                 }
                 const Tile w = tile_of(t);
                 const int a_m = w.mb * C::kTileM + static_cast<int>(rank) * kRowsPerCta;
-                const int b_n = w.nb * kBN + static_cast<int>(rank) * C::kBRows;
+                const int b_n = w.nb * kTileN + static_cast<int>(rank) * C::kBRows;
                 // The next tile id is fetched two ring depths before the last k-slice:
                 // early enough to hide the round trip, late enough that a fast cluster
                 // does not take two tiles while a slow one has none.
@@ -401,7 +408,7 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
                     const uint32_t sb = sa + C::kABytes;
                     const uint32_t fb = full0 + 8 * stage;
                     const uint32_t bar = kPair ? mapa_shared(fb, 0) : fb;
-                    if (rank == 0) mbar_arrive_expect_tx(fb, kCtaGroup * C::kStageBytes);
+                    if (rank == 0) mbar_arrive_expect_tx(fb, kCtaGroup * (p.a_bytes + C::kBBytes));
                     auto load = [&](uint32_t dst, const CUtensorMap* map, int x, int y) {
                         if constexpr (kPair) tma_load_2d_pair(dst, map, bar, x, y);
                         else tma_load_2d(dst, map, bar, x, y);
@@ -444,7 +451,7 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
         if (rank == 0 && elect_one()) {
             const uint32_t fmt = p.fp16 ? 0u : 1u;
             const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((kAMn ? 1u : 0u) << 15) |
-                                   ((kBMn ? 1u : 0u) << 16) | ((kBN >> 3) << 17) |
+                                   ((kBMn ? 1u : 0u) << 16) | ((kTileN >> 3) << 17) |
                                    (((kRowsPerCta * kCtaGroup) >> 4) << 24);
             uint32_t stage = 0, phase = 0, unit = 0, qs = 0, qph = 0;
             bool ok = true;
@@ -461,7 +468,7 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
                     // kDrain k-slices of it for the statistics.
                     const int in_unit = kOp == kStats ? (kb - w.kb0) % kDrain : kb - w.kb0;
                     const uint32_t slot = unit & 1;
-                    const uint32_t d_tmem = tmem_base + slot * kBN;
+                    const uint32_t d_tmem = tmem_base + slot * kTileN;
                     if (in_unit == 0) {
                         if (!mbar_wait(tempty0 + 8 * slot, ((unit >> 1) & 1) ^ 1, status, p.timeout_ns,
                                               B200_DEV_TIMEOUT_MMA_TMEM)) {
@@ -567,7 +574,7 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
             const Tile w = tile_of(t);
             if (w.kb0 == w.kb1) continue;
             const int row0 = w.mb * C::kTileM + static_cast<int>(rank) * kRowsPerCta + q * 32;
-            const int col0 = w.nb * kBN + half * kHalfN;  // first column of this warp
+            const int col0 = w.nb * kTileN + half * kHalfN;  // first column of this warp
             const uint32_t t_lane = tmem_base + half * kHalfN + (static_cast<uint32_t>(q * 32) << 16);
 
             // The row's targets: position of the first one at or behind the warp's
@@ -581,7 +588,7 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
                 const int c = pos < p.top ? __ldg(p.ecol + ebase + pos) : kNoCol;
                 cur = c == kNoCol ? kNoCol : c - p.v0;
             };
-            if constexpr (kOp == kStats || kOp == kGrad) {
+            if constexpr (is_stats(kOp) || kOp == kGrad) {
                 if (active) {
                     const int r = __ldg(p.rowmap + grow);
                     ebase = static_cast<long long>(r) * p.top;
@@ -601,7 +608,7 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
             }
 
             if (!wait_unit()) break;
-            const uint32_t t_row = t_lane + (unit & 1) * kBN;
+            const uint32_t t_row = t_lane + (unit & 1) * kTileN;
             if constexpr (kOp == kStats) {
                 float acc[kHalfN];
 #pragma unroll
@@ -613,7 +620,7 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
                 for (int kb = w.kb0 + kDrain; kb < w.kb1; kb += kDrain) {
                     ok = wait_unit();
                     if (!ok) break;
-                    const uint32_t t_next = t_lane + (unit & 1) * kBN;
+                    const uint32_t t_next = t_lane + (unit & 1) * kTileN;
 #pragma unroll
                     for (int g = 0; g < kHalfN / 32; ++g) {
                         uint32_t r[32];
@@ -653,8 +660,51 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
 #pragma unroll
                 for (int i = 0; i < kHalfN; ++i) s4[i & 3] += exp2_approx(fmaf(acc[i], p.c2, ref));
                 if (active)
-                    p.part[static_cast<long long>(2 * w.nb + half) * p.part_ld + grow] =
+                    p.part[grow * p.part_ld + 2 * w.nb + half] =
                         make_float2(m, (s4[0] + s4[1]) + (s4[2] + s4[3]));
+            } else if constexpr (kOp == kStatsShort) {
+                // One accumulator holds the whole contraction: 32 columns at a time from
+                // TMEM, with a running maximum. A tenth of the code above, which a small
+                // call would wait for (5 us of instruction fetches).
+                float m = -INFINITY, s = 0.0f;
+#pragma unroll 1
+                for (int c = 0; c < kHalfN / 32; ++c) {
+                    const int left = p.n - (col0 + c * 32);
+                    if (left <= 0) break;
+                    uint32_t r[32];
+                    tmem_ld_32x32b_x32(t_row + c * 32, r);
+                    tmem_ld_wait();
+                    if (left < 32) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (i >= left) r[i] = __float_as_uint(-INFINITY);
+                    }
+                    float m4[4] = {m, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(r[i]));
+                    const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+                    const float ref = -finite_or_zero(mx) * p.c2;
+                    float s4[4] = {s * exp2_approx(fmaf(finite_or_zero(m), p.c2, ref)), 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) s4[i & 3] += exp2_approx(fmaf(__uint_as_float(r[i]), p.c2, ref));
+                    s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+                    m = mx;
+                    // Logits at the targets: all lanes read the column, the lanes that
+                    // want it keep it.
+                    while (true) {
+                        const int col = __reduce_min_sync(0xffffffffu, cur);
+                        if (col >= col0 + (c + 1) * 32) break;
+                        const float z = tmem_ld_col(t_row + (col - col0));
+                        if (cur == col) {
+                            p.zsel[ebase + pos] = z;
+                            ++pos;
+                            load_cur();
+                        }
+                    }
+                }
+                release_unit();
+                if (active && col0 < p.n)
+                    p.part[grow * p.part_ld + 2 * w.nb + half] = make_float2(m, s);
             } else if constexpr (kOp == kGrad) {
 #pragma unroll 1
                 for (int c = 0; c < kHalfN / 64; ++c) {
@@ -705,7 +755,7 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
                     store_chunk(x, row0, false);
                 }
                 release_unit();
-            } else if constexpr (kOp == kDh) {
+            } else if constexpr (kSplit) {
 #pragma unroll 1
                 for (int c = 0; c < kHalfN / 32; ++c) {
                     uint32_t r[32];
@@ -944,7 +994,10 @@ __global__ void __launch_bounds__(1024) rows_kernel(const RowsParams p) {
             if (!p.gather) p.rowmap[t] = t;
             else if (in) p.rowmap[at] = t;
             at += in;
-            if (p.rscale != nullptr && in && p.reduction == B200_VL_NONE) {
+            if (p.rscale == nullptr) continue;
+            if (p.reduction != B200_VL_NONE) {
+                p.rscale[t] = f[j] == kBad ? NAN : 1.0f;
+            } else if (in) {
                 const float g = fabsf(p.grad[t]);
                 gmax = g > gmax || g != g ? g : gmax;  // a NaN stays
             }
@@ -962,14 +1015,8 @@ __global__ void __launch_bounds__(1024) rows_kernel(const RowsParams p) {
         if (lane == 0) warp_max[warp] = gmax;
         __syncthreads();
         for (int i = 0; i < 32; ++i) gmax = warp_max[i] > gmax || warp_max[i] != warp_max[i] ? warp_max[i] : gmax;
-    }
-    if (p.rscale != nullptr) {
-        __syncthreads();  // the flags are other threads'
         const float unit = gmax > 0.0f ? gmax : 1.0f;
-        for (int t = tid; t < p.rows; t += 1024) {
-            const float g = p.reduction == B200_VL_NONE ? p.grad[t] / unit : 1.0f;
-            p.rscale[t] = p.flag[t] == kBad ? NAN : g;
-        }
+        for (int t = tid; t < p.rows; t += 1024) p.rscale[t] = p.flag[t] == kBad ? NAN : p.grad[t] / unit;
     }
     if (tid == 0) {
         Head h;
@@ -1010,6 +1057,7 @@ struct MergeParams {
     const float2* part;
     long long part_ld;
     int tiles;            // half tiles
+    int warps_per_row;    // 1 or kMergeWarps
     int rows, top, reduction;
     const int* inv;
     const int* flag;
@@ -1021,57 +1069,60 @@ struct MergeParams {
     float* loss;
 };
 
-// 32 rows per block: each of the warps takes an equal run of the half tiles
-// (lane = row, so the reads are contiguous), one joins them in order, then each
-// forms a row's loss. The last block to finish adds the rows in order.
-constexpr int kMergeWarps = 32;
+// A warp, or all eight of a block where there are few rows, merges a row's half
+// tiles in a fixed order and forms its loss; the last block to finish adds the
+// rows in order. Reads 8 bytes per (row, half tile).
+constexpr int kMergeWarps = 8;
 __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const MergeParams p) {
-    __shared__ float sm[kMergeWarps][32], ss[kMergeWarps][32], slse[32];
+    __shared__ float sm[kMergeWarps], ss[kMergeWarps];
     __shared__ double sums[kMergeWarps];
     __shared__ int last;
     griddep_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int t0 = blockIdx.x * 32;
-    const int t = t0 + lane;
-    const int i = t < p.rows ? p.inv[t] : -1;
+    const int row = blockIdx.x * (kMergeWarps / p.warps_per_row) + warp / p.warps_per_row;
+    const int i = row < p.rows ? p.inv[row] : -1;
     float m = -INFINITY, s = 0.0f;
+    auto join = [&](float m2, float s2) {
+        const float mx = fmaxf(m, m2);
+        const float ref = -finite_or_zero(mx) * p.c2;
+        s = s * exp2_approx(fmaf(finite_or_zero(m), p.c2, ref)) + s2 * exp2_approx(fmaf(finite_or_zero(m2), p.c2, ref));
+        m = mx;
+    };
     if (i >= 0) {
-        const int b = static_cast<int>(static_cast<long long>(p.tiles) * warp / kMergeWarps);
-        const int e = static_cast<int>(static_cast<long long>(p.tiles) * (warp + 1) / kMergeWarps);
+        const float2* part = p.part + i * p.part_ld;
+        const int step = 32 * p.warps_per_row;
 #pragma unroll 8
-        for (int j = b; j < e; ++j) {
-            const float2 v = p.part[j * p.part_ld + i];
-            const float mx = fmaxf(m, v.x);
-            const float ref = -finite_or_zero(mx) * p.c2;
-            s = s * exp2_approx(fmaf(finite_or_zero(m), p.c2, ref)) + v.y * exp2_approx(fmaf(finite_or_zero(v.x), p.c2, ref));
-            m = mx;
+        for (int j = (warp % p.warps_per_row) * 32 + lane; j < p.tiles; j += step) {
+            const float2 v = part[j];
+            join(v.x, v.y);
         }
     }
-    sm[warp][lane] = m;
-    ss[warp][lane] = s;
-    __syncthreads();
-    if (warp == 0) {
-        for (int w = 1; w < kMergeWarps; ++w) {
-            const float mx = fmaxf(m, sm[w][lane]);
-            const float ref = -finite_or_zero(mx) * p.c2;
-            s = s * exp2_approx(fmaf(finite_or_zero(m), p.c2, ref)) + ss[w][lane] * exp2_approx(fmaf(finite_or_zero(sm[w][lane]), p.c2, ref));
-            m = mx;
-        }
-        const float l = i >= 0 ? logf(s) + finite_or_zero(m) * p.inv_tau : 0.0f;
-        slse[lane] = l;
-        if (t < p.rows) p.lse[t] = l;
+    for (int o = 16; o; o >>= 1) {
+        const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+        join(m2, s2);
     }
-    __syncthreads();
+    if (p.warps_per_row > 1) {
+        if (lane == 0) {
+            sm[warp] = m;
+            ss[warp] = s;
+        }
+        __syncthreads();
+        m = sm[0];
+        s = ss[0];
+        for (int w = 1; w < kMergeWarps; ++w) join(sm[w], ss[w]);
+    }
+    const float lse = i >= 0 ? logf(s) + finite_or_zero(m) * p.inv_tau : 0.0f;
+    const bool leader = row < p.rows && warp % p.warps_per_row == 0;
+    if (leader && lane == 0) p.lse[row] = lse;
     const bool failed = p.head->status != 0;
-    for (int r = warp; r < 32 && t0 + r < p.rows; r += kMergeWarps) {
-        const int row = t0 + r;
+    if (leader) {
         const int f = p.flag[row];
         float v = 0.0f;
         if (f == kLoss) {
             const long long e = static_cast<long long>(row) * p.top;
             for (int k = lane; k < p.top; k += 32) {
                 const float qv = p.eq == nullptr ? 1.0f : p.eq[e + k];
-                if (qv != 0.0f) v += qv * ((p.eq == nullptr ? 0.0f : logf(qv)) + (slse[r] - p.zsel[e + k] * p.inv_tau));
+                if (qv != 0.0f) v += qv * ((p.eq == nullptr ? 0.0f : logf(qv)) + (lse - p.zsel[e + k] * p.inv_tau));
             }
             for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
             v *= p.tau2;
@@ -1103,53 +1154,55 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const MergePara
 struct FinishParams {
     const Head* head;
     const int* inv;
-    const float* part;    // [splits][rows_pad][hidden]
-    long long split_stride;
-    int splits, rows, hidden, vocab, fp16;
+    const float* part_h;  // dH: [splits][rows_pad][hidden]
+    const float* part_w;  // dW: the same over the vocabulary, or null: written by the product
+    long long stride_h, stride_w;
+    int splits_h, splits_w, rows, hidden, vocab, fp16;
     void* d_hidden;
     void* d_weight;
 };
 
-// dH: adds the splits in order, applies the common factor, rounds, and puts the
-// rows back in their places; rows without a loss get zeros. 4 bytes read per
-// split and 2 written for each element.
+// Adds the splits of dH (and of dW) in order, applies the common factor, rounds,
+// and puts the rows of dH back in their places; rows without a loss get zeros.
+// 4 bytes read per split and 2 written for each element.
 __global__ void __launch_bounds__(256) finish_kernel(const FinishParams p) {
     griddep_wait();
     const bool failed = p.head->status != 0;
     const float alpha = p.head->alpha;
     const int vecs = p.hidden / 8;
-    if (p.d_hidden != nullptr) {
-        for (int t = blockIdx.x; t < p.rows; t += gridDim.x) {
-            const int i = p.inv[t];
-            uint4* out = static_cast<uint4*>(p.d_hidden) + static_cast<long long>(t) * vecs;
-            for (int v = threadIdx.x; v < vecs; v += 256) {
-                float x[8] = {};
-                if (i >= 0) {
-                    const float* src = p.part + static_cast<long long>(i) * p.hidden + v * 8;
-                    for (int s = 0; s < p.splits; ++s) {
-                        const float4 a = __ldcs(reinterpret_cast<const float4*>(src + s * p.split_stride));
-                        const float4 b = __ldcs(reinterpret_cast<const float4*>(src + s * p.split_stride) + 1);
-                        x[0] += a.x; x[1] += a.y; x[2] += a.z; x[3] += a.w;
-                        x[4] += b.x; x[5] += b.y; x[6] += b.z; x[7] += b.w;
-                    }
+    // Runs of dW's contraction that had no row were not written.
+    const int num_k = (max(p.head->n_rows, 1) + kBK - 1) / kBK;
+    const int rows_h = p.d_hidden != nullptr ? p.rows : 0;
+    const int rows_w = p.d_weight != nullptr && (failed || p.part_w != nullptr) ? p.vocab : 0;
+    for (int r = blockIdx.x; r < rows_h + rows_w; r += gridDim.x) {
+        const bool is_h = r < rows_h;
+        const int t = is_h ? r : r - rows_h;
+        const int i = is_h ? p.inv[t] : t;
+        const int splits = is_h ? p.splits_h : p.splits_w;
+        const long long stride = is_h ? p.stride_h : p.stride_w;
+        const float* part = (is_h ? p.part_h : p.part_w) + static_cast<long long>(max(i, 0)) * p.hidden;
+        uint4* out = static_cast<uint4*>(is_h ? p.d_hidden : p.d_weight) + static_cast<long long>(t) * vecs;
+        for (int v = threadIdx.x; v < vecs; v += 256) {
+            float x[8] = {};
+            if (i >= 0 && !failed) {
+                for (int s = 0; s < splits; ++s) {
+                    if (!is_h && static_cast<long long>(num_k) * s / splits == static_cast<long long>(num_k) * (s + 1) / splits) continue;
+                    const float4* src = reinterpret_cast<const float4*>(part + s * stride) + 2 * v;
+                    const float4 a = __ldcs(src), b = __ldcs(src + 1);
+                    x[0] += a.x; x[1] += a.y; x[2] += a.z; x[3] += a.w;
+                    x[4] += b.x; x[5] += b.y; x[6] += b.z; x[7] += b.w;
                 }
-                uint32_t o[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float lo = failed ? NAN : (i >= 0 ? alpha * x[2 * j] : 0.0f);
-                    const float hi = failed ? NAN : (i >= 0 ? alpha * x[2 * j + 1] : 0.0f);
-                    o[j] = p.fp16 ? pack_half2(lo, hi) : pack_bf16x2(lo, hi);
-                }
-                out[v] = make_uint4(o[0], o[1], o[2], o[3]);
             }
+            uint32_t o[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                // Never a silent half of a gradient: a launch that was given up leaves NaN.
+                const float lo = failed ? NAN : (i >= 0 ? alpha * x[2 * j] : 0.0f);
+                const float hi = failed ? NAN : (i >= 0 ? alpha * x[2 * j + 1] : 0.0f);
+                o[j] = p.fp16 ? pack_half2(lo, hi) : pack_bf16x2(lo, hi);
+            }
+            out[v] = make_uint4(o[0], o[1], o[2], o[3]);
         }
-    }
-    if (failed && p.d_weight != nullptr) {
-        // Never a silent half of a gradient: a launch that was given up leaves NaN.
-        const long long n = static_cast<long long>(p.vocab) * vecs;
-        const uint4 nan4 = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
-        for (long long v = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; v < n; v += static_cast<long long>(gridDim.x) * 256)
-            static_cast<uint4*>(p.d_weight)[v] = nan4;
     }
 }
 
@@ -1164,13 +1217,13 @@ constexpr int64_t kPieceBytes = int64_t(256) << 20;
 constexpr int64_t kPartialBytes = int64_t(256) << 20;
 
 struct Layout {
-    int cta_group;
-    int64_t tile_m, piece, pieces, splits, rows_pad;
-    int64_t n_tiles;
+    int cta_group, tile_n;          // tiles of the logits (Stats, Grad)
+    int cta_group_h;                // tiles of dH, 256 wide
+    int64_t tile_m, tile_m_h, piece, pieces, splits_h, splits_w, rows_pad;
     // Offsets in the workspace.
     int64_t flag, rowmap, inv, ecol, eq;                 // both directions
     int64_t zsel, part, row_loss, gathered_forward;
-    int64_t rscale, gathered_backward, g, partial;
+    int64_t rscale, gathered_backward, g, part_h, part_w;
     int64_t bytes_forward, bytes_backward;
     bool gather_forward;
 };
@@ -1244,44 +1297,86 @@ static int check_desc(const B200VocabLossDesc* d) {
 }
 
 // The host's choices for a call: a function of the sizes and the SM count alone.
+// Costs are in k-slices of a 256 x 256 pair tile (about 0.27 us).
 static Layout layout_for(const B200VocabLossDesc& d, int64_t sms) {
     Layout l{};
     const int64_t T = std::max<int64_t>(d.rows, 1), K = std::max<int64_t>(d.top, 1);
-    l.cta_group = T <= kRowsPerCta ? 1 : 2;
+    const int64_t V = d.vocab, D = d.hidden;
+    const int64_t pairs = std::max<int64_t>(sms / 2, 1);
+    const int64_t kd = ceil_div(D, kBK), kt = ceil_div(T, kBK);
+    // Tiles of the logits: pairs 256 x 256, or single CTAs 128 x 256 or 128 x 128
+    // where those finish in fewer rounds. The smaller ones read their operands more
+    // often per product.
+    struct Shape { int cta_group, tile_n; double slice; };
+    double best_rounds = 0.0;
+    for (const Shape& c : {Shape{2, 256, 1.0}, Shape{1, 256, 1.1}, Shape{1, 128, 0.55}}) {
+        if (c.cta_group == 2 && T <= kRowsPerCta) continue;
+        const int64_t tiles = ceil_div(T, kRowsPerCta * c.cta_group) * ceil_div(V, c.tile_n);
+        const double rounds = static_cast<double>(ceil_div(tiles, std::max<int64_t>(sms / c.cta_group, 1))) *
+                              (c.slice * static_cast<double>(kd) + 4.0);
+        if (l.cta_group == 0 || rounds < best_rounds) {
+            best_rounds = rounds;
+            l.cta_group = c.cta_group;
+            l.tile_n = c.tile_n;
+        }
+    }
     l.tile_m = kRowsPerCta * l.cta_group;
-    l.rows_pad = align_up(T, l.tile_m);
-    l.n_tiles = ceil_div(d.vocab, kBN);
+    l.cta_group_h = T <= kRowsPerCta ? 1 : 2;
+    l.tile_m_h = kRowsPerCta * l.cta_group_h;
+    l.rows_pad = align_up(T, l.tile_m_h);
     l.gather_forward = T > kRowsPerCta;
-    const int64_t slots = std::max<int64_t>(sms / l.cta_group, 1), pairs = std::max<int64_t>(sms / 2, 1);
-    const int64_t mb = l.rows_pad / l.tile_m, nb = ceil_div(d.hidden, kBN);
-    const int64_t kd = ceil_div(d.hidden, kBK), kt = ceil_div(T, kBK);
-    // Piece of the vocabulary (in blocks of 256) and runs of dH's contraction: the
-    // least k-slices on the longest cluster, over the three products of all
-    // pieces, with eight k-slices for each launch's start and end. One piece where
-    // G has room; otherwise up to 64 widths between half the room and all of it.
-    // More than one run only where dH's tiles leave clusters idle.
-    const int64_t most = std::max<int64_t>(1, std::min(l.n_tiles, std::max(kPieceBytes, 2 * l.rows_pad * d.hidden) / (2 * kBN * l.rows_pad)));
-    const int64_t least = most == l.n_tiles ? most : std::max<int64_t>(1, most / 2);
+    // Piece of the vocabulary (in blocks of 256) and runs of the contractions of dH
+    // and dW: the least k-slices on the longest cluster, over the three products of
+    // all pieces, with eight k-slices for each launch's start and end. One piece
+    // where G has room; otherwise up to 64 widths between half the room and all of
+    // it. A further run of a contraction writes and reads its sums once more.
+    const int64_t blocks_v = ceil_div(V, kBN), nb = ceil_div(D, kBN), mb = l.rows_pad / l.tile_m_h;
+    const int64_t slots_h = std::max<int64_t>(sms / l.cta_group_h, 1);
+    const int64_t slots = std::max<int64_t>(sms / l.cta_group, 1);
+    const int64_t most =
+        std::max<int64_t>(1, std::min(blocks_v, std::max(kPieceBytes, 2 * l.rows_pad * D) / (2 * kBN * l.rows_pad)));
+    const int64_t least = most == blocks_v ? most : std::max<int64_t>(1, most / 2);
     const int64_t step = std::max<int64_t>(1, (most - least) / 64);
-    int64_t max_splits = 1;
-    if (mb * nb < 2 * slots)
-        max_splits = std::max<int64_t>(1, std::min<int64_t>(kMaxSplits, kPartialBytes / (4 * l.rows_pad * d.hidden)));
-    max_splits = std::min(max_splits, ceil_div(d.vocab, kBK));
+    const int64_t run_bytes = int64_t(1800) << 10;  // bytes in the time of a k-slice
+    auto splits_most = [&](int64_t tiles, int64_t slots_, int64_t rows, int64_t slices) -> int64_t {
+        if (tiles >= 4 * slots_) return 1;
+        return std::max<int64_t>(1, std::min<int64_t>({kMaxSplits, kPartialBytes / (4 * rows * D), slices}));
+    };
+    auto rounds_of = [](int64_t tiles, int64_t slots_) { return ceil_div(tiles, slots_); };
     int64_t best = -1;
     for (int64_t b = least; b <= most; b += step) {
-        const int64_t pieces = ceil_div(l.n_tiles, b), rest = l.n_tiles - (pieces - 1) * b;
-        auto cost_of = [&](int64_t blocks, int64_t s) {
-            return ceil_div(mb * blocks, slots) * kd + ceil_div(blocks * nb, pairs) * kt +
-                   ceil_div(mb * nb * s, slots) * ceil_div(blocks * (kBN / kBK), s) + 24;
-        };
-        for (int64_t s = 1; s <= max_splits && s <= b * (kBN / kBK); ++s) {
-            const int64_t cost = (pieces - 1) * cost_of(b, s) + cost_of(rest, s) + 2 * (s - 1);
-            if (best < 0 || cost < best) {
-                best = cost;
-                l.piece = b * kBN;
-                l.pieces = pieces;
-                l.splits = s;
+        const int64_t pieces = ceil_div(blocks_v, b), rest = blocks_v - (pieces - 1) * b;
+        auto both = [&](auto cost) { return (pieces - 1) * cost(b) + cost(rest); };
+        const int64_t grad = both([&](int64_t n) {
+            return rounds_of(ceil_div(T, l.tile_m) * ceil_div(n * kBN, l.tile_n), slots) * kd + 8;
+        });
+        int64_t best_h = -1, splits_h = 1, best_w = -1, splits_w = 1;
+        const int64_t most_h = splits_most(mb * nb, slots_h, l.rows_pad, std::min(ceil_div(V, kBK), b * (kBN / kBK)));
+        for (int64_t s = 1; s <= most_h; ++s) {
+            const int64_t c = both([&](int64_t n) {
+                return rounds_of(mb * nb * s, slots_h) * ceil_div(n * (kBN / kBK), s) + 8 + 4 * l.rows_pad * D * (s - 1) / run_bytes;
+            }) + 4 * l.rows_pad * D * (s - 1) / run_bytes;
+            if (best_h < 0 || c < best_h) {
+                best_h = c;
+                splits_h = s;
             }
+        }
+        const int64_t most_w = pieces > 1 ? 1 : splits_most(b * nb, pairs, b * kBN, kt);
+        for (int64_t s = 1; s <= most_w; ++s) {
+            const int64_t c = both([&](int64_t n) { return rounds_of(n * nb * s, pairs) * ceil_div(kt, s) + 8; }) +
+                              (s > 1 ? 4 + 8 * b * kBN * D * s / run_bytes : 0);
+            if (best_w < 0 || c < best_w) {
+                best_w = c;
+                splits_w = s;
+            }
+        }
+        const int64_t cost = grad + best_h + best_w;
+        if (best < 0 || cost < best) {
+            best = cost;
+            l.piece = b * kBN;
+            l.pieces = pieces;
+            l.splits_h = splits_h;
+            l.splits_w = splits_w;
         }
     }
     int64_t at = 256;
@@ -1297,29 +1392,55 @@ static Layout layout_for(const B200VocabLossDesc& d, int64_t sms) {
     l.eq = take(d.top > 0 ? 4 * T * K : 0);
     const int64_t common = at;
     l.zsel = take(4 * T * K);
-    l.part = take(8 * ceil_div(d.vocab, kHalfN) * T);
+    l.part = take(8 * ceil_div(V, l.tile_n / 2) * T);
     l.row_loss = take(4 * T);
-    l.gathered_forward = take(l.gather_forward ? 2 * T * d.hidden : 0);
+    l.gathered_forward = take(l.gather_forward ? 2 * T * D : 0);
     l.bytes_forward = at;
     at = common;
     l.rscale = take(4 * T);
-    l.gathered_backward = take(2 * T * d.hidden);
+    l.gathered_backward = take(2 * T * D);
     l.g = take(2 * T * l.piece);
-    l.partial = take(4 * l.splits * l.rows_pad * d.hidden);
+    l.part_h = take(4 * l.splits_h * l.rows_pad * D);
+    l.part_w = take(l.splits_w > 1 ? 4 * l.splits_w * l.piece * D : 0);
     l.bytes_backward = at;
     return l;
 }
 
 using KernelFn = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, Params);
 
-template <int G>
-static KernelFn kernel_of(int op, bool fp16) {
-    switch (op) {
-        case kStats: return vocab_gemm_kernel<G, kStats, false>;
-        case kGrad: return fp16 ? vocab_gemm_kernel<G, kGrad, true> : vocab_gemm_kernel<G, kGrad, false>;
-        case kDh: return vocab_gemm_kernel<G, kDh, false>;
-        default: return fp16 ? vocab_gemm_kernel<2, kDw, true> : vocab_gemm_kernel<2, kDw, false>;
-    }
+struct Variant {
+    int cta_group, tile_n, op;
+    bool fp16;
+    KernelFn fn;
+    int smem;
+};
+
+template <int kCtaGroup, int kTileN, int kOp, bool kHalf = false>
+static Variant variant() {
+    return {kCtaGroup, kTileN, kOp, kHalf, vocab_gemm_kernel<kCtaGroup, kTileN, kOp, kHalf>, Cfg<kCtaGroup, kTileN>::kSmemBytes};
+}
+
+// Every product in the shapes that the layout can choose.
+static const Variant* variants(int* count) {
+    static const Variant all[] = {
+        variant<2, 256, kStats>(), variant<1, 256, kStats>(), variant<1, 128, kStats>(),
+        variant<2, 256, kStatsShort>(), variant<1, 256, kStatsShort>(), variant<1, 128, kStatsShort>(),
+        variant<2, 256, kGrad, false>(), variant<1, 256, kGrad, false>(), variant<1, 128, kGrad, false>(),
+        variant<2, 256, kGrad, true>(), variant<1, 256, kGrad, true>(), variant<1, 128, kGrad, true>(),
+        variant<2, 256, kDh>(), variant<1, 256, kDh>(),
+        variant<2, 256, kDw, false>(), variant<2, 256, kDw, true>(), variant<2, 256, kDwParts>(),
+    };
+    *count = static_cast<int>(sizeof(all) / sizeof(all[0]));
+    return all;
+}
+
+static const Variant* variant_of(int cta_group, int tile_n, int op, bool fp16) {
+    int n = 0;
+    const Variant* all = variants(&n);
+    const bool half = fp16 && (op == kGrad || op == kDw);
+    for (int i = 0; i < n; ++i)
+        if (all[i].cta_group == cta_group && all[i].tile_n == tile_n && all[i].op == op && all[i].fp16 == half) return all + i;
+    return nullptr;
 }
 
 struct DeviceState {
@@ -1348,14 +1469,11 @@ static int device_state(DeviceState* out) {
     std::lock_guard<std::mutex> lock(mu);
     DeviceState& s = cache[device];
     if (!s.ready) {
-        for (int i = 0; i < 8; ++i) {
-            const int op = i / 2;
-            const void* one = reinterpret_cast<const void*>(kernel_of<1>(op, i % 2));
-            const void* two = reinterpret_cast<const void*>(kernel_of<2>(op, i % 2));
-            if (op != kDw)
-                B200_CUDA_TRY(cudaFuncSetAttribute(one, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<1>::kSmemBytes));
-            B200_CUDA_TRY(cudaFuncSetAttribute(two, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<2>::kSmemBytes));
-        }
+        int n = 0;
+        const Variant* all = variants(&n);
+        for (int i = 0; i < n; ++i)
+            B200_CUDA_TRY(cudaFuncSetAttribute(reinterpret_cast<const void*>(all[i].fn),
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, all[i].smem));
         cudaLaunchConfig_t cfg = {};
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1364,11 +1482,11 @@ static int device_state(DeviceState* out) {
         attr[0].val.clusterDim.z = 1;
         cfg.gridDim = dim3(props.sm_count & ~1, 1, 1);
         cfg.blockDim = dim3(kThreads, 1, 1);
-        cfg.dynamicSmemBytes = Cfg<2>::kSmemBytes;
+        cfg.dynamicSmemBytes = all[0].smem;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
         int clusters = 0;
-        const cudaError_t err = cudaOccupancyMaxActiveClusters(&clusters, reinterpret_cast<const void*>(kernel_of<2>(kStats, false)), &cfg);
+        const cudaError_t err = cudaOccupancyMaxActiveClusters(&clusters, reinterpret_cast<const void*>(all[0].fn), &cfg);
         if (err != cudaSuccess || clusters <= 0) {
             cudaGetLastError();
             clusters = props.sm_count / 2;
@@ -1526,12 +1644,23 @@ static int group_for(int64_t tile_m, int64_t k) {
     return std::max(2, std::min(32, static_cast<int>(rows / tile_m + 0.5)));
 }
 
-static int launch_gemm(const Call& c, int op, int cta_group, int64_t tiles, const CUtensorMap& a0, const CUtensorMap& a1,
-                       const CUtensorMap& b0, const CUtensorMap& b1, const CUtensorMap& dmap, const Params& p) {
+static int launch_gemm(const Call& c, int op, int cta_group, int tile_n, int64_t tiles, const CUtensorMap& a0,
+                       const CUtensorMap& a1, const CUtensorMap& b0, const CUtensorMap& b1, const CUtensorMap& dmap,
+                       const Params& p) {
+    const Variant* v = variant_of(cta_group, tile_n, op, p.fp16);
+    if (v == nullptr) {
+        set_error("internal error: no kernel for product %d with %d x %d tiles", op, kRowsPerCta * cta_group, tile_n);
+        return B200_ERR_INTERNAL;
+    }
     const int64_t slots = cta_group == 2 ? c.dev.pairs : c.dev.sms;
     const int grid = static_cast<int>(std::max<int64_t>(1, std::min(tiles, slots))) * cta_group;
-    return launch(cta_group == 2 ? kernel_of<2>(op, p.fp16) : kernel_of<1>(op, p.fp16), grid, kThreads,
-                  cta_group == 2 ? Cfg<2>::kSmemBytes : Cfg<1>::kSmemBytes, cta_group, true, c.stream, a0, a1, b0, b1, dmap, p);
+    return launch(v->fn, grid, kThreads, v->smem, cta_group, true, c.stream, a0, a1, b0, b1, dmap, p);
+}
+
+// Rows of an A tile that are loaded: all 128, or in single-CTA tiles the rows of
+// the call. What a tile holds beyond them reaches only rows that nobody reads.
+static int a_rows(const B200VocabLossDesc& d, int cta_group) {
+    return cta_group == 1 ? static_cast<int>(std::min<int64_t>(kRowsPerCta, align_up(d.rows, 8))) : kRowsPerCta;
 }
 
 static int begin(const B200VocabLossDesc* d, void* workspace, int64_t bytes, bool backward, void* stream, Call* c) {
@@ -1572,10 +1701,10 @@ static int forward(const B200VocabLossDesc* d, const void* hidden, const void* w
     if (rc != B200_OK) return rc;
     const Layout& l = c.l;
     CUtensorMap a0, a1, b;
-    const int box_n = kBN / l.cta_group;
-    rc = map_2d(c, &a0, hidden, d->rows, d->hidden, d->ld_hidden, kRowsPerCta, kBK);
+    const int box_n = l.tile_n / l.cta_group, box_m = a_rows(*d, l.cta_group);
+    rc = map_2d(c, &a0, hidden, d->rows, d->hidden, d->ld_hidden, box_m, kBK);
     if (rc == B200_OK)
-        rc = l.gather_forward ? map_2d(c, &a1, c.at<void>(l.gathered_forward), d->rows, d->hidden, d->hidden, kRowsPerCta, kBK)
+        rc = l.gather_forward ? map_2d(c, &a1, c.at<void>(l.gathered_forward), d->rows, d->hidden, d->hidden, box_m, kBK)
                               : (a1 = a0, B200_OK);
     if (rc == B200_OK) rc = map_2d(c, &b, weight, d->vocab, d->hidden, d->ld_weight, box_n, kBK);
     if (rc != B200_OK) return rc;
@@ -1587,14 +1716,18 @@ static int forward(const B200VocabLossDesc* d, const void* hidden, const void* w
     p.group_m = group_for(l.tile_m, d->hidden);
     p.zsel = c.at<float>(l.zsel);
     p.part = c.at<float2>(l.part);
-    p.part_ld = d->rows;
-    rc = launch_gemm(c, kStats, l.cta_group, l.rows_pad / l.tile_m * l.n_tiles, a0, a1, b, b, b, p);
+    p.part_ld = ceil_div(d->vocab, l.tile_n / 2);
+    p.a_bytes = box_m * kBK * 2;
+    rc = launch_gemm(c, d->hidden <= kDrain * kBK ? kStatsShort : kStats, l.cta_group, l.tile_n,
+                     ceil_div(d->rows, l.tile_m) * ceil_div(d->vocab, l.tile_n), a0, a1, b, b, b, p);
     if (rc != B200_OK) return rc;
     MergeParams m{};
     m.head = c.head();
     m.part = p.part;
     m.part_ld = p.part_ld;
-    m.tiles = static_cast<int>(ceil_div(d->vocab, kHalfN));
+    m.tiles = static_cast<int>(p.part_ld);
+    // A block for each row up to eight blocks per SM.
+    m.warps_per_row = d->rows <= 8 * c.dev.sms ? kMergeWarps : 1;
     m.rows = static_cast<int>(d->rows);
     m.top = p.top;
     m.reduction = static_cast<int>(d->reduction);
@@ -1608,8 +1741,8 @@ static int forward(const B200VocabLossDesc* d, const void* hidden, const void* w
     m.lse = lse;
     m.row_loss = d->reduction == B200_VL_NONE ? loss : c.at<float>(l.row_loss);
     m.loss = loss;
-    return launch(merge_kernel, static_cast<int>(ceil_div(d->rows, 32)), 32 * kMergeWarps, 0, 1, true,
-                  c.stream, m);
+    return launch(merge_kernel, static_cast<int>(ceil_div(d->rows, kMergeWarps / m.warps_per_row)), 32 * kMergeWarps, 0, 1,
+                  true, c.stream, m);
 }
 
 static int backward(const B200VocabLossDesc* d, const void* hidden, const void* weight, const void* index,
@@ -1634,23 +1767,26 @@ static int backward(const B200VocabLossDesc* d, const void* hidden, const void* 
     const Layout& l = c.l;
     void* hg = c.at<void>(l.gathered_backward);
     void* g = c.at<void>(l.g);
-    CUtensorMap h_k, hg_k, h_mn, hg_mn, w_k, w_mn, g_st, g_k, g_mn, part_st, dw_st;
-    std::memset(&part_st, 0, sizeof(part_st));
+    CUtensorMap h_k, hg_k, h_mn, hg_mn, w_k, w_mn, g_st, g_k, g_mn, dh_st, dw_st;
     std::memset(&dw_st, 0, sizeof(dw_st));
     const int64_t T = d->rows, V = d->vocab, D = d->hidden;
-    rc = map_2d(c, &h_k, hidden, T, D, d->ld_hidden, kRowsPerCta, kBK);
-    if (rc == B200_OK) rc = map_2d(c, &hg_k, hg, T, D, D, kRowsPerCta, kBK);
+    const int box_m = a_rows(*d, l.cta_group), box_m_h = a_rows(*d, l.cta_group_h);
+    rc = map_2d(c, &h_k, hidden, T, D, d->ld_hidden, box_m, kBK);
+    if (rc == B200_OK) rc = map_2d(c, &hg_k, hg, T, D, D, box_m, kBK);
     if (rc == B200_OK) rc = map_2d(c, &h_mn, hidden, T, D, d->ld_hidden, kBK, 64);
     if (rc == B200_OK) rc = map_2d(c, &hg_mn, hg, T, D, D, kBK, 64);
-    if (rc == B200_OK) rc = map_2d(c, &w_k, weight, V, D, d->ld_weight, kBN / l.cta_group, kBK);
+    if (rc == B200_OK) rc = map_2d(c, &w_k, weight, V, D, d->ld_weight, l.tile_n / l.cta_group, kBK);
     if (rc == B200_OK) rc = map_2d(c, &w_mn, weight, V, D, d->ld_weight, kBK, 64);
     if (rc == B200_OK) rc = map_2d(c, &g_st, g, T, l.piece, l.piece, 32, 64);
-    if (rc == B200_OK) rc = map_2d(c, &g_k, g, T, l.piece, l.piece, kRowsPerCta, kBK);
+    if (rc == B200_OK) rc = map_2d(c, &g_k, g, T, l.piece, l.piece, box_m_h, kBK);
     if (rc == B200_OK) rc = map_2d(c, &g_mn, g, T, l.piece, l.piece, kBK, 64);
-    if (rc == B200_OK)
-        rc = encode_tmap_2d(&part_st, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, c.at<void>(l.partial), l.splits * l.rows_pad, D,
-                            D, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (rc == B200_OK && d_weight != nullptr) rc = map_2d(c, &dw_st, d_weight, V, D, D, 32, 64);
+    auto partial_map = [&](CUtensorMap* map, int64_t offset, int64_t rows) {
+        return encode_tmap_2d(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, c.at<void>(offset), rows, D, D, 32, 32,
+                              CU_TENSOR_MAP_SWIZZLE_128B);
+    };
+    if (rc == B200_OK) rc = partial_map(&dh_st, l.part_h, l.splits_h * l.rows_pad);
+    if (rc == B200_OK && d_weight != nullptr)
+        rc = l.splits_w > 1 ? partial_map(&dw_st, l.part_w, l.splits_w * l.piece) : map_2d(c, &dw_st, d_weight, V, D, D, 32, 64);
     if (rc != B200_OK) return rc;
     rc = launch_rows(c, index, teacher, hidden, true, l.gathered_backward, grad_loss);
     for (int64_t v0 = 0; rc == B200_OK && v0 < V; v0 += l.piece) {
@@ -1662,40 +1798,52 @@ static int backward(const B200VocabLossDesc* d, const void* hidden, const void* 
         p.n = static_cast<int>(vp);
         p.k = static_cast<int>(D);
         p.group_m = group_for(l.tile_m, D);
-        rc = launch_gemm(c, kGrad, l.cta_group, l.rows_pad / l.tile_m * ceil_div(vp, kBN), h_k, hg_k, w_k, w_k, g_st, p);
+        p.a_bytes = box_m * kBK * 2;
+        rc = launch_gemm(c, kGrad, l.cta_group, l.tile_n, ceil_div(T, l.tile_m) * ceil_div(vp, l.tile_n), h_k, hg_k, w_k, w_k,
+                         g_st, p);
         if (rc == B200_OK && d_hidden != nullptr) {
             Params q = p;
             q.n = static_cast<int>(D);
             q.k = static_cast<int>(vp);
-            q.group_m = group_for(l.tile_m, l.piece);
-            q.splits = static_cast<int>(l.splits);
+            q.group_m = group_for(l.tile_m_h, l.piece);
+            q.a_bytes = box_m_h * kBK * 2;
+            q.splits = static_cast<int>(l.splits_h);
             q.rows_pad = static_cast<int>(l.rows_pad);
             q.accumulate = v0 > 0;
-            rc = launch_gemm(c, kDh, l.cta_group, l.rows_pad / l.tile_m * ceil_div(D, kBN) * l.splits, g_k, g_k, w_mn,
-                             w_mn, part_st, q);
+            rc = launch_gemm(c, kDh, l.cta_group_h, kBN, l.rows_pad / l.tile_m_h * ceil_div(D, kBN) * l.splits_h, g_k, g_k,
+                             w_mn, w_mn, dh_st, q);
         }
         if (rc == B200_OK && d_weight != nullptr) {
             Params q = p;
             q.m = static_cast<int>(vp);
             q.n = static_cast<int>(D);
             q.group_m = group_for(2 * kRowsPerCta, T);
-            rc = launch_gemm(c, kDw, 2, ceil_div(vp, 2 * kRowsPerCta) * ceil_div(D, kBN), g_mn, g_mn, h_mn, hg_mn, dw_st, q);
+            q.a_bytes = kRowsPerCta * kBK * 2;
+            q.splits = static_cast<int>(l.splits_w);
+            q.rows_pad = static_cast<int>(l.piece);
+            rc = launch_gemm(c, l.splits_w > 1 ? kDwParts : kDw, 2, kBN,
+                             ceil_div(vp, 2 * kRowsPerCta) * ceil_div(D, kBN) * l.splits_w, g_mn, g_mn, h_mn, hg_mn, dw_st, q);
         }
     }
     if (rc != B200_OK) return rc;
     FinishParams f{};
     f.head = c.head();
     f.inv = c.at<int>(l.inv);
-    f.part = c.at<float>(l.partial);
-    f.split_stride = l.rows_pad * D;
-    f.splits = static_cast<int>(l.splits);
+    f.part_h = c.at<float>(l.part_h);
+    f.part_w = d_weight != nullptr && l.splits_w > 1 ? c.at<float>(l.part_w) : nullptr;
+    f.stride_h = l.rows_pad * D;
+    f.stride_w = l.piece * D;
+    f.splits_h = static_cast<int>(l.splits_h);
+    f.splits_w = static_cast<int>(l.splits_w);
     f.rows = static_cast<int>(T);
     f.hidden = static_cast<int>(D);
     f.vocab = static_cast<int>(V);
     f.fp16 = d->dtype == B200_VL_F16;
     f.d_hidden = d_hidden;
     f.d_weight = d_weight;
-    return launch(finish_kernel, static_cast<int>(std::min<int64_t>(T, 8 * c.dev.sms)), 256, 0, 1, true, c.stream, f);
+    const int64_t rows = (d_hidden != nullptr ? T : 0) + (f.part_w != nullptr ? V : 0);
+    return launch(finish_kernel, static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(rows, 8 * c.dev.sms))), 256, 0, 1,
+                  true, c.stream, f);
 }
 
 }  // namespace vl
@@ -1719,10 +1867,11 @@ int b200_vocab_loss_info(const B200VocabLossDesc* desc, int sm_count, B200VocabL
     const b200::vl::Layout l = b200::vl::layout_for(*desc, sm_count);
     out->cta_group = l.cta_group;
     out->tile_m = l.tile_m;
-    out->vocab_tiles = l.n_tiles;
+    out->tile_n = l.tile_n;
     out->piece = l.piece;
     out->pieces = l.pieces;
-    out->splits = l.splits;
+    out->splits_hidden = l.splits_h;
+    out->splits_weight = l.splits_w;
     out->workspace_forward = l.bytes_forward;
     out->workspace_backward = l.bytes_backward;
     const int64_t teacher = desc->top > 0 ? 1 : 0;

@@ -431,12 +431,13 @@ typedef struct B200VocabLossDesc {
 
 /* The host's choices for a call, a function of the sizes and the SM count. */
 typedef struct B200VocabLossInfo {
-    int64_t cta_group;     /* CTAs per tile of the logits: 1 up to 128 rows, else 2 */
-    int64_t tile_m;
-    int64_t vocab_tiles;
+    int64_t cta_group;     /* CTAs per tile of the logits */
+    int64_t tile_m;        /* rows and columns of such a tile */
+    int64_t tile_n;
     int64_t piece;         /* columns of the vocabulary per step of the backward pass */
     int64_t pieces;
-    int64_t splits;        /* runs of the contraction over the vocabulary in d_hidden */
+    int64_t splits_hidden; /* runs of the contraction over the vocabulary in d_hidden */
+    int64_t splits_weight; /* runs of the contraction over the rows in d_weight */
     int64_t workspace_forward;  /* bytes, 256-byte aligned */
     int64_t workspace_backward;
     int64_t launches_forward;
