@@ -134,3 +134,317 @@ def test_distillation_minus_infinity_is_padding():
         logits[5] = -math.inf
     loss, dh, _ = kd(60, 300, 64, 9, reduction="none", change=change)
     assert loss[5] == 0 and not dh[5].any()
+
+
+# --------------------------------------------------------------------------
+# Every tile shape and split that the host can choose
+# --------------------------------------------------------------------------
+@pytest.mark.parametrize("rows,vocab,hidden,want", [
+    (40, 600, 72, dict(cta_group=1, tile_n=128)),                      # one row block, few columns
+    (100, 38000, 72, dict(cta_group=1, tile_n=256)),
+    (250, 18000, 72, dict(cta_group=2, tile_n=256)),
+    (90, 700, 1096, dict(cta_group=1, tile_n=128)),                    # statistics over several units
+    (120, 37801, 520, dict(cta_group=1, tile_n=256)),
+    (1000, 9000, 584, dict(cta_group=2, tile_n=256)),
+    (3000, 300, 136, dict(tile_n=128)),                                # dW in runs over the rows
+])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_cross_entropy_tile_shapes(rows, vocab, hidden, want, dtype):
+    from b200gemm import vocab_loss
+    p = vocab_loss.policy(rows, vocab, hidden)
+    assert {k: p[k] for k in want} == want, p
+    ce(rows, vocab, hidden, dtype, reduction="none", ignored=0.2, seed=3)
+
+
+def test_weight_gradient_in_runs():
+    from b200gemm import vocab_loss
+    p = vocab_loss.policy(5000, 300, 64)
+    assert p["splits_weight"] > 1 and p["splits_hidden"] >= 1
+    ce(5000, 300, 64, reduction="sum")
+    # So few rows with a loss that most runs have none.
+    ce(5000, 300, 64, reduction="sum", ignored=0.995)
+
+
+def test_hidden_gradient_in_runs():
+    from b200gemm import vocab_loss
+    assert vocab_loss.policy(130, 20000, 64)["splits_hidden"] > 1
+    ce(130, 20000, 64, reduction="sum", ignored=0.5)
+
+
+# --------------------------------------------------------------------------
+# How a program calls them
+# --------------------------------------------------------------------------
+def test_same_call_same_bits():
+    a = ce(700, 5000, 264, ignored=0.3, reduction="none", seed=5)
+    b = ce(700, 5000, 264, ignored=0.3, reduction="none", seed=5)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_strides_and_leading_dimensions():
+    from b200gemm import vocab_loss
+    g, h, w = make(6 * 35, 901, 80)
+    wide_h, wide_w = torch.full((6, 35, 104), math.nan, dtype=BF16, device="cuda"), torch.full((901, 96), math.nan, dtype=BF16, device="cuda")
+    wide_h[..., 16:96] = h.reshape(6, 35, 80)
+    wide_w[:, 8:88] = w
+    target = torch.randint(0, 901, (35, 6), generator=g, device="cuda").t()  # not contiguous
+    up = torch.randn(6, 35, generator=g, device="cuda")
+    hs, ws = wide_h[..., 16:96].detach().requires_grad_(), wide_w[:, 8:88].detach().requires_grad_()
+    loss = vocab_loss.linear_cross_entropy(hs, ws, target, reduction="none")
+    assert loss.shape == (6, 35)
+    dh, dw = torch.autograd.grad(loss, (hs, ws), up)
+    plain = run(vocab_loss.linear_cross_entropy, h, w, (target.reshape(-1).contiguous(),), up.reshape(-1), reduction="none")
+    assert torch.equal(loss.detach().reshape(-1), plain[0])
+    assert torch.equal(dh.reshape(-1, 80), plain[1]) and torch.equal(dw, plain[2])
+
+
+def test_single_row_without_leading_dimension():
+    from b200gemm import vocab_loss
+    g, h, w = make(1, 500, 64)
+    t = torch.tensor(7, device="cuda")
+    a = vocab_loss.linear_cross_entropy(h[0], w, t, reduction="none")
+    b = vocab_loss.linear_cross_entropy(h, w, t[None], reduction="none")
+    assert a.shape == () and torch.equal(a, b[0])
+
+
+def test_one_gradient_at_a_time():
+    from b200gemm import vocab_loss
+    g, h, w = make(300, 1000, 136)
+    t = torch.randint(0, 1000, (300,), generator=g, device="cuda")
+    both = run(vocab_loss.linear_cross_entropy, h, w, (t,), torch.ones((), device="cuda"))
+    hg, wg = h.detach().requires_grad_(), w.detach().requires_grad_()
+    vocab_loss.linear_cross_entropy(hg, w, t).backward()
+    assert torch.equal(hg.grad, both[1])
+    vocab_loss.linear_cross_entropy(h, wg, t).backward()
+    assert torch.equal(wg.grad, both[2])
+    loss = vocab_loss.linear_cross_entropy(hg, wg, t)
+    assert torch.equal(torch.autograd.grad(loss, wg, retain_graph=True)[0], both[2])
+    assert torch.equal(torch.autograd.grad(loss, hg, retain_graph=True)[0], both[1])  # twice on one graph
+    with torch.no_grad():
+        assert torch.equal(vocab_loss.linear_cross_entropy(hg, wg, t), both[0])
+
+
+def test_differentiable_once():
+    from b200gemm import vocab_loss
+    g, h, w = make(10, 100, 64)
+    h.requires_grad_()
+    loss = vocab_loss.linear_cross_entropy(h, w, torch.zeros(10, dtype=torch.long, device="cuda"))
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(loss, h, create_graph=True)
+
+
+def test_no_rows():
+    from b200gemm import vocab_loss
+    for reduction in ("none", "mean", "sum"):
+        h = torch.empty(0, 64, dtype=BF16, device="cuda", requires_grad=True)
+        w = torch.ones(30, 64, dtype=BF16, device="cuda", requires_grad=True)
+        loss = vocab_loss.linear_cross_entropy(h, w, torch.empty(0, dtype=torch.long, device="cuda"), reduction=reduction)
+        assert loss.shape == ((0,) if reduction == "none" else ()) and not loss.any()
+        dh, dw = torch.autograd.grad(loss.sum(), (h, w))
+        assert dh.shape == h.shape and dw.shape == w.shape and not dw.any()
+
+
+def test_two_streams_at_once():
+    from b200gemm import vocab_loss
+    jobs = []
+    for seed, (rows, vocab, hidden) in enumerate([(900, 20000, 512), (64, 30000, 1024), (2000, 3000, 256)]):
+        g, h, w = make(rows, vocab, hidden, seed=seed)
+        t = torch.randint(0, vocab, (rows,), generator=g, device="cuda")
+        jobs.append((h, w, t))
+    one = torch.ones((), device="cuda")
+    want = [run(vocab_loss.linear_cross_entropy, h, w, (t,), one) for h, w, t in jobs]
+    streams = [torch.cuda.Stream() for _ in jobs]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for (h, w, t), s in zip(jobs, streams):
+            with torch.cuda.stream(s):
+                got.append(run(vocab_loss.linear_cross_entropy, h, w, (t,), one))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_captured_and_replayed():
+    """Two graphs with their own inputs, replayed in turn and on new data."""
+    from b200gemm import vocab_loss
+    graphs = []
+    for seed, (rows, vocab, hidden) in enumerate([(300, 2000, 128), (40, 5000, 64)]):
+        g, h, w = make(rows, vocab, hidden, seed=seed)
+        t = torch.randint(0, vocab, (rows,), generator=g, device="cuda")
+        one = torch.ones((), device="cuda")
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            run(vocab_loss.linear_cross_entropy, h, w, (t,), one)
+        torch.cuda.current_stream().wait_stream(s)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run(vocab_loss.linear_cross_entropy, h, w, (t,), one)
+        graphs.append((graph, h, w, t, one, out))
+    for step in range(3):
+        for graph, h, w, t, one, out in graphs:
+            h.copy_(torch.randn_like(h))
+            t.copy_(torch.randint_like(t, w.shape[0]))
+            t[::3] = IGNORE
+            one.fill_(step + 0.5)
+        for graph, *_ in graphs:
+            graph.replay()
+        for graph, h, w, t, one, out in graphs:
+            want = run(vocab_loss.linear_cross_entropy, h, w, (t,), one)
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+# --------------------------------------------------------------------------
+# Values
+# --------------------------------------------------------------------------
+def test_target_outside_the_vocabulary():
+    """The row's loss is NaN, and the gradients that it reaches; other rows' are not."""
+    from b200gemm import vocab_loss
+    g, h, w = make(9, 50, 64)
+    t = torch.arange(9, device="cuda")
+    t[2], t[5] = 50, -7
+    loss, dh, dw = run(vocab_loss.linear_cross_entropy, h, w, (t,), torch.ones(9, device="cuda"), reduction="none")
+    bad = torch.zeros(9, dtype=torch.bool, device="cuda")
+    bad[[2, 5]] = True
+    assert torch.equal(loss.isnan(), bad) and torch.equal(dh.isnan().all(1), bad) and torch.equal(dh.isnan().any(1), bad)
+    assert dw.isnan().all()
+    idx = torch.randint(0, 50, (9, 4), generator=g, device="cuda")
+    idx[2, 1] = 50
+    loss = vocab_loss.linear_distillation(h, w, torch.zeros(9, 4, device="cuda"), idx, reduction="none")
+    bad[5] = False
+    assert torch.equal(loss.isnan(), bad)
+    assert vocab_loss.linear_cross_entropy(h, w, t).isnan()
+
+
+def test_upstream_zeros_and_scales():
+    from b200gemm import vocab_loss
+    for dtype in (BF16, FP16):
+        g, h, w = make(140, 400, 64, dtype)
+        t = torch.randint(0, 400, (140,), generator=g, device="cuda")
+        up = torch.zeros(140, device="cuda")
+        _, dh, dw = run(vocab_loss.linear_cross_entropy, h, w, (t,), up, reduction="none")
+        assert not dh.any() and not dw.any()
+        # Loss scales far from 1, as mixed precision uses them, and weights 2^20 apart.
+        up = torch.exp2(torch.randint(-10, 11, (140,), generator=g, device="cuda").float()) * (1 if dtype == FP16 else 2.0 ** 40)
+        kept, idx, q = ref.targets_of(t, IGNORE)
+        check_all(run(vocab_loss.linear_cross_entropy, h, w, (t,), up, reduction="none"),
+                  ref.reference(h, w, kept, idx, q, 1.0, "none", up))
+
+
+@pytest.mark.parametrize("std", [0.0, 3.0])
+def test_flat_and_peaked_logits(std):
+    """All logits equal; logits hundreds apart, where all but one probability vanish."""
+    from b200gemm import vocab_loss
+    g, h, w = make(200, 700, 512, seed=1, std=std or 1.0)
+    if not std:
+        w.zero_()
+    t = torch.randint(0, 700, (200,), generator=g, device="cuda")
+    t[::2] = (h @ w.t()).argmax(1)[::2]
+    up = torch.rand((), device="cuda") + 0.5
+    kept, idx, q = ref.targets_of(t, IGNORE)
+    check_all(run(vocab_loss.linear_cross_entropy, h, w, (t,), up), ref.reference(h, w, kept, idx, q, 1.0, "mean", up))
+
+
+@pytest.mark.parametrize("hidden", [64, 1024])
+def test_infinite_logits(hidden):
+    """Tokens that the projection masks with -inf have no part in the loss."""
+    from b200gemm import vocab_loss
+    g, h, w = make(70, 600, hidden)
+    h = h.abs().clamp(min=0.01)
+    w[100:400] = -math.inf
+    t = torch.randint(0, 100, (70,), generator=g, device="cuda")
+    loss = vocab_loss.linear_cross_entropy(h, w, t, reduction="none")
+    live = torch.cat([w[:100], w[400:]])
+    kept, idx, q = ref.targets_of(t, IGNORE)
+    want = ref.reference(h, live, kept, idx, q, 1.0, "none", torch.ones(70, device="cuda"))
+    ref.check("loss", loss, want[0], want[1])
+    t[3] = 200
+    assert vocab_loss.linear_cross_entropy(h, w, t, reduction="none")[3] == math.inf
+
+
+def test_gradients_against_differences():
+    """Central differences of the loss itself along a direction. hidden +- step * u is exact in bf16; the
+    remainder is the third cumulant of the logits' change over 6, at most R^3 / (36 sqrt(3)) a row for a
+    change of range R; the losses are off by 2^-19 each, the inner product by half a step of its terms."""
+    from b200gemm import vocab_loss
+    g = torch.Generator(device="cuda").manual_seed(11)
+    rows, vocab, hidden, step = 50, 300, 64, 2.0 ** -4
+    h = (torch.randint(-16, 17, (rows, hidden), generator=g, device="cuda") / 16).to(BF16)
+    w = (torch.randn(vocab, hidden, generator=g, device="cuda") / 16).to(BF16)
+    t = torch.randint(0, vocab, (rows,), generator=g, device="cuda")
+    logits, index = torch.randn(rows, 5, generator=g, device="cuda"), torch.randint(0, vocab, (rows, 5), generator=g, device="cuda")
+    u = torch.randint(0, 2, (rows, hidden), generator=g, device="cuda") * 2.0 - 1
+    change = step * (u.double() @ w.double().t())
+    spread = change.max(1).values - change.min(1).values
+    for tau, f in ((1.0, lambda x: vocab_loss.linear_cross_entropy(x, w, t, reduction="none")),
+                   (1.5, lambda x: vocab_loss.linear_distillation(x, w, logits, index, temperature=1.5, reduction="none"))):
+        x = h.detach().requires_grad_()
+        dh, = torch.autograd.grad(f(x).sum(), x)
+        plus, minus = f((h + step * u).to(BF16)), f((h - step * u).to(BF16))
+        got = step * (dh.double() * u).sum(1)
+        diff = (plus.double() - minus.double()) / 2
+        bound = (tau ** 2 * (spread / tau) ** 3 / (36 * math.sqrt(3)) + 2.0 ** -19 * (plus.abs() + minus.abs() + 1)
+                 + step * (2.0 ** -8 + 2.0 ** -8) * dh.double().abs().sum(1) + step * 2.0 ** -8 * tau * 2 * w.double().abs().max(0).values.sum())
+        assert bool(((got - diff).abs() <= bound).all())
+        # The bound is no empty one: it is below the difference itself in most rows.
+        assert float((diff.abs() > bound).double().mean()) > 0.5
+
+
+def test_many_rows():
+    """More rows than a grid's second dimension, and than a pass of the row numbering."""
+    ce(70001, 256, 64, ignored=0.4, reduction="none")
+
+
+def test_weight_beyond_32_bit_offsets():
+    """V x D above 2^31 elements: the last rows of the projection are read and written."""
+    from b200gemm import vocab_loss
+    V, D, T = 262400, 8192, 3
+    assert V * D > 2 ** 31
+    g = torch.Generator(device="cuda").manual_seed(0)
+    w = torch.empty(V, D, dtype=BF16, device="cuda")
+    for v in range(0, V, 16400):
+        w[v:v + 16400] = torch.randn(16400, D, generator=g, device="cuda") * 0.02
+    h = torch.randn(T, D, generator=g, device="cuda").to(BF16)
+    t = torch.tensor([0, V - 1, V // 2], device="cuda")
+    loss, dh, dw = run(vocab_loss.linear_cross_entropy, h, w, (t,), torch.ones(T, device="cuda"), reduction="none")
+    z = torch.cat([h.double() @ w[v:v + 16400].double().t() for v in range(0, V, 16400)], 1)
+    p = torch.softmax(z, 1)
+    dz = (D / 16 + 16) * 2.0 ** -23 * float((h.double().abs() @ w[:16400].double().abs().t()).max()) * 1.2
+    want = torch.logsumexp(z, 1) - z.gather(1, t[:, None])[:, 0]
+    assert bool(((loss.double() - want).abs() <= 2 * dz + 2.0 ** -18 + 2.0 ** -20 * want).all())
+    G = p.scatter_add(1, t[:, None], -torch.ones(T, 1, dtype=torch.float64, device="cuda"))
+    for rows in (slice(0, 40), slice(V // 2 - 20, V // 2 + 20), slice(V - 40, V)):
+        exact = G[:, rows].t() @ h.double()
+        bound = (2.0 ** -8 + 2.0 ** -8 + 2 * dz + 2.0 ** -17) * (G[:, rows].abs().t() @ h.double().abs()) + 2.0 ** -17
+        assert bool(((dw[rows].double() - exact).abs() <= bound).all())
+    assert bool(dw.isfinite().all()) and bool(dh.isfinite().all())
+
+
+# --------------------------------------------------------------------------
+# Together
+# --------------------------------------------------------------------------
+def test_losses_of_one_step_together():
+    """A distillation step: both losses on the same hidden states and projection, gradients added by torch,
+    next to the framework's GEMM, which gives the same logits."""
+    from b200gemm import gemm, vocab_loss
+    rows, vocab, hidden, top = 260, 1200, 128, 12
+    g, h, w = make(rows, vocab, hidden, seed=2)
+    t = torch.randint(0, vocab, (rows,), generator=g, device="cuda")
+    t[-20:] = IGNORE
+    logits = torch.randn(rows, top, generator=g, device="cuda")
+    index = torch.randint(0, vocab, (rows, top), generator=g, device="cuda")
+    index[-20:] = -1
+    hg, wg = h.detach().requires_grad_(), w.detach().requires_grad_()
+    a = vocab_loss.linear_cross_entropy(hg, wg, t)
+    b = vocab_loss.linear_distillation(hg, wg, logits, index, temperature=2.0)
+    (0.25 * a + 0.75 * b).backward()
+    ra = ref.reference(h, w, *ref.targets_of(t, IGNORE), 1.0, "mean", torch.tensor(0.25, device="cuda"))
+    rb = ref.reference(h, w, *ref.teacher_of(logits, index, 2.0), 2.0, "mean", torch.tensor(0.75, device="cuda"))
+    ref.check("ce", a.detach(), ra[0], ra[1])
+    ref.check("kd", b.detach(), rb[0], rb[1])
+    for i, got in ((2, hg.grad), (4, wg.grad)):
+        want = ra[i] + rb[i]
+        ref.check("gradient", got, want, ra[i + 1] + rb[i + 1] + 2.0 ** -8 * (ra[i].abs() + rb[i].abs() + ra[i + 1] + rb[i + 1]))
+    z = gemm.gemm(h, w, out_dtype=torch.float32).double()
+    loss = (torch.logsumexp(z, 1) - z.gather(1, t.clamp(min=0)[:, None])[:, 0])[:-20].mean()
+    assert abs(float(loss) - float(a.detach())) <= 2 * float(ra[1])

@@ -9,6 +9,8 @@ Bounds, element by element, from the roundings that the kernels make:
   themselves (exp2, log, sums of up to 256 terms per tile: 2^-18 relative of the sum of exponentials);
 * G = g (p - q) is rounded to the operands' type (half a step h), p and q are off by a relative 2 dz /
   tau + 2^-18; in half precision, steps below 2^-14 are 2^-24 wide, whatever the value;
+* numbers below 2^-126, the smallest normal number of 32 bits and of bf16, may be zeros: the
+  exponentials (scaled by at most the largest g), and a result;
 * the products with G accumulate n terms in 32 bits, at most (n / 16 + 16 + 16) * 2^-23 of the
   magnitudes' sum (splits and pieces included), and round to the operands' type once.
 """
@@ -70,9 +72,9 @@ def reference(hidden, weight, kept, index, q, tau, reduction, up):
     hs = half_step(dtype)
     rel = 2 * zmax[:, None] / tau + 2.0 ** -18
     E = hs * G.abs() + (tau * g.abs())[:, None] * (p * rel + dense * 2.0 ** -18)
-    if dtype == torch.float16 and n:  # G is scaled to at most 1 before it is rounded
-        E = E + tau * g.abs().max() * 2.0 ** -25
-    tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 2.0 ** -126
+    if n:  # G is scaled to at most 1 before it is rounded
+        E = E + tau * g.abs().max() * tiny
 
     def product(a, e, b):
         d = a @ b
