@@ -242,3 +242,23 @@ def test_bounds_notice_mistakes():
         ref.check("nan", torch.full_like(dh, math.nan), dh, bh)
     with pytest.raises(AssertionError):
         ref.check("shape", dh[:1], dh, bh)
+
+
+# --------------------------------------------------------------------------
+# The command
+# --------------------------------------------------------------------------
+@pytest.mark.parametrize("args", [["--loss", "mse"], ["--iterations", "0"], ["--rows", "0"], ["--ignored", "1.0"],
+                                  ["--temperature", "2.0"], ["--way", "backward"]])
+def test_command_usage_errors(args, capsys):
+    from b200gemm.cli import vocab_loss as cli
+    assert cli.main(args) == 2
+    assert capsys.readouterr().out == ""
+
+
+def test_command_needs_a_gpu(capsys):
+    from b200gemm.cli import vocab_loss as cli
+    if torch.cuda.is_available():
+        pytest.skip("a GPU is visible")
+    assert cli.main([]) == 1
+    got = capsys.readouterr()
+    assert got.out == "" and "ERROR" in got.err

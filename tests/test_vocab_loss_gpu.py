@@ -448,3 +448,15 @@ def test_losses_of_one_step_together():
     z = gemm.gemm(h, w, out_dtype=torch.float32).double()
     loss = (torch.logsumexp(z, 1) - z.gather(1, t.clamp(min=0)[:, None])[:, 0])[:-20].mean()
     assert abs(float(loss) - float(a.detach())) <= 2 * float(ra[1])
+
+
+@pytest.mark.parametrize("args", [["--loss", "ce", "--ignored", "0.25"], ["--loss", "kd", "--top", "9", "--temperature", "2"],
+                                  ["--loss", "ce", "--dtype", "fp16", "--way", "forward"]])
+def test_command(args, capsys):
+    from b200gemm.cli import vocab_loss as cli
+    assert cli.main(args + ["--rows", "300", "--vocab", "5000", "--hidden", "256", "--iterations", "2", "--warmup", "1"]) == 0
+    lines = capsys.readouterr().out.strip().splitlines()
+    assert lines[0].startswith("loss,way,") and len(lines) == (2 if "--way" in args else 3)
+    for line in lines[1:]:
+        r = dict(zip(lines[0].split(","), line.split(",")))
+        assert float(r["ms"]) > 0 and int(r["rows_with_loss"]) == (225 if "0.25" in args else 300)
