@@ -120,6 +120,8 @@ struct Params {
     // Stats, Grad. One target per row (cross entropy): ecol and zsel go by the
     // gathered row, rowmap and eq are null. A teacher's: by the row of the call.
     const int* rowmap;    // gathered row -> row
+    const unsigned short* epos;  // [rows][epos_ld]: first entry at or behind each half tile
+    long long epos_ld;
     const int* ecol;      // [rows][top] ascending target columns, kNoCol behind the last
     const float* eq;      // [rows][top] their probabilities
     float* zsel;          // Stats: [rows][top] logits at the targets
@@ -181,29 +183,6 @@ __device__ __forceinline__ void tma_reduce_add_2d(const void* tmap, uint32_t src
         "cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];"
         ::"l"(reinterpret_cast<uint64_t>(tmap)), "r"(src), "r"(x), "r"(y)
         : "memory");
-}
-
-// a[i], the index uniform in the warp: a branch for the group of 32, then five
-// levels of selects.
-__device__ __forceinline__ float pick_32(const float* a, int i) {
-    float v[16];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = (i & 16) ? a[j + 16] : a[j];
-#pragma unroll
-    for (int w = 8; w; w >>= 1) {
-#pragma unroll
-        for (int j = 0; j < w; ++j) v[j] = (i & w) ? v[j + w] : v[j];
-    }
-    return v[0];
-}
-
-template <int kN>
-__device__ __forceinline__ float pick(const float (&a)[kN], int i) {
-    if constexpr (kN == 128) {
-        if (i >= 96) return pick_32(a + 96, i);
-        if (i >= 64) return pick_32(a + 64, i);
-    }
-    return i >= 32 ? pick_32(a + 32, i) : pick_32(a, i);
 }
 
 // 2^x by the hardware's approximation (absolute error about 2^-22 of the
@@ -577,36 +556,38 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
             const int col0 = w.nb * kTileN + half * kHalfN;  // first column of this warp
             const uint32_t t_lane = tmem_base + half * kHalfN + (static_cast<uint32_t>(q * 32) << 16);
 
-            // The row's targets: position of the first one at or behind the warp's
-            // first column, that column and the next two (read ahead: a row of a
-            // teacher may have several in a tile). What one load gives is only looked
-            // at after the accumulator is there.
+            // The row's targets: position of the first one in the warp's columns and
+            // behind the last, and up to four columns. A row of a teacher may have
+            // several in a tile; a load for each as it is reached would cost the warp its
+            // latency every time, a search for the first one two more (together 14 % of
+            // the statistics of 4096 rows with 128 logits).
             const int grow = row0 + lane;  // row of the products
             const bool active = grow < n_rows;
             const int first = p.v0 + col0;
-            int pos = 0, cur = kNoCol, ahead1 = kNoCol, ahead2 = kNoCol;
+            int pos = 0, end = 0, cur = kNoCol, ahead1 = kNoCol, ahead2 = kNoCol, ahead3 = kNoCol, used = 0;
             long long ebase = grow;
             float2 rg = make_float2(0.0f, 0.0f);
-            auto col_at = [&](int i) { return i < p.top ? __ldg(p.ecol + ebase + i) : kNoCol; };
-            if constexpr (is_stats(kOp) || kOp == kGrad) {
-                if (active) {
-                    if constexpr (kOp == kGrad) rg = __ldg(p.rgrad + grow);
-                    if (p.rowmap == nullptr) {
-                        cur = __ldg(p.ecol + grow);
-                    } else {
-                        ebase = static_cast<long long>(__ldg(p.rowmap + grow)) * p.top;
-                        int hi = p.top;
-                        while (pos < hi) {
-                            const int mid = (pos + hi) >> 1;
-                            if (__ldg(p.ecol + ebase + mid) < first) pos = mid + 1;
-                            else hi = mid;
-                        }
-                        cur = col_at(pos);
-                        ahead1 = col_at(pos + 1);
-                        ahead2 = col_at(pos + 2);
-                    }
+            auto col_at = [&](int i) { return i < end ? __ldg(p.ecol + ebase + i) : kNoCol; };
+            auto load_four = [&]() {
+                cur = col_at(pos);
+                ahead1 = col_at(pos + 1);
+                ahead2 = col_at(pos + 2);
+                ahead3 = col_at(pos + 3);
+            };
+            auto load_targets = [&]() {
+                if (!active) return;
+                if constexpr (kOp == kGrad) rg = __ldg(p.rgrad + grow);
+                if (p.rowmap == nullptr) {
+                    cur = __ldg(p.ecol + grow);
+                    return;
                 }
-            }
+                const int r = __ldg(p.rowmap + grow);
+                const unsigned short* e = p.epos + r * p.epos_ld + first / kHalfN;
+                pos = __ldg(e);
+                end = __ldg(e + 1);
+                ebase = static_cast<long long>(r) * p.top;
+                load_four();
+            };
             // The lowest column left in the warp's rows, relative to the piece.
             auto lowest = [&]() {
                 const int c = __reduce_min_sync(0xffffffffu, cur < first ? kNoCol : cur);
@@ -615,10 +596,14 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
             auto advance = [&]() {
                 cur = ahead1;
                 ahead1 = ahead2;
+                ahead2 = ahead3;
                 ++pos;
-                ahead2 = p.rowmap == nullptr ? kNoCol : col_at(pos + 2);
+                if (p.rowmap != nullptr && (++used & 3) == 0) load_four();
             };
 
+            // The statistics over several units look the targets up between two of them:
+            // the first accumulator of a tile is not kept waiting.
+            if constexpr (kOp == kStatsShort || kOp == kGrad) load_targets();
             if (!wait_unit()) break;
             const uint32_t t_row = t_lane + (unit & 1) * kTileN;
             if constexpr (kOp == kStats) {
@@ -627,9 +612,11 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
                 for (int g = 0; g < kHalfN / 32; ++g) tmem_ld_32x32b_x32(t_row + 32 * g, reinterpret_cast<uint32_t(&)[32]>(acc[32 * g]));
                 tmem_ld_wait();
                 release_unit();
+                load_targets();
                 bool ok = true;
 #pragma unroll 1
                 for (int kb = w.kb0 + kDrain; kb < w.kb1; kb += kDrain) {
+                    if (kb > w.kb0 + kDrain) release_unit();
                     ok = wait_unit();
                     if (!ok) break;
                     const uint32_t t_next = t_lane + (unit & 1) * kTileN;
@@ -641,9 +628,29 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
 #pragma unroll
                         for (int i = 0; i < 32; ++i) acc[32 * g + i] += __uint_as_float(r[i]);
                     }
-                    release_unit();
                 }
                 if (!ok) break;
+                // Logits at the targets: a register cannot be picked by number, a TMEM
+                // column can. Where a row has a target here, the sums go back over the last
+                // unit's accumulator; all lanes read each target's column, those that want
+                // it keep it.
+                int col = lowest();
+                if (col < col0 + kHalfN) {
+                    const uint32_t t_last = t_lane + (unit & 1) * kTileN;
+#pragma unroll
+                    for (int g = 0; g < kHalfN / 32; ++g)
+                        tmem_st_32x32b_x32(t_last + 32 * g, reinterpret_cast<uint32_t(&)[32]>(acc[32 * g]));
+                    tmem_st_wait();
+#pragma unroll 1
+                    for (; col < col0 + kHalfN; col = lowest()) {
+                        const float z = tmem_ld_col(t_last + (col - col0));
+                        if (cur == col + p.v0) {
+                            p.zsel[ebase + pos] = z;
+                            advance();
+                        }
+                    }
+                }
+                release_unit();
                 const int left = p.n - col0;  // columns of the vocabulary in this half
                 if (left <= 0) continue;
                 if (left < kHalfN) {
@@ -656,17 +663,6 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
                 for (int i = 4; i < kHalfN; ++i) m4[i & 3] = fmaxf(m4[i & 3], acc[i]);
                 const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
                 const float ref = -finite_or_zero(m) * p.c2;
-                // Logits at the targets, before the exponentials take their place: the
-                // column is the same for all lanes, the lanes that want it keep it.
-                while (true) {
-                    const int col = lowest();
-                    if (col >= col0 + kHalfN) break;
-                    const float z = pick(acc, col - col0);
-                    if (cur == col + p.v0) {
-                        p.zsel[ebase + pos] = z;
-                        advance();
-                    }
-                }
                 float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int i = 0; i < kHalfN; ++i) s4[i & 3] += exp2_approx(fmaf(acc[i], p.c2, ref));
@@ -833,14 +829,18 @@ struct TeacherParams {
     long long ld_index, ld_teacher;
     int rows, vocab, top;
     float inv_tau;
+    int half;             // columns of a half tile
+    long long epos_ld;
     int* ecol;
     float* eq;
+    unsigned short* epos;
     int* flag;
 };
 
 // A warp turns one row of a teacher's logits into its target distribution:
 // softmax over the entries that are there, sorted by column, entries of one
-// column added up in the order given. 2 x 8 bytes per entry in, 8 out.
+// column added up in the order given. 2 x 8 bytes per entry in, 8 out. It also
+// leaves where in the row each half tile of the vocabulary begins.
 constexpr int kTeacherWarps = 8;
 __global__ void __launch_bounds__(kTeacherWarps * 32) teacher_kernel(const TeacherParams p, int pad) {
     extern __shared__ unsigned long long teacher_smem[];
@@ -900,6 +900,7 @@ __global__ void __launch_bounds__(kTeacherWarps * 32) teacher_kernel(const Teach
         }
     }
     int out = 0;
+    unsigned* cols = reinterpret_cast<unsigned*>(prob + static_cast<size_t>(kTeacherWarps) * pad);
     int* ecol = p.ecol + static_cast<long long>(t) * p.top;
     float* eq = p.eq + static_cast<long long>(t) * p.top;
     for (int base = 0; base < pad; base += 32) {
@@ -917,6 +918,7 @@ __global__ void __launch_bounds__(kTeacherWarps * 32) teacher_kernel(const Teach
                 v += prob[static_cast<unsigned>(key[j])];
             const int o = out + __popc(heads & ((1u << lane) - 1));
             ecol[o] = static_cast<int>(col);
+            cols[o] = col;
             eq[o] = v * inv;
         }
         out += __popc(heads);
@@ -926,6 +928,18 @@ __global__ void __launch_bounds__(kTeacherWarps * 32) teacher_kernel(const Teach
         eq[i] = 0.0f;
     }
     if (lane == 0) p.flag[t] = bad ? kBad : (any ? kLoss : kNoLoss);
+    __syncwarp();
+    unsigned short* epos = p.epos + t * p.epos_ld;
+    for (long long j = lane; j < p.epos_ld; j += 32) {
+        const long long col = j * p.half;
+        int lo = 0, hi = out;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (cols[mid] < col) lo = mid + 1;
+            else hi = mid;
+        }
+        epos[j] = static_cast<unsigned short>(lo);
+    }
 }
 
 struct RowsParams {
@@ -1232,10 +1246,10 @@ struct Layout {
     int cta_group_h;                // tiles of dH, 256 wide
     int64_t tile_m, tile_m_h, piece, pieces, splits_h, splits_w, rows_pad;
     // Offsets in the workspace.
-    int64_t flag, rowmap, inv, ecol, eq;                 // both directions
+    int64_t flag, rowmap, inv, ecol, eq, epos;           // both directions
     int64_t zsel, part, row_loss, gathered_forward;
     int64_t rgrad, gathered_backward, g, part_h, part_w;
-    int64_t ld_gathered, ld_part;                        // row pitches on 128-byte lines
+    int64_t epos_ld, ld_gathered, ld_part;                        // row pitches on 128-byte lines
     int64_t bytes_forward, bytes_backward;
     bool gather_forward;
 };
@@ -1404,6 +1418,9 @@ static Layout layout_for(const B200VocabLossDesc& d, int64_t sms) {
     l.inv = take(4 * T);
     l.ecol = take(4 * T * K);
     l.eq = take(d.top > 0 ? 4 * T * K : 0);
+    // One entry for each half tile of the padded vocabulary and one behind them.
+    l.epos_ld = ceil_div(V, kBN) * (2 * kBN / l.tile_n) + 1;
+    l.epos = take(d.top > 0 ? 2 * T * l.epos_ld : 0);
     const int64_t common = at;
     l.zsel = take(4 * T * K);
     l.part = take(8 * ceil_div(V, l.tile_n / 2) * T);
@@ -1604,13 +1621,16 @@ static int launch_rows(const Call& c, const void* index, const void* teacher, co
         t.vocab = static_cast<int>(d.vocab);
         t.top = static_cast<int>(d.top);
         t.inv_tau = static_cast<float>(1.0 / d.temperature);
+        t.half = l.tile_n / 2;
+        t.epos_ld = l.epos_ld;
+        t.epos = c.at<unsigned short>(l.epos);
         t.ecol = c.at<int>(l.ecol);
         t.eq = c.at<float>(l.eq);
         t.flag = c.at<int>(l.flag);
         int pad = 2;
         while (pad < t.top) pad *= 2;
         const int rc = launch(teacher_kernel, static_cast<int>(ceil_div(d.rows, kTeacherWarps)), kTeacherWarps * 32,
-                              kTeacherWarps * pad * 12, 1, false, c.stream, t, pad);
+                              kTeacherWarps * pad * 16, 1, false, c.stream, t, pad);
         if (rc != B200_OK) return rc;
     }
     RowsParams r{};
@@ -1651,6 +1671,8 @@ static Params base_params(const Call& c) {
     p.rows = static_cast<int>(d.rows);
     p.splits = 1;
     p.rowmap = d.top > 0 ? c.at<int>(c.l.rowmap) : nullptr;
+    p.epos = c.at<unsigned short>(c.l.epos);
+    p.epos_ld = c.l.epos_ld;
     p.ecol = c.at<int>(c.l.ecol);
     p.eq = d.top > 0 ? c.at<float>(c.l.eq) : nullptr;
     p.top = static_cast<int>(std::max<int64_t>(d.top, 1));
