@@ -114,6 +114,7 @@ struct Params {
     int v0;               // first vocabulary row of the piece
     int group_m;          // m-blocks per raster group
     int a_bytes;          // bytes of an A tile: rows beyond the call's are not loaded
+    int early;            // Stats: the operands are the call's own, all rows in their order
     int splits;           // Dh, DwParts: runs of the contraction
     int rows_pad;         // Dh, DwParts: rows between two splits' partial sums
     int accumulate;       // Dh: 1 add to the partial sums, 0 write them
@@ -198,6 +199,12 @@ __device__ __forceinline__ float exp2_approx(float x) {
 // inf - inf).
 __device__ __forceinline__ float finite_or_zero(float m) { return fabsf(m) == INFINITY ? 0.0f : m; }
 
+// What a sum of exponentials against `from` is multiplied by to stand against `to`.
+// A sum against -inf is empty: nothing, not 0 times the overflow of exp(0 - to).
+__device__ __forceinline__ float rescale(float from, float to, float c2) {
+    return from == -INFINITY ? 0.0f : exp2_approx((finite_or_zero(from) - finite_or_zero(to)) * c2);
+}
+
 template <int kCtaGroup, int kTileN, int kOp, bool kHalf>
 __global__ void __launch_bounds__(kThreads, 1)
 vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmA1,
@@ -212,11 +219,11 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
     constexpr bool kBMn = kOp == kDh || is_dw(kOp);
     constexpr int kBoxBytes = 64 * kBK * 2;  // an MN-major box
 
-    int* const status = &p.head->status;
+    int* const status_word = &p.head->status;
     // Launch contract: uniform across the grid, checked before any barrier.
     if (blockDim.x != kThreads || blockDim.y != 1 || blockDim.z != 1 ||
         (kPair && cluster_nctarank() != 2) || (gridDim.x % kCtaGroup) != 0) {
-        if (threadIdx.x == 0) report_status(status, B200_DEV_BAD_LAUNCH);
+        if (threadIdx.x == 0) report_status(status_word, B200_DEV_BAD_LAUNCH);
         return;
     }
 
@@ -274,11 +281,18 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
     if constexpr (kPair) cluster_sync(); else __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
-    // Nothing in global memory is touched before the previous kernel is done.
-    griddep_wait();
+    // Nothing in global memory is touched before the previous kernel is done, with
+    // one exception: where the operands are the call's own and no row is left out
+    // (early), the first tile is loaded and multiplied meanwhile. The kernels before
+    // this one in the call write neither, and the first of them began when everything
+    // before the call was done. Each role then waits before it touches the workspace, the
+    // status word included (one token over 128256 x 4096: 3 us of 187).
+    const bool early = is_stats(kOp) && p.early;
+    int* status = early ? nullptr : status_word;
+    if (!early) griddep_wait();
 
-    const int n_rows = p.head->n_rows;
-    const bool compact = p.head->compact != 0;
+    const int n_rows = early ? p.rows : p.head->n_rows;
+    const bool compact = !early && p.head->compact != 0;
     // Of H, the gathered copy where rows were left out. Without a single row the
     // products still run over one block of zero rows: dW is then written as zeros.
     const CUtensorMap* tmA = ((is_stats(kOp) || kOp == kGrad) && compact) ? &tmA1 : &tmA0;
@@ -334,6 +348,7 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
             // The first tile is the cluster's own number, later ones come from the
             // launch-wide counter.
             int next = cluster;
+            bool waited = !early;
             while (ok) {
                 int t;
                 if (rank == 0) {
@@ -344,6 +359,7 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
                     t = next;
                     if (t >= num_tiles) {
                         t = -1;
+                        if (!waited) griddep_wait();
                         __threadfence();
                         if (atomicAdd(&p.head->counter[1], 1) == num_clusters - 1) {
                             // Every cluster has made its last fetch: ready for the next launch.
@@ -377,7 +393,7 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
                 const int fetch_kb = max(w.kb0, w.kb1 - 2 * kStages);
                 if (rank == 0 && w.kb0 == w.kb1) next = atomicAdd(&p.head->counter[0], 1) + num_clusters;
                 for (int kb = w.kb0; kb < w.kb1; ++kb) {
-                    if (rank == 0 && kb == fetch_kb) next = atomicAdd(&p.head->counter[0], 1) + num_clusters;
+                    if (rank == 0 && kb == fetch_kb && waited) next = atomicAdd(&p.head->counter[0], 1) + num_clusters;
                     if (!mbar_wait(empty0 + 8 * stage, phase ^ 1, status, p.timeout_ns,
                                    B200_DEV_TIMEOUT_PRODUCER)) {
                         ok = false;
@@ -411,8 +427,15 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
                     ++issued;
                     if (++stage == kStages) { stage = 0; phase ^= 1; }
                 }
+                if (!waited) {
+                    griddep_wait();
+                    status = status_word;
+                    waited = true;
+                    if (rank == 0) next = atomicAdd(&p.head->counter[0], 1) + num_clusters;
+                }
             }
-            if (status_failed(status) && rank == 0) {
+            if (!waited) griddep_wait();
+            if (status_failed(status_word) && rank == 0) {
                 // The launch is being abandoned: before this CTA (pair) exits, wait
                 // (bounded) for the loads it still has in flight into its ring.
                 const unsigned long long drain_ns = min(p.timeout_ns, 100000000ull);
@@ -491,11 +514,19 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
                         ++unit;
                     }
                 }
+                if (status == nullptr) {
+                    griddep_wait();
+                    status = status_word;
+                }
             }
         }
         __syncwarp();
     } else {
         // ----------------------------------------------------------- epilogue
+        if (early) {
+            griddep_wait();
+            status = status_word;
+        }
         const int q = warp & 3;  // TMEM lane quadrant this warp may access
         const int half = (warp - 2) >> 2;
         const uint32_t sbuf = sbase + C::kEpiOffset + (warp - 2) * kEpiBufBytes;
@@ -691,7 +722,7 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
                     for (int i = 0; i < 32; ++i) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(r[i]));
                     const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
                     const float ref = -finite_or_zero(mx) * p.c2;
-                    float s4[4] = {s * exp2_approx(fmaf(finite_or_zero(m), p.c2, ref)), 0.0f, 0.0f, 0.0f};
+                    float s4[4] = {s * rescale(m, mx, p.c2), 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int i = 0; i < 32; ++i) s4[i & 3] += exp2_approx(fmaf(__uint_as_float(r[i]), p.c2, ref));
                     s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
@@ -849,6 +880,7 @@ __global__ void __launch_bounds__(kTeacherWarps * 32) teacher_kernel(const Teach
     float* prob = reinterpret_cast<float*>(teacher_smem + static_cast<size_t>(kTeacherWarps) * pad) +
                   static_cast<size_t>(warp) * pad;
     const int t = blockIdx.x * kTeacherWarps + warp;
+    griddep_launch_dependents();
     if (t >= p.rows) return;
     float mx = -INFINITY;
     bool any = false, bad = false, nan = false;
@@ -968,6 +1000,10 @@ __global__ void __launch_bounds__(1024) rows_kernel(const RowsParams p) {
     __shared__ int warp_sum[32];
     __shared__ float warp_max[32];
     __shared__ int base;
+    // What follows may set itself up, and load what the call was given, from the
+    // start; it waits for this kernel's end before it looks at the workspace.
+    griddep_launch_dependents();
+    griddep_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) base = 0;
     float gmax = 0.0f;
@@ -1058,7 +1094,6 @@ __global__ void __launch_bounds__(1024) rows_kernel(const RowsParams p) {
         }
         *p.head = h;
     }
-    griddep_launch_dependents();
 }
 
 // Gathers the rows that have a loss; a block of rows of zeros follows the last
@@ -1106,48 +1141,56 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const MergePara
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int row = blockIdx.x * (kMergeWarps / p.warps_per_row) + warp / p.warps_per_row;
     const int i = row < p.rows ? p.inv[row] : -1;
+    const int f = row < p.rows ? p.flag[row] : kNoLoss;
+    const bool failed = p.head->status != 0;
+    const float z_one = i >= 0 && p.eq == nullptr ? p.zsel[i] : 0.0f;
+    // The maximum first, then the sums against it: eight parts of a lane at a time,
+    // then the lanes, then the warps.
     float m = -INFINITY, s = 0.0f;
-    auto join = [&](float m2, float s2) {
-        const float mx = fmaxf(m, m2);
-        const float ref = -finite_or_zero(mx) * p.c2;
-        s = s * exp2_approx(fmaf(finite_or_zero(m), p.c2, ref)) + s2 * exp2_approx(fmaf(finite_or_zero(m2), p.c2, ref));
-        m = mx;
-    };
+    auto scale = [&](float from, float to) { return rescale(from, to, p.c2); };
     if (i >= 0) {
         const float2* part = p.part + i * p.part_ld;
         const int step = 32 * p.warps_per_row;
-#pragma unroll 8
-        for (int j = (warp % p.warps_per_row) * 32 + lane; j < p.tiles; j += step) {
-            const float2 v = part[j];
-            join(v.x, v.y);
+        for (int j0 = (warp % p.warps_per_row) * 32 + lane; j0 < p.tiles; j0 += 8 * step) {
+            float2 v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = j0 + j * step < p.tiles ? part[j0 + j * step] : make_float2(-INFINITY, 0.0f);
+            float mx = m;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) mx = fmaxf(mx, v[j].x);
+            s *= scale(m, mx);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s += v[j].y * scale(v[j].x, mx);
+            m = mx;
         }
     }
-    for (int o = 16; o; o >>= 1) {
-        const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-        join(m2, s2);
-    }
+    float mx = m;
+    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    s *= scale(m, mx);
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    m = mx;
     if (p.warps_per_row > 1) {
         if (lane == 0) {
             sm[warp] = m;
             ss[warp] = s;
         }
         __syncthreads();
-        m = sm[0];
-        s = ss[0];
-        for (int w = 1; w < kMergeWarps; ++w) join(sm[w], ss[w]);
+        for (int w = 0; w < kMergeWarps; ++w) m = fmaxf(m, sm[w]);
+        s = 0.0f;
+        for (int w = 0; w < kMergeWarps; ++w) s += ss[w] * scale(sm[w], m);
     }
     const float lse = i >= 0 ? logf(s) + finite_or_zero(m) * p.inv_tau : 0.0f;
     const bool leader = row < p.rows && warp % p.warps_per_row == 0;
     if (leader && lane == 0) p.lse[row] = lse;
-    const bool failed = p.head->status != 0;
     if (leader) {
-        const int f = p.flag[row];
         float v = 0.0f;
-        if (f == kLoss) {
-            const long long e = p.eq == nullptr ? i : static_cast<long long>(row) * p.top;
+        if (f == kLoss && p.eq == nullptr) {
+            v = lse - z_one;
+        } else if (f == kLoss) {
+            const long long e = static_cast<long long>(row) * p.top;
             for (int k = lane; k < p.top; k += 32) {
-                const float qv = p.eq == nullptr ? 1.0f : p.eq[e + k];
-                if (qv != 0.0f) v += qv * ((p.eq == nullptr ? 0.0f : logf(qv)) + (lse - p.zsel[e + k] * p.inv_tau));
+                const float qv = p.eq[e + k];
+                if (qv != 0.0f) v += qv * (logf(qv) + (lse - p.zsel[e + k] * p.inv_tau));
             }
             for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
             v *= p.tau2;
@@ -1653,7 +1696,7 @@ static int launch_rows(const Call& c, const void* index, const void* teacher, co
     r.lse = lse;
     r.rgrad = grad != nullptr ? c.at<float2>(l.rgrad) : nullptr;
     r.tau = static_cast<float>(d.temperature);
-    int rc = launch(rows_kernel, 1, 1024, 0, 1, false, c.stream, r);
+    int rc = launch(rows_kernel, 1, 1024, 0, 1, d.top > 0, c.stream, r);
     if (rc != B200_OK || !gather) return rc;
     const int vecs = static_cast<int>(d.hidden / 8);
     return launch(gather_kernel, static_cast<int>(std::min<int64_t>(d.rows, 8 * c.dev.sms)), 256, 0, 1, true, c.stream,
@@ -1758,6 +1801,7 @@ static int forward(const B200VocabLossDesc* d, const void* hidden, const void* w
     p.group_m = group_for(l.tile_m, d->hidden);
     p.zsel = c.at<float>(l.zsel);
     p.part = c.at<float2>(l.part);
+    p.early = !l.gather_forward;
     p.part_ld = ceil_div(d->vocab, l.tile_n / 2);
     p.a_bytes = box_m * kBK * 2;
     rc = launch_gemm(c, d->hidden <= kDrain * kBK ? kStatsShort : kStats, l.cta_group, l.tile_n,

@@ -346,6 +346,22 @@ def test_flat_and_peaked_logits(std):
 
 
 @pytest.mark.parametrize("hidden", [64, 1024])
+@pytest.mark.parametrize("shift", [-300.0, 300.0])
+@pytest.mark.parametrize("vocab", [1, 100, 1000, 5000])
+def test_logits_far_from_zero(hidden, shift, vocab):
+    """All logits near the same large number: exp of it, or of its negative, is beyond 32 bits."""
+    from b200gemm import vocab_loss
+    g, h, w = make(150, vocab, hidden)
+    h[:, 0] = 20.0
+    w[:, 0] = shift / 20
+    t = torch.randint(0, vocab, (150,), generator=g, device="cuda")
+    up = torch.rand(150, generator=g, device="cuda")
+    kept, idx, q = ref.targets_of(t, IGNORE)
+    check_all(run(vocab_loss.linear_cross_entropy, h, w, (t,), up, reduction="none"),
+              ref.reference(h, w, kept, idx, q, 1.0, "none", up))
+
+
+@pytest.mark.parametrize("hidden", [64, 1024])
 def test_infinite_logits(hidden):
     """Tokens that the projection masks with -inf have no part in the loss."""
     from b200gemm import vocab_loss
