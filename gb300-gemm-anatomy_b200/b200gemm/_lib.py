@@ -180,8 +180,9 @@ SIGNATURES = {
     "b200_vocab_loss_desc_size": (ctypes.c_size_t, []),
     "b200_vocab_loss_info_size": (ctypes.c_size_t, []),
     "b200_vocab_loss_info": (_INT, [ctypes.POINTER(VocabLossDesc), _INT, ctypes.POINTER(VocabLossInfo)]),
-    "b200_vocab_loss_forward": (_INT, [ctypes.POINTER(VocabLossDesc), _P, _P, _P, _P, _P, _P, _P, _I64, _P]),
-    "b200_vocab_loss_backward": (_INT, [ctypes.POINTER(VocabLossDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P,
+    "b200_vocab_loss_forward": (_INT, [ctypes.POINTER(VocabLossDesc), _P, _P, _P, _P, _P, _P, _P, _P, _I64,
+                                       _P]),
+    "b200_vocab_loss_backward": (_INT, [ctypes.POINTER(VocabLossDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P,
                                         _I64, _P]),
     "b200_selftest_bounded_wait": (_INT, [ctypes.c_ulonglong, _P, _P]),
     "b200_selftest_occupy": (_INT, [_INT, _INT, ctypes.c_ulonglong, _P]),

@@ -18,6 +18,7 @@ A kernel wait that runs out (``B200_WAIT_TIMEOUT_MS``) leaves NaN in the results
 from __future__ import annotations
 
 import ctypes
+import operator
 
 import torch
 
@@ -72,8 +73,12 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
     ``[0, V)`` makes the loss NaN. reduction: "none" (shape of target), "mean" over the rows with a
     loss (0 without any) or "sum"; fp32. The gradients have the operands' type.
     """
-    if not isinstance(ignore_index, int) or not -2 ** 63 <= ignore_index < 2 ** 63:
-        raise ValueError(f"ignore_index={ignore_index!r} is no 64-bit integer")
+    try:
+        ignore_index = operator.index(ignore_index)
+    except TypeError:
+        raise ValueError(f"ignore_index={ignore_index!r} is no integer") from None
+    if not -2 ** 63 <= ignore_index < 2 ** 63:
+        raise ValueError(f"ignore_index={ignore_index} is no 64-bit integer")
     return _call(hidden, weight, target, None, ("hidden", "weight", "target"), ignore_index, reduction, 1.0)
 
 
@@ -84,7 +89,7 @@ def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_logi
 
     teacher_logits: ``... x K`` fp32, bf16 or fp16, the logits a teacher kept for each row;
     teacher_index: ``... x K`` int32 or int64, their tokens, in any order; K from 1 to 256. q is the
-    softmax of ``teacher_logits / temperature`` over the row's entries: those with a negative index
+    softmax of ``teacher_logits / temperature`` (from 2^-20 to 2^20) over the row's entries: those with a negative index
     or a logit of -inf are padding, entries of the same token add up. A row of nothing but padding
     has no loss, like an ignored target in ``linear_cross_entropy``; an index of V or more makes it
     NaN. The teacher gets no gradient. Everything else as in ``linear_cross_entropy``.

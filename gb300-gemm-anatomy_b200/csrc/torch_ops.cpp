@@ -102,14 +102,14 @@ struct VocabLoss : public torch::autograd::Function<VocabLoss> {
         check_rc(g_api.info(&d, at::cuda::getCurrentDeviceProperties()->multiProcessorCount, &p.info),
                  "b200_vocab_loss_info");
         Tensor loss = per_row ? at::empty({rows}, f32) : at::empty({}, f32);
-        Tensor lse = at::empty({rows}, f32);
+        Tensor lse = at::empty({rows}, f32), target_logp = at::empty({rows, teacher ? d.top : 1}, f32);
         Tensor ws = workspace(p.info.workspace_forward, hidden);
         check_rc(g_api.forward(&d, hidden.const_data_ptr(), weight.const_data_ptr(), index.const_data_ptr(),
                                teacher ? teacher->const_data_ptr() : nullptr, loss.mutable_data_ptr<float>(),
-                               lse.mutable_data_ptr<float>(), ws.mutable_data_ptr(), p.info.workspace_forward,
+                               lse.mutable_data_ptr<float>(), target_logp.mutable_data_ptr<float>(), ws.mutable_data_ptr(), p.info.workspace_forward,
                                c10::cuda::getCurrentCUDAStream().stream()),
                  "b200_vocab_loss_forward");
-        ctx->save_for_backward({hidden, weight, index, teacher.value_or(Tensor()), lse});
+        ctx->save_for_backward({hidden, weight, index, teacher.value_or(Tensor()), lse, target_logp});
         ctx->saved_data["problem"] = pack(p);
         return loss;
     }
@@ -127,7 +127,7 @@ struct VocabLoss : public torch::autograd::Function<VocabLoss> {
             return {dh, dw, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
         }
         const Problem p = unpack(ctx->saved_data["problem"]);
-        const Tensor &index = saved[2], &teacher = saved[3], &lse = saved[4];
+        const Tensor &index = saved[2], &teacher = saved[3], &lse = saved[4], &target_logp = saved[5];
         const c10::cuda::CUDAGuard guard(hidden.device());
         const Tensor grad = grads[0].to(at::kFloat).contiguous();
         if (want_h) dh = at::empty(hidden.sizes(), hidden.options());
@@ -136,7 +136,8 @@ struct VocabLoss : public torch::autograd::Function<VocabLoss> {
             Tensor ws = workspace(p.info.workspace_backward, hidden);
             check_rc(g_api.backward(&p.desc, hidden.const_data_ptr(), weight.const_data_ptr(), index.const_data_ptr(),
                                     teacher.defined() ? teacher.const_data_ptr() : nullptr,
-                                    lse.const_data_ptr<float>(), grad.const_data_ptr<float>(),
+                                    lse.const_data_ptr<float>(), target_logp.const_data_ptr<float>(),
+                                    grad.const_data_ptr<float>(),
                                     want_h ? dh.mutable_data_ptr() : nullptr, want_w ? dw.mutable_data_ptr() : nullptr,
                                     ws.mutable_data_ptr(), p.info.workspace_backward,
                                     c10::cuda::getCurrentCUDAStream().stream()),
@@ -175,8 +176,8 @@ Tensor vocab_loss(const Tensor& hidden, const Tensor& weight, const Tensor& inde
         TORCH_CHECK_VALUE(teacher->size(-1) >= 1 && teacher->size(-1) <= 256,
                           "a teacher's row holds 1 to 256 logits, got ", teacher->size(-1));
         TORCH_CHECK_VALUE(!teacher->requires_grad(), "teacher_logits gets no gradient: detach it");
-        TORCH_CHECK_VALUE(temperature > 0.0 && std::isfinite(temperature),
-                          "temperature must be positive and finite, got ", temperature);
+        TORCH_CHECK_VALUE(temperature >= 0x1p-20 && temperature <= 0x1p20,
+                          "temperature must be between 2^-20 and 2^20, got ", temperature);
     } else {
         TORCH_CHECK_VALUE(is_index(index.scalar_type()), "target must be int32 or int64, got ", index.scalar_type());
         TORCH_CHECK_VALUE(index.sizes() == lead, "target has shape ", index.sizes(), ", expected ", lead);

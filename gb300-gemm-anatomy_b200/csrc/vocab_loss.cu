@@ -118,17 +118,17 @@ struct Params {
     int splits;           // Dh, DwParts: runs of the contraction
     int rows_pad;         // Dh, DwParts: rows between two splits' partial sums
     int accumulate;       // Dh: 1 add to the partial sums, 0 write them
-    // Stats, Grad. One target per row (cross entropy): ecol and zsel go by the
-    // gathered row, rowmap and eq are null. A teacher's: by the row of the call.
+    // Stats, Grad. One target per row (cross entropy): ecol and zsel (Stats) go by
+    // the gathered row, rowmap and eq are null. A teacher's: by the row of the call.
     const int* rowmap;    // gathered row -> row
     const unsigned short* epos;  // [rows][epos_ld]: first entry at or behind each half tile
     long long epos_ld;
     const int* ecol;      // [rows][top] ascending target columns, kNoCol behind the last
     const float* eq;      // [rows][top] their probabilities
-    float* zsel;          // Stats: [rows][top] logits at the targets
+    float* zsel;          // Stats: [rows][top] logits at the targets; Grad: their log-probabilities
     float2* part;         // Stats: [gathered row][part_ld half tiles] (maximum, sum of exponentials)
     long long part_ld;
-    const float2* rgrad;  // Grad: [gathered row] (g_t, -lse_t log2(e))
+    const float4* rgrad;  // Grad: [gathered row] (g_t, -lse_t log2(e), g_t (p - 1) at the one target, 0)
     int top;
     float c2;             // log2(e) / tau
 };
@@ -597,7 +597,7 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
             const int first = p.v0 + col0;
             int pos = 0, end = 0, cur = kNoCol, ahead1 = kNoCol, ahead2 = kNoCol, ahead3 = kNoCol, used = 0;
             long long ebase = grow;
-            float2 rg = make_float2(0.0f, 0.0f);
+            float4 rg = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             auto col_at = [&](int i) { return i < end ? __ldg(p.ecol + ebase + i) : kNoCol; };
             auto load_four = [&]() {
                 cur = col_at(pos);
@@ -693,10 +693,10 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
 #pragma unroll
                 for (int i = 4; i < kHalfN; ++i) m4[i & 3] = fmaxf(m4[i & 3], acc[i]);
                 const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-                const float ref = -finite_or_zero(m) * p.c2;
+                const float ref = finite_or_zero(m);
                 float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int i = 0; i < kHalfN; ++i) s4[i & 3] += exp2_approx(fmaf(acc[i], p.c2, ref));
+                for (int i = 0; i < kHalfN; ++i) s4[i & 3] += exp2_approx((acc[i] - ref) * p.c2);
                 if (active)
                     p.part[grow * p.part_ld + 2 * w.nb + half] =
                         make_float2(m, (s4[0] + s4[1]) + (s4[2] + s4[3]));
@@ -721,10 +721,10 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
 #pragma unroll
                     for (int i = 0; i < 32; ++i) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(r[i]));
                     const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-                    const float ref = -finite_or_zero(mx) * p.c2;
+                    const float ref = finite_or_zero(mx);
                     float s4[4] = {s * rescale(m, mx, p.c2), 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) s4[i & 3] += exp2_approx(fmaf(__uint_as_float(r[i]), p.c2, ref));
+                    for (int i = 0; i < 32; ++i) s4[i & 3] += exp2_approx((__uint_as_float(r[i]) - ref) * p.c2);
                     s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
                     m = mx;
                     // Logits at the targets: all lanes read the column, the lanes that
@@ -773,21 +773,23 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
                     for (int i = 0; i < 32; ++i) pk[i] = active ? pk[i] : 0u;
                     if (row0 >= p.rows) continue;  // nothing of the call in these rows
                     stage_chunk(pk);
-                    // The targets' columns again, from the unrounded logit: p - q.
-                    while (true) {
-                        const int col = lowest();
-                        if (col >= x + 64) break;
-                        const float z = tmem_ld_col(t_row + (col - col0));
-                        if (cur == col + p.v0) {
-                            const float qv = p.eq == nullptr ? 1.0f : __ldg(p.eq + ebase + pos);
-                            const float g = rg.x * (exp2_approx(fmaf(z, p.c2, rg.y)) - qv);
-                            const int i = col - x;
-                            asm volatile("st.shared.u16 [%0], %1;"
-                                         ::"r"(row_addr + (((i >> 3) ^ (lane & 7)) << 4) + (i & 7) * 2),
-                                         "h"(static_cast<uint16_t>(pack(g, 0.0f) & 0xffffu)) : "memory");
-                            advance();
+                    // The targets' columns again, p - q from the forward pass's
+                    // log-probabilities: where p is near q, this product's logits (added
+                    // up without rounding to nearest) against a rounded lse are too far off.
+                    const int lo = p.v0 + x;
+                    while (cur >= lo && cur < lo + 64) {
+                        float g = rg.z;
+                        if (p.rowmap != nullptr) {
+                            const float logp = __ldg(p.zsel + ebase + pos), qv = __ldg(p.eq + ebase + pos);
+                            g = rg.x * (exp2_approx(logp * kLog2e) - qv);
                         }
+                        const int i = cur - lo;
+                        asm volatile("st.shared.u16 [%0], %1;"
+                                     ::"r"(row_addr + (((i >> 3) ^ (lane & 7)) << 4) + (i & 7) * 2),
+                                     "h"(static_cast<uint16_t>(pack(g, 0.0f) & 0xffffu)) : "memory");
+                        advance();
                     }
+                    __syncwarp();
                     store_chunk(x, row0, false);
                 }
                 release_unit();
@@ -989,7 +991,8 @@ struct RowsParams {
     int* inv;             // row -> gathered row, -1 without a loss
     const float* grad;    // backward: what comes from above
     const float* lse;
-    float2* rgrad;        // [gathered row] (g_t, -lse_t log2(e))
+    const float* target_logp;
+    float4* rgrad;        // see Params
     float tau;
 };
 
@@ -1059,7 +1062,9 @@ __global__ void __launch_bounds__(1024) rows_kernel(const RowsParams p) {
             if (p.target != nullptr) p.ecol[i] = col[j];
             if (p.rgrad == nullptr) continue;
             const float g = p.reduction == B200_VL_NONE ? p.grad[t] : 1.0f;
-            p.rgrad[i] = make_float2(f[j] == kBad ? NAN : g, -p.lse[t] * kLog2e);
+            // p - 1 at the one target, without the difference of two numbers near 1.
+            const float below = p.target != nullptr ? expm1f(p.target_logp[t]) : 0.0f;
+            p.rgrad[i] = f[j] == kBad ? make_float4(NAN, NAN, NAN, 0.0f) : make_float4(g, -p.lse[t] * kLog2e, g * below, 0.0f);
             gmax = fabsf(g) > gmax || g != g ? fabsf(g) : gmax;  // a NaN stays
         }
         __syncthreads();
@@ -1077,7 +1082,10 @@ __global__ void __launch_bounds__(1024) rows_kernel(const RowsParams p) {
         for (int i = 0; i < 32; ++i) gmax = warp_max[i] > gmax || warp_max[i] != warp_max[i] ? warp_max[i] : gmax;
         // At most 1, so that G fits half precision whatever the loss is scaled by.
         const float unit = gmax > 0.0f ? gmax : 1.0f;
-        for (int i = tid; i < n_valid; i += 1024) p.rgrad[i].x /= unit;
+        for (int i = tid; i < n_valid; i += 1024) {
+            p.rgrad[i].x /= unit;
+            p.rgrad[i].z /= unit;
+        }
     }
     if (tid == 0) {
         Head h;
@@ -1125,6 +1133,7 @@ struct MergeParams {
     const float* zsel;
     float c2, inv_tau, tau2;
     float* lse;
+    float* target_logp;    // [rows][top]
     float* row_loss;   // reduction none: the result
     float* loss;
 };
@@ -1179,18 +1188,23 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const MergePara
         s = 0.0f;
         for (int w = 0; w < kMergeWarps; ++w) s += ss[w] * scale(sm[w], m);
     }
-    const float lse = i >= 0 ? logf(s) + finite_or_zero(m) * p.inv_tau : 0.0f;
+    // Log-probabilities at the targets as differences from the maximum: next to lse,
+    // which is rounded to its own size, those near 0 would be lost.
+    const float ref = finite_or_zero(m), logs = logf(s);
     const bool leader = row < p.rows && warp % p.warps_per_row == 0;
-    if (leader && lane == 0) p.lse[row] = lse;
+    if (leader && lane == 0) p.lse[row] = i >= 0 ? logs + ref * p.inv_tau : 0.0f;
     if (leader) {
         float v = 0.0f;
         if (f == kLoss && p.eq == nullptr) {
-            v = lse - z_one;
+            v = logs - (z_one - ref);
+            if (lane == 0) p.target_logp[row] = -v;
         } else if (f == kLoss) {
             const long long e = static_cast<long long>(row) * p.top;
             for (int k = lane; k < p.top; k += 32) {
                 const float qv = p.eq[e + k];
-                if (qv != 0.0f) v += qv * (logf(qv) + (lse - p.zsel[e + k] * p.inv_tau));
+                const float logp = (p.zsel[e + k] - ref) * p.inv_tau - logs;
+                p.target_logp[e + k] = logp;
+                if (qv != 0.0f) v += qv * (logf(qv) - logp);
             }
             for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
             v *= p.tau2;
@@ -1354,8 +1368,9 @@ static int check_desc(const B200VocabLossDesc* d) {
                       (long long)d->ld_teacher, (long long)d->top);
             return B200_ERR_INVALID_ARGUMENT;
         }
-        if (!(d->temperature > 0.0) || !std::isfinite(d->temperature)) {
-            set_error("temperature=%g must be positive and finite", d->temperature);
+        // Its inverse and its square stay far inside 32 bits.
+        if (!(d->temperature >= 0x1p-20 && d->temperature <= 0x1p20)) {
+            set_error("temperature=%g must be between 2^-20 and 2^20", d->temperature);
             return B200_ERR_INVALID_ARGUMENT;
         }
     } else if (d->temperature != 1.0) {
@@ -1473,7 +1488,7 @@ static Layout layout_for(const B200VocabLossDesc& d, int64_t sms) {
     l.gathered_forward = take(l.gather_forward ? 2 * T * l.ld_gathered : 0);
     l.bytes_forward = at;
     at = common;
-    l.rgrad = take(8 * T);
+    l.rgrad = take(16 * T);
     l.gathered_backward = take(2 * T * l.ld_gathered);
     l.g = take(2 * T * l.piece);
     l.part_h = take(4 * l.splits_h * l.rows_pad * l.ld_part);
@@ -1550,6 +1565,12 @@ static int device_state(DeviceState* out) {
         for (int i = 0; i < n; ++i)
             B200_CUDA_TRY(cudaFuncSetAttribute(reinterpret_cast<const void*>(all[i].fn),
                                                cudaFuncAttributeMaxDynamicSharedMemorySize, all[i].smem));
+        // Loaded now, not at a first launch that a stream capture may hold.
+        cudaFuncAttributes loaded;
+        for (const void* fn : {reinterpret_cast<const void*>(teacher_kernel), reinterpret_cast<const void*>(rows_kernel),
+                               reinterpret_cast<const void*>(gather_kernel), reinterpret_cast<const void*>(merge_kernel),
+                               reinterpret_cast<const void*>(finish_kernel)})
+            B200_CUDA_TRY(cudaFuncGetAttributes(&loaded, fn));
         cudaLaunchConfig_t cfg = {};
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1649,7 +1670,8 @@ static int map_2d(const Call& c, CUtensorMap* map, const void* base, int64_t row
 
 // Targets, row numbers and the gathered copy of H.
 static int launch_rows(const Call& c, const void* index, const void* teacher, const void* hidden, bool gather,
-                       int64_t gathered, const float* grad, const float* lse) {
+                       int64_t gathered, const float* grad, const float* lse,
+                       const float* target_logp) {
     const B200VocabLossDesc& d = *c.d;
     const Layout& l = c.l;
     if (d.top > 0) {
@@ -1694,7 +1716,8 @@ static int launch_rows(const Call& c, const void* index, const void* teacher, co
     r.inv = c.at<int>(l.inv);
     r.grad = grad;
     r.lse = lse;
-    r.rgrad = grad != nullptr ? c.at<float2>(l.rgrad) : nullptr;
+    r.target_logp = target_logp;
+    r.rgrad = grad != nullptr ? c.at<float4>(l.rgrad) : nullptr;
     r.tau = static_cast<float>(d.temperature);
     int rc = launch(rows_kernel, 1, 1024, 0, 1, d.top > 0, c.stream, r);
     if (rc != B200_OK || !gather) return rc;
@@ -1769,7 +1792,8 @@ static int begin(const B200VocabLossDesc* d, void* workspace, int64_t bytes, boo
 }
 
 static int forward(const B200VocabLossDesc* d, const void* hidden, const void* weight, const void* index,
-                   const void* teacher, float* loss, float* lse, void* workspace, int64_t bytes, void* stream) {
+                   const void* teacher, float* loss, float* lse, float* target_logp, void* workspace, int64_t bytes,
+                   void* stream) {
     int rc = check_desc(d);
     if (rc != B200_OK) return rc;
     if (d->rows == 0) {
@@ -1777,7 +1801,7 @@ static int forward(const B200VocabLossDesc* d, const void* hidden, const void* w
         return B200_ERR_UNSUPPORTED;
     }
     rc = check_pointers({{hidden, "hidden"}, {weight, "weight"}, {index, "index"}, {loss, "loss"}, {lse, "lse"},
-                         {workspace, "workspace"}});
+                         {target_logp, "target_logp"}, {workspace, "workspace"}});
     if (rc == B200_OK && d->top > 0) rc = check_pointers({{teacher, "teacher"}});
     if (rc == B200_OK) rc = check_aligned({{hidden, "hidden"}, {weight, "weight"}});
     if (rc != B200_OK) return rc;
@@ -1793,7 +1817,7 @@ static int forward(const B200VocabLossDesc* d, const void* hidden, const void* w
                               : (a1 = a0, B200_OK);
     if (rc == B200_OK) rc = map_2d(c, &b, weight, d->vocab, d->hidden, d->ld_weight, box_n, kBK);
     if (rc != B200_OK) return rc;
-    rc = launch_rows(c, index, teacher, hidden, l.gather_forward, l.gathered_forward, nullptr, nullptr);
+    rc = launch_rows(c, index, teacher, hidden, l.gather_forward, l.gathered_forward, nullptr, nullptr, nullptr);
     if (rc != B200_OK) return rc;
     Params p = base_params(c);
     p.n = static_cast<int>(d->vocab);
@@ -1825,6 +1849,7 @@ static int forward(const B200VocabLossDesc* d, const void* hidden, const void* w
     m.inv_tau = static_cast<float>(1.0 / d->temperature);
     m.tau2 = static_cast<float>(d->temperature * d->temperature);
     m.lse = lse;
+    m.target_logp = target_logp;
     m.row_loss = d->reduction == B200_VL_NONE ? loss : c.at<float>(l.row_loss);
     m.loss = loss;
     return launch(merge_kernel, static_cast<int>(ceil_div(d->rows, kMergeWarps / m.warps_per_row)), 32 * kMergeWarps, 0, 1,
@@ -1832,8 +1857,8 @@ static int forward(const B200VocabLossDesc* d, const void* hidden, const void* w
 }
 
 static int backward(const B200VocabLossDesc* d, const void* hidden, const void* weight, const void* index,
-                    const void* teacher, const float* lse, const float* grad_loss, void* d_hidden, void* d_weight,
-                    void* workspace, int64_t bytes, void* stream) {
+                    const void* teacher, const float* lse, const float* target_logp, const float* grad_loss,
+                    void* d_hidden, void* d_weight, void* workspace, int64_t bytes, void* stream) {
     int rc = check_desc(d);
     if (rc != B200_OK) return rc;
     if (d->rows == 0 || (d_hidden == nullptr && d_weight == nullptr)) {
@@ -1842,7 +1867,7 @@ static int backward(const B200VocabLossDesc* d, const void* hidden, const void* 
         return B200_ERR_UNSUPPORTED;
     }
     rc = check_pointers({{hidden, "hidden"}, {weight, "weight"}, {index, "index"}, {lse, "lse"},
-                         {grad_loss, "grad_loss"}, {workspace, "workspace"}});
+                         {target_logp, "target_logp"}, {grad_loss, "grad_loss"}, {workspace, "workspace"}});
     if (rc == B200_OK && d->top > 0) rc = check_pointers({{teacher, "teacher"}});
     if (rc == B200_OK)
         rc = check_aligned({{hidden, "hidden"}, {weight, "weight"}, {d_hidden, "d_hidden"}, {d_weight, "d_weight"}});
@@ -1874,12 +1899,13 @@ static int backward(const B200VocabLossDesc* d, const void* hidden, const void* 
     if (rc == B200_OK && d_weight != nullptr)
         rc = l.splits_w > 1 ? partial_map(&dw_st, l.part_w, l.splits_w * l.piece) : map_2d(c, &dw_st, d_weight, V, D, D, 32, 64);
     if (rc != B200_OK) return rc;
-    rc = launch_rows(c, index, teacher, hidden, true, l.gathered_backward, grad_loss, lse);
+    rc = launch_rows(c, index, teacher, hidden, true, l.gathered_backward, grad_loss, lse, target_logp);
     for (int64_t v0 = 0; rc == B200_OK && v0 < V; v0 += l.piece) {
         const int64_t vp = std::min(l.piece, V - v0);
         Params p = base_params(c);
         p.v0 = static_cast<int>(v0);
-        p.rgrad = c.at<float2>(l.rgrad);
+        p.rgrad = c.at<float4>(l.rgrad);
+        p.zsel = const_cast<float*>(target_logp);
         p.n = static_cast<int>(vp);
         p.k = static_cast<int>(D);
         p.group_m = group_for(l.tile_m, D);
@@ -1968,21 +1994,22 @@ int b200_vocab_loss_info(const B200VocabLossDesc* desc, int sm_count, B200VocabL
 }
 
 int b200_vocab_loss_forward(const B200VocabLossDesc* desc, const void* hidden, const void* weight,
-                            const void* index, const void* teacher, float* loss, float* lse, void* workspace,
-                            int64_t workspace_bytes, void* stream) {
+                            const void* index, const void* teacher, float* loss, float* lse,
+                            float* target_logp, void* workspace, int64_t workspace_bytes, void* stream) {
     B200_ABI_GUARD_BEGIN
     b200::clear_error();
-    return b200::vl::forward(desc, hidden, weight, index, teacher, loss, lse, workspace, workspace_bytes, stream);
+    return b200::vl::forward(desc, hidden, weight, index, teacher, loss, lse, target_logp, workspace, workspace_bytes, stream);
     B200_ABI_GUARD_END
 }
 
 int b200_vocab_loss_backward(const B200VocabLossDesc* desc, const void* hidden, const void* weight,
-                             const void* index, const void* teacher, const float* lse, const float* grad_loss,
-                             void* d_hidden, void* d_weight, void* workspace, int64_t workspace_bytes, void* stream) {
+                             const void* index, const void* teacher, const float* lse,
+                             const float* target_logp, const float* grad_loss, void* d_hidden, void* d_weight,
+                             void* workspace, int64_t workspace_bytes, void* stream) {
     B200_ABI_GUARD_BEGIN
     b200::clear_error();
-    return b200::vl::backward(desc, hidden, weight, index, teacher, lse, grad_loss, d_hidden, d_weight, workspace,
-                              workspace_bytes, stream);
+    return b200::vl::backward(desc, hidden, weight, index, teacher, lse, target_logp, grad_loss, d_hidden, d_weight,
+                              workspace, workspace_bytes, stream);
     B200_ABI_GUARD_END
 }
 

@@ -426,7 +426,7 @@ typedef struct B200VocabLossDesc {
     int64_t teacher_dtype; /* B200_VL_BF16, B200_VL_F16 or B200_VL_F32 */
     int64_t ignore_index;  /* cross entropy */
     int64_t reduction;
-    double temperature;    /* distillation; 1 otherwise */
+    double temperature;    /* distillation: 2^-20 to 2^20; 1 otherwise */
 } B200VocabLossDesc;
 
 /* The host's choices for a call, a function of the sizes and the SM count. */
@@ -451,12 +451,13 @@ size_t b200_vocab_loss_info_size(void);
 int b200_vocab_loss_info(const B200VocabLossDesc* desc, int sm_count, B200VocabLossInfo* out);
 
 /* Asynchronous on `stream`, on the current device. loss: fp32, rows values
- * (NONE) or one; lse: fp32, rows values (log sum exp(z / tau)) for the backward
- * pass. The workspace is scratch for this call alone. A wait that runs out in a
+ * (NONE) or one. For the backward pass: lse, fp32, rows values (log sum
+ * exp(z / tau)); target_logp, fp32, rows x max(top, 1) values, the
+ * log-probabilities of the targets in an order of its own. The workspace is scratch for this call alone. A wait that runs out in a
  * kernel leaves NaN in loss. */
 int b200_vocab_loss_forward(const B200VocabLossDesc* desc, const void* hidden, const void* weight,
                             const void* index, const void* teacher, float* loss, float* lse,
-                            void* workspace, int64_t workspace_bytes, void* stream);
+                            float* target_logp, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* grad_loss: fp32, the gradient of the loss (rows values for NONE, else one).
  * d_hidden (rows x hidden) and d_weight (vocab x hidden): contiguous, of the
@@ -464,7 +465,7 @@ int b200_vocab_loss_forward(const B200VocabLossDesc* desc, const void* hidden, c
  * written. A wait that runs out in a kernel leaves NaN in both. */
 int b200_vocab_loss_backward(const B200VocabLossDesc* desc, const void* hidden, const void* weight,
                              const void* index, const void* teacher, const float* lse,
-                             const float* grad_loss, void* d_hidden, void* d_weight,
+                             const float* target_logp, const float* grad_loss, void* d_hidden, void* d_weight,
                              void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------ */

@@ -32,7 +32,7 @@ def longs(*shape):
     (dict(target=longs(4, 1)), "expected"),
     (dict(target=torch.zeros(4)), "int32 or int64"),
     (dict(reduction="batchmean"), "reduction"),
-    (dict(ignore_index=1.5), "64-bit"),
+    (dict(ignore_index=1.5), "integer"),
     (dict(ignore_index=2 ** 63), "64-bit"),
     (dict(), "CUDA device"),
 ])
@@ -56,6 +56,8 @@ def test_cross_entropy_refusals(change, match):
     (dict(logits=torch.zeros(4, 3, requires_grad=True)), "detach"),
     (dict(temperature=0.0), "temperature"),
     (dict(temperature=-1.0), "temperature"),
+    (dict(temperature=1e-7), "temperature"),
+    (dict(temperature=2e6), "temperature"),
     (dict(temperature=math.inf), "temperature"),
     (dict(temperature=math.nan), "temperature"),
     (dict(reduction="none "), "reduction"),
@@ -104,8 +106,8 @@ def test_c_abi_refuses_descriptions(change, code):
     d, info = desc(**change), _lib.VocabLossInfo()
     assert lib.b200_vocab_loss_info(ctypes.byref(d), 148, ctypes.byref(info)) == code
     assert _lib.last_error(lib)
-    assert lib.b200_vocab_loss_forward(ctypes.byref(d), 256, 256, 256, 256, 256, 256, 256, 1 << 40, None) == code
-    assert lib.b200_vocab_loss_backward(ctypes.byref(d), 256, 256, 256, 256, 256, 256, 256, 256, 256, 1 << 40, None) == code
+    assert lib.b200_vocab_loss_forward(ctypes.byref(d), *([256] * 8), 1 << 40, None) == code
+    assert lib.b200_vocab_loss_backward(ctypes.byref(d), *([256] * 10), 1 << 40, None) == code
 
 
 def test_c_abi_refuses_pointers():
@@ -114,8 +116,8 @@ def test_c_abi_refuses_pointers():
     assert lib.b200_vocab_loss_info(ctypes.byref(d), 0, ctypes.byref(info)) == _lib.ERR_INVALID_ARGUMENT
     assert lib.b200_vocab_loss_info(ctypes.byref(d), 148, None) == _lib.ERR_INVALID_ARGUMENT
     assert lib.b200_vocab_loss_info(None, 148, ctypes.byref(info)) == _lib.ERR_INVALID_ARGUMENT
-    good = [256] * 7 + [1 << 40, None]
-    for i in (0, 1, 2, 4, 5, 6):  # hidden, weight, index, loss, lse, workspace
+    good = [256] * 8 + [1 << 40, None]
+    for i in (0, 1, 2, 4, 5, 6, 7):  # hidden, weight, index, loss, lse, target_logp, workspace
         args = list(good)
         args[i] = None
         assert lib.b200_vocab_loss_forward(ctypes.byref(d), *args) == _lib.ERR_INVALID_ARGUMENT
@@ -125,16 +127,16 @@ def test_c_abi_refuses_pointers():
         assert lib.b200_vocab_loss_forward(ctypes.byref(d), *args) == _lib.ERR_UNSUPPORTED
     t = desc(top=4, ld_index=4, ld_teacher=4)
     assert lib.b200_vocab_loss_forward(ctypes.byref(t), 256, 256, 256, None, *good[4:]) == _lib.ERR_INVALID_ARGUMENT
-    good = [256] * 9 + [1 << 40, None]
-    for i in (0, 1, 2, 4, 5, 8):
+    good = [256] * 10 + [1 << 40, None]
+    for i in (0, 1, 2, 4, 5, 6, 9):
         args = list(good)
         args[i] = None
         assert lib.b200_vocab_loss_backward(ctypes.byref(d), *args) == _lib.ERR_INVALID_ARGUMENT
     args = list(good)
-    args[6] = args[7] = None
+    args[7] = args[8] = None
     assert lib.b200_vocab_loss_backward(ctypes.byref(d), *args) == _lib.ERR_UNSUPPORTED  # nothing asked for
     empty = desc(rows=0)
-    assert lib.b200_vocab_loss_forward(ctypes.byref(empty), *([256] * 7), 1 << 40, None) == _lib.ERR_UNSUPPORTED
+    assert lib.b200_vocab_loss_forward(ctypes.byref(empty), *([256] * 8), 1 << 40, None) == _lib.ERR_UNSUPPORTED
 
 
 def sizes():

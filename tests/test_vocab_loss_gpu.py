@@ -128,6 +128,14 @@ def test_distillation_all_entries_of_one_tile():
     kd(160, 1000, 64, 64, change=change)
 
 
+def test_distillation_vanishing_probabilities():
+    """Teacher logits hundreds apart: entries of probability 0 are still part of the student's softmax."""
+    def change(logits, idx):
+        logits[:, 1::2] -= 200.0
+    kd(90, 400, 64, 12, change=change)
+    kd(90, 400, 1024, 12, change=change)
+
+
 def test_distillation_minus_infinity_is_padding():
     def change(logits, idx):
         logits[::2, ::3] = -math.inf
@@ -221,6 +229,51 @@ def test_one_gradient_at_a_time():
     assert torch.equal(torch.autograd.grad(loss, hg, retain_graph=True)[0], both[1])  # twice on one graph
     with torch.no_grad():
         assert torch.equal(vocab_loss.linear_cross_entropy(hg, wg, t), both[0])
+
+
+def test_refused_layouts():
+    from b200gemm import vocab_loss
+    g, h, w = make(6, 100, 64)
+    t = torch.zeros(6, dtype=torch.long, device="cuda")
+    flat = torch.zeros(7 * 80, dtype=BF16, device="cuda")
+    for bad in (flat[4:4 + 6 * 64].view(6, 64), flat.as_strided((6, 64), (68, 1)), h[:1].expand(6, 64)):
+        with pytest.raises(ValueError):
+            vocab_loss.linear_cross_entropy(bad, w, t)
+    wide = torch.zeros(100, 80, dtype=BF16, device="cuda")
+    for bad in (wide[:, 4:68], wide.view(-1)[: 99 * 76 + 64].as_strided((100, 64), (76, 1))):
+        with pytest.raises(ValueError):
+            vocab_loss.linear_cross_entropy(h, bad, t)
+    with pytest.raises(ValueError, match="target must be on"):
+        vocab_loss.linear_cross_entropy(h, w, t.cpu())
+    with pytest.raises(ValueError, match="weight must be on"):
+        vocab_loss.linear_cross_entropy(h, w.cpu(), t)
+
+
+def test_first_call_of_a_process_may_be_captured():
+    import subprocess
+    import sys
+    from pathlib import Path
+    root = Path(__file__).resolve().parents[1]
+    code = """
+import sys; sys.path.insert(0, %r)
+import torch
+from b200gemm import vocab_loss
+h = torch.randn(300, 64, device="cuda").bfloat16().requires_grad_()
+w = torch.randn(900, 64, device="cuda").bfloat16().requires_grad_()
+t = torch.randint(0, 900, (300,), device="cuda")
+up = torch.ones((), device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    loss = vocab_loss.linear_cross_entropy(h, w, t)
+    grads = torch.autograd.grad(loss, (h, w), up)
+graph.replay()
+want = vocab_loss.linear_cross_entropy(h, w, t)
+assert torch.equal(loss, want) and all(torch.equal(a, b) for a, b in zip(grads, torch.autograd.grad(want, (h, w), up)))
+print("same")
+""" % str(root / "gb300-gemm-anatomy_b200")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
 
 
 def test_differentiable_once():
@@ -404,6 +457,34 @@ def test_gradients_against_differences():
         assert bool(((got - diff).abs() <= bound).all())
         # The bound is no empty one: it is below the difference itself in most rows.
         assert float((diff.abs() > bound).double().mean()) > 0.5
+
+
+def test_gradients_of_confident_rows():
+    """Where the model is sure and right, p - 1 is small: its own precision counts, not that of 1 or of lse.
+    log p is a difference from the largest logit: off by 2^-21 (a sum of up to 256 terms, its logarithm) and by
+    how far the logits are off (dz, see the reference), the target's own cancelling but for the share 1 - p."""
+    from b200gemm import vocab_loss
+    rows, vocab, hidden = 64, 500, 2048
+    g, h, w = make(rows, vocab, hidden, seed=4, std=0.02)
+    t = torch.randint(0, vocab, (rows,), generator=g, device="cuda")
+    h = (h + w[t].float() * torch.linspace(14, 20, rows, device="cuda")[:, None]).to(BF16)
+    z = h.double() @ w.double().t()
+    p = torch.softmax(z, 1)
+    G = p.clone()
+    G.scatter_(1, t[:, None], 0.0)
+    miss = G.sum(1, keepdim=True)  # 1 - p
+    assert float(miss.min()) < 1e-3 and float(miss.max()) > 1e-2
+    up = (1 / miss[:, 0]).float()  # each row's gradient at one size
+    loss, dh, _ = run(vocab_loss.linear_cross_entropy, h, w, (t,), up, reduction="none")
+    dz = (hidden / 16 + 16) * 2.0 ** -23 * (h.double().abs() @ w.double().abs().t()).max(1, keepdim=True).values
+    off = 2.0 ** -21 + 2 * dz * miss
+    assert bool(((loss.double() + torch.log1p(-miss[:, 0])).abs() <= off[:, 0]).all())
+    E = G * (2.0 ** -8 + 2 * dz + 2.0 ** -18)
+    E.scatter_(1, t[:, None], 2.0 ** -8 * miss + off)
+    G.scatter_(1, t[:, None], -miss)
+    want = (G / miss) @ w.double()
+    bound = (E / miss) @ w.double().abs() + 2.0 ** -8 * want.abs() + 2.0 ** -16 * (G / miss).abs() @ w.double().abs()
+    assert bool(((dh.double() - want).abs() <= bound).all())
 
 
 def test_many_rows():
