@@ -56,9 +56,12 @@ constexpr int kThreads = 64 + 32 * kEpiWarps;
 constexpr int kEpiBufBytes = 32 * 128;
 // k-slices between two drains of the statistics' accumulators. The tensor cores
 // add to a 32-bit accumulator without rounding to nearest: over D = 4096 the lost
-// bits add up to 5e-6 of a logit. Sums of 512 products are added up in registers
-// instead, rounded to nearest.
-constexpr int kDrain = 8;
+// bits add up to 5e-6 of a logit. Sums of 512 products (256 in single CTAs, whose
+// calls wait for the weight anyway) are added up in registers instead, rounded to
+// nearest. Sums of 1024 would be 1 % faster and as far off as a plain sum in 32 bits.
+constexpr int kDrainMost = 8;
+template <int kCtaGroup>
+constexpr int kDrain = kCtaGroup == 1 ? 4 : kDrainMost;
 constexpr int kQueue = 4;
 constexpr int kNoCol = INT_MAX;
 constexpr int kMaxTop = 256;      // teacher logits per row
@@ -67,7 +70,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 // The products. Operands: Stats, Grad: A = H, B = W (both K-major); Dh: A = G
 // (K-major), B = W (MN-major); Dw: A = G, B = H (both MN-major). StatsShort is
-// Stats over at most kDrain k-slices, DwParts leaves runs of Dw's contraction
+// Stats over at most kDrainMost k-slices, DwParts leaves runs of Dw's contraction
 // as partial sums.
 enum Op { kStats = 0, kStatsShort = 1, kGrad = 2, kDh = 3, kDw = 4, kDwParts = 5 };
 __host__ __device__ constexpr bool is_stats(int op) { return op == kStats || op == kStatsShort; }
@@ -215,6 +218,7 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
     constexpr int kHalfN = kTileN / 2;
     constexpr int kTmemCols = 2 * kTileN;  // two accumulators
     constexpr bool kPair = kCtaGroup == 2;
+    constexpr int kDrain = vl::kDrain<kCtaGroup>;
     constexpr bool kAMn = is_dw(kOp);
     constexpr bool kBMn = kOp == kDh || is_dw(kOp);
     constexpr int kBoxBytes = 64 * kBK * 2;  // an MN-major box
@@ -619,11 +623,6 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
                 ebase = static_cast<long long>(r) * p.top;
                 load_four();
             };
-            // The lowest column left in the warp's rows, relative to the piece.
-            auto lowest = [&]() {
-                const int c = __reduce_min_sync(0xffffffffu, cur < first ? kNoCol : cur);
-                return c == kNoCol ? kNoCol : c - p.v0;
-            };
             auto advance = [&]() {
                 cur = ahead1;
                 ahead1 = ahead2;
@@ -632,6 +631,31 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
                 if (p.rowmap != nullptr && (++used & 3) == 0) load_four();
             };
 
+            // The lowest target column left in the warp's rows.
+            auto lowest = [&]() {
+                const int c = __reduce_min_sync(0xffffffffu, cur < first ? kNoCol : cur);
+                return c == kNoCol ? kNoCol : c - p.v0;
+            };
+            // Keeps the logits at the row's targets among the 32 columns of `r` that start
+            // at `lo`. A register cannot be picked by a lane's own number: each lane
+            // writes its row to the warp's buffer and reads its own columns back, as many
+            // steps as the fullest row has (one step per column of the warp: 37 against
+            // 29 us for 3537 rows of 115 logits over 807 x 384).
+            auto targets_in = [&](int lo) { return cur >= lo && cur < lo + 32; };
+            auto keep_targets = [&](const uint32_t (&r)[32], int lo) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    st_shared_v4(row_addr + ((j ^ (lane & 7)) << 4), r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+                while (targets_in(lo)) {
+                    const int i = cur - lo;
+                    float z;
+                    asm volatile("ld.shared.f32 %0, [%1];"
+                                 : "=f"(z) : "r"(row_addr + (((i >> 2) ^ (lane & 7)) << 4) + (i & 3) * 4) : "memory");
+                    p.zsel[ebase + pos] = z;
+                    advance();
+                }
+                __syncwarp();
+            };
             // The statistics over several units look the targets up between two of them:
             // the first accumulator of a tile is not kept waiting.
             if constexpr (kOp == kStatsShort || kOp == kGrad) load_targets();
@@ -664,7 +688,9 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
                 // Logits at the targets: a register cannot be picked by number, a TMEM
                 // column can. Where a row has a target here, the sums go back over the last
                 // unit's accumulator; all lanes read each target's column, those that want
-                // it keep it.
+                // it keep it. (Looking through 32 columns at a time, as for short
+                // contractions, needs the registers that the sums are in: 407 against
+                // 364 us for 6970 rows of 102 logits over 30798 x 680.)
                 int col = lowest();
                 if (col < col0 + kHalfN) {
                     const uint32_t t_last = t_lane + (unit & 1) * kTileN;
@@ -727,17 +753,7 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
                     for (int i = 0; i < 32; ++i) s4[i & 3] += exp2_approx((__uint_as_float(r[i]) - ref) * p.c2);
                     s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
                     m = mx;
-                    // Logits at the targets: all lanes read the column, the lanes that
-                    // want it keep it.
-                    while (true) {
-                        const int col = lowest();
-                        if (col >= col0 + (c + 1) * 32) break;
-                        const float z = tmem_ld_col(t_row + (col - col0));
-                        if (cur == col + p.v0) {
-                            p.zsel[ebase + pos] = z;
-                            advance();
-                        }
-                    }
+                    if (__any_sync(0xffffffffu, targets_in(first + c * 32))) keep_targets(r, first + c * 32);
                 }
                 release_unit();
                 if (active && col0 < p.n)
@@ -1297,6 +1313,8 @@ static int64_t align_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
 // Room for G: this, or as much as H itself takes (one 256-column block at least).
 constexpr int64_t kPieceBytes = int64_t(256) << 20;
 constexpr int64_t kPartialBytes = int64_t(256) << 20;
+// A piece of G that is still in L2 (126 MB) when the second product reads it.
+constexpr int64_t kL2Piece = int64_t(48) << 20;
 
 struct Layout {
     int cta_group, tile_n;          // tiles of the logits (Stats, Grad)
@@ -1389,15 +1407,22 @@ static Layout layout_for(const B200VocabLossDesc& d, int64_t sms) {
     const int64_t pairs = std::max<int64_t>(sms / 2, 1);
     const int64_t kd = ceil_div(D, kBK), kt = ceil_div(T, kBK);
     // Tiles of the logits: pairs 256 x 256, or single CTAs 128 x 256 or 128 x 128
-    // where those finish in fewer rounds. The smaller ones read their operands more
-    // often per product.
-    struct Shape { int cta_group, tile_n; double slice; };
+    // where those finish in fewer rounds. A k-slice takes the longer of its products
+    // (512 cycles for 128 x 256 columns of a CTA) and its operands' way from L2 to the
+    // SM (57 bytes per cycle measured with all SMs reading, 32 KiB in 575 cycles; in
+    // proportion with fewer), and a tile at least its epilogue.
+    struct Shape { int cta_group, tile_n; };
     double best_rounds = 0.0;
-    for (const Shape& c : {Shape{2, 256, 1.0}, Shape{1, 256, 1.1}, Shape{1, 128, 0.55}}) {
+    for (const Shape& c : {Shape{2, 256}, Shape{1, 256}, Shape{1, 128}}) {
         if (c.cta_group == 2 && T <= kRowsPerCta) continue;
         const int64_t tiles = ceil_div(T, kRowsPerCta * c.cta_group) * ceil_div(V, c.tile_n);
-        const double rounds = static_cast<double>(ceil_div(tiles, std::max<int64_t>(sms / c.cta_group, 1))) *
-                              (c.slice * static_cast<double>(kd) + 4.0);
+        const int64_t at_once = std::max<int64_t>(sms / c.cta_group, 1);
+        const int64_t rows_a = c.cta_group == 2 ? kRowsPerCta : std::min<int64_t>(kRowsPerCta, align_up(T, 8));
+        const double bytes = static_cast<double>(rows_a + c.tile_n / c.cta_group) / 256.0;
+        const double slice =
+            std::max(c.tile_n / 256.0, bytes * std::min(1.0, static_cast<double>(tiles) / static_cast<double>(at_once)));
+        const double rounds = static_cast<double>(ceil_div(tiles, at_once)) *
+                              (std::max(slice * static_cast<double>(kd), 8.0 * c.tile_n / 256) + 4.0);
         if (l.cta_group == 0 || rounds < best_rounds) {
             best_rounds = rounds;
             l.cta_group = c.cta_group;
@@ -1413,9 +1438,12 @@ static Layout layout_for(const B200VocabLossDesc& d, int64_t sms) {
     l.gather_forward = ceil_div(T, l.tile_m) * ceil_div(V, l.tile_n) > sms / l.cta_group && T > l.tile_m;
     // Piece of the vocabulary (in blocks of 256) and runs of the contractions of dH
     // and dW: the least k-slices on the longest cluster, over the three products of
-    // all pieces, with eight k-slices for each launch's start and end. One piece
-    // where G has room; otherwise up to 64 widths between half the room and all of
-    // it. A further run of a contraction writes and reads its sums once more.
+    // all pieces, with eight k-slices for each launch's start and end. Widths: all
+    // that G has room for, up to 64 between half of that and all of it where that is
+    // not the whole vocabulary, and what stays in L2 between the three products, since
+    // with a short D the way of G through HBM takes longer than the products. A further
+    // run of a contraction writes and reads its sums once more, a further piece reads
+    // and writes dH's sums.
     const int64_t blocks_v = ceil_div(V, kBN), nb = ceil_div(D, kBN), mb = l.rows_pad / l.tile_m_h;
     const int64_t slots_h = std::max<int64_t>(sms / l.cta_group_h, 1);
     const int64_t slots = std::max<int64_t>(sms / l.cta_group, 1);
@@ -1423,6 +1451,7 @@ static Layout layout_for(const B200VocabLossDesc& d, int64_t sms) {
         std::max<int64_t>(1, std::min(blocks_v, std::max(kPieceBytes, 2 * l.rows_pad * D) / (2 * kBN * l.rows_pad)));
     const int64_t least = most == blocks_v ? most : std::max<int64_t>(1, most / 2);
     const int64_t step = std::max<int64_t>(1, (most - least) / 64);
+    const int64_t in_l2 = std::max<int64_t>(1, kL2Piece / (2 * kBN * l.rows_pad));
     const int64_t run_bytes = int64_t(1800) << 10;  // bytes in the time of a k-slice
     auto splits_most = [&](int64_t tiles, int64_t slots_, int64_t rows, int64_t slices) -> int64_t {
         if (tiles >= 4 * slots_) return 1;
@@ -1430,18 +1459,22 @@ static Layout layout_for(const B200VocabLossDesc& d, int64_t sms) {
     };
     auto rounds_of = [](int64_t tiles, int64_t slots_) { return ceil_div(tiles, slots_); };
     int64_t best = -1;
-    for (int64_t b = least; b <= most; b += step) {
+    for (int64_t i = in_l2 < least ? -1 : 0; least + i * step <= most; ++i) {
+        const int64_t b = i < 0 ? in_l2 : least + i * step;
         const int64_t pieces = ceil_div(blocks_v, b), rest = blocks_v - (pieces - 1) * b;
         auto both = [&](auto cost) { return (pieces - 1) * cost(b) + cost(rest); };
+        // What G costs a product that writes or reads it, where it does not stay in L2.
+        auto hbm = [&](int64_t n) { return n > in_l2 ? 2 * l.rows_pad * n * kBN / run_bytes : 0; };
         const int64_t grad = both([&](int64_t n) {
-            return rounds_of(ceil_div(T, l.tile_m) * ceil_div(n * kBN, l.tile_n), slots) * kd + 8;
+            return std::max(rounds_of(ceil_div(T, l.tile_m) * ceil_div(n * kBN, l.tile_n), slots) * std::max<int64_t>(kd, 8), hbm(n)) + 8;
         });
         int64_t best_h = -1, splits_h = 1, best_w = -1, splits_w = 1;
         const int64_t most_h = splits_most(mb * nb, slots_h, l.rows_pad, std::min(ceil_div(V, kBK), b * (kBN / kBK)));
         for (int64_t s = 1; s <= most_h; ++s) {
             const int64_t c = both([&](int64_t n) {
-                return rounds_of(mb * nb * s, slots_h) * ceil_div(n * (kBN / kBK), s) + 8 + 4 * l.rows_pad * D * (s - 1) / run_bytes;
-            }) + 4 * l.rows_pad * D * (s - 1) / run_bytes;
+                return std::max(rounds_of(mb * nb * s, slots_h) * ceil_div(n * (kBN / kBK), s), hbm(n)) + 8 +
+                       4 * l.rows_pad * D * (s - 1) / run_bytes;
+            }) + 4 * l.rows_pad * D * (s - 1 + 2 * (pieces - 1)) / run_bytes;
             if (best_h < 0 || c < best_h) {
                 best_h = c;
                 splits_h = s;
@@ -1449,7 +1482,7 @@ static Layout layout_for(const B200VocabLossDesc& d, int64_t sms) {
         }
         const int64_t most_w = pieces > 1 ? 1 : splits_most(b * nb, pairs, b * kBN, kt);
         for (int64_t s = 1; s <= most_w; ++s) {
-            const int64_t c = both([&](int64_t n) { return rounds_of(n * nb * s, pairs) * ceil_div(kt, s) + 8; }) +
+            const int64_t c = both([&](int64_t n) { return std::max(rounds_of(n * nb * s, pairs) * ceil_div(kt, s), hbm(n)) + 8; }) +
                               (s > 1 ? 4 + 8 * b * kBN * D * s / run_bytes : 0);
             if (best_w < 0 || c < best_w) {
                 best_w = c;
@@ -1828,7 +1861,7 @@ static int forward(const B200VocabLossDesc* d, const void* hidden, const void* w
     p.early = !l.gather_forward;
     p.part_ld = ceil_div(d->vocab, l.tile_n / 2);
     p.a_bytes = box_m * kBK * 2;
-    rc = launch_gemm(c, d->hidden <= kDrain * kBK ? kStatsShort : kStats, l.cta_group, l.tile_n,
+    rc = launch_gemm(c, d->hidden <= kDrainMost * kBK ? kStatsShort : kStats, l.cta_group, l.tile_n,
                      ceil_div(d->rows, l.tile_m) * ceil_div(d->vocab, l.tile_n), a0, a1, b, b, b, p);
     if (rc != B200_OK) return rc;
     MergeParams m{};
