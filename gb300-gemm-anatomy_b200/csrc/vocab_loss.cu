@@ -106,6 +106,27 @@ struct Cfg {
     static_assert(kSmemBytes <= 232448, "exceeds the 227 KB opt-in shared memory");
 };
 
+// Runs of a contraction over `slices` k-slices whose product has `tiles` tiles
+// for `slots` clusters: the fewest k-slices on the longest cluster, with what a
+// further run's sums cost to write and read again (in k-slices, 1 / 16ths).
+__host__ __device__ inline unsigned runs_cost(unsigned s, unsigned tiles, unsigned slots, unsigned slices, unsigned run_cost16) {
+    const unsigned rounds = (tiles * s + slots - 1) / slots;
+    const unsigned long long cost =
+        16ull * rounds * ((slices + s - 1) / s) + static_cast<unsigned long long>(run_cost16) * (s - 1);
+    return cost < 0xfffffffeull ? static_cast<unsigned>(cost) : 0xfffffffeu;
+}
+
+// The rows that carry a loss are known on the device alone, so the kernels choose,
+// all of them the same: a warp tries a number of runs per lane.
+__device__ __forceinline__ int runs_for_warp(int tiles, int slots, int slices, int most, int run_cost16) {
+    static_assert(kMaxSplits <= 32, "a lane for each number of runs");
+    if (most == 1) return 1;
+    const int s = static_cast<int>(threadIdx.x & 31) + 1;
+    const unsigned cost = s <= min(most, slices) ? runs_cost(s, tiles, slots, slices, run_cost16) : 0xffffffffu;
+    const unsigned least = __reduce_min_sync(0xffffffffu, cost);
+    return __ffs(__ballot_sync(0xffffffffu, cost == least));
+}
+
 struct Params {
     Head* head;
     unsigned long long timeout_ns;
@@ -118,7 +139,10 @@ struct Params {
     int group_m;          // m-blocks per raster group
     int a_bytes;          // bytes of an A tile: rows beyond the call's are not loaded
     int early;            // Stats: the operands are the call's own, all rows in their order
-    int splits;           // Dh, DwParts: runs of the contraction
+    int splits;           // Dh, DwParts: runs of the contraction at most
+    int run_slots;        // clusters that they are chosen for
+    int run_slices;       // Dh: k-slices of the first piece (all pieces are cut alike)
+    int run_cost16;
     int rows_pad;         // Dh, DwParts: rows between two splits' partial sums
     int accumulate;       // Dh: 1 add to the partial sums, 0 write them
     // Stats, Grad. One target per row (cross entropy): ecol and zsel (Stats) go by
@@ -308,7 +332,9 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
     const int num_k = (k_ext + kBK - 1) / kBK;
     const int tiles_mn = num_m * num_n;
     constexpr bool kSplit = kOp == kDh || kOp == kDwParts;
-    const int num_tiles = kSplit ? tiles_mn * p.splits : tiles_mn;
+    const int splits =
+        kSplit ? runs_for_warp(tiles_mn, p.run_slots, kOp == kDh ? p.run_slices : num_k, p.splits, p.run_cost16) : 1;
+    const int num_tiles = tiles_mn * splits;
 
     // Tile id -> blocks and k-slices. Groups of m-blocks walk all n-blocks, so
     // the tiles in flight share rows of both operands in L2.
@@ -323,8 +349,8 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
         if constexpr (kSplit) {
             w.split = t / tiles_mn;
             t -= w.split * tiles_mn;
-            w.kb0 = static_cast<int>(static_cast<long long>(num_k) * w.split / p.splits);
-            w.kb1 = static_cast<int>(static_cast<long long>(num_k) * (w.split + 1) / p.splits);
+            w.kb0 = static_cast<int>(static_cast<long long>(num_k) * w.split / splits);
+            w.kb1 = static_cast<int>(static_cast<long long>(num_k) * (w.split + 1) / splits);
         }
         const int per_group = p.group_m * num_n;
         const int g = t / per_group;
@@ -1256,6 +1282,7 @@ struct FinishParams {
     const float* part_w;  // dW: the same over the vocabulary, or null: written by the product
     long long ld_part, stride_h, stride_w;
     int splits_h, splits_w, rows, hidden, vocab, fp16;
+    int tile_m_h, slots_h, slots_w, slices_h, cost16_h, cost16_w;  // of runs_for, as in the products
     void* d_hidden;
     void* d_weight;
 };
@@ -1268,15 +1295,19 @@ __global__ void __launch_bounds__(256) finish_kernel(const FinishParams p) {
     const bool failed = p.head->status != 0;
     const float alpha = p.head->alpha;
     const int vecs = p.hidden / 8;
-    // Runs of dW's contraction that had no row were not written.
-    const int num_k = (max(p.head->n_rows, 1) + kBK - 1) / kBK;
+    const int n_rows = max(p.head->n_rows, 1);
+    const int num_n = (p.hidden + kBN - 1) / kBN;
+    const int splits_h = runs_for_warp((n_rows + p.tile_m_h - 1) / p.tile_m_h * num_n, p.slots_h, p.slices_h, p.splits_h, p.cost16_h);
+    const int splits_w = p.part_w == nullptr ? 1
+                                             : runs_for_warp((p.vocab + kBN - 1) / kBN * num_n, p.slots_w, (n_rows + kBK - 1) / kBK,
+                                                        p.splits_w, p.cost16_w);
     const int rows_h = p.d_hidden != nullptr ? p.rows : 0;
     const int rows_w = p.d_weight != nullptr && (failed || p.part_w != nullptr) ? p.vocab : 0;
     for (int r = blockIdx.x; r < rows_h + rows_w; r += gridDim.x) {
         const bool is_h = r < rows_h;
         const int t = is_h ? r : r - rows_h;
         const int i = is_h ? p.inv[t] : t;
-        const int splits = is_h ? p.splits_h : p.splits_w;
+        const int splits = is_h ? splits_h : splits_w;
         const long long stride = is_h ? p.stride_h : p.stride_w;
         const float* part = (is_h ? p.part_h : p.part_w) + max(i, 0) * p.ld_part;
         uint4* out = static_cast<uint4*>(is_h ? p.d_hidden : p.d_weight) + static_cast<long long>(t) * vecs;
@@ -1284,7 +1315,6 @@ __global__ void __launch_bounds__(256) finish_kernel(const FinishParams p) {
             float x[8] = {};
             if (i >= 0 && !failed) {
                 for (int s = 0; s < splits; ++s) {
-                    if (!is_h && static_cast<long long>(num_k) * s / splits == static_cast<long long>(num_k) * (s + 1) / splits) continue;
                     const float4* src = reinterpret_cast<const float4*>(part + s * stride) + 2 * v;
                     const float4 a = __ldcs(src), b = __ldcs(src + 1);
                     x[0] += a.x; x[1] += a.y; x[2] += a.z; x[3] += a.w;
@@ -1307,6 +1337,13 @@ __global__ void __launch_bounds__(256) finish_kernel(const FinishParams p) {
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
+static int runs_for(int tiles, int slots, int slices, int most, int run_cost16) {
+    int best = 1;
+    for (int s = 2; s <= most && s <= slices; ++s)
+        if (runs_cost(s, tiles, slots, slices, run_cost16) < runs_cost(best, tiles, slots, slices, run_cost16)) best = s;
+    return best;
+}
+
 static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 static int64_t align_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
 
@@ -1319,7 +1356,9 @@ constexpr int64_t kL2Piece = int64_t(48) << 20;
 struct Layout {
     int cta_group, tile_n;          // tiles of the logits (Stats, Grad)
     int cta_group_h;                // tiles of dH, 256 wide
-    int64_t tile_m, tile_m_h, piece, pieces, splits_h, splits_w, rows_pad;
+    int64_t tile_m, tile_m_h, piece, pieces, rows_pad;
+    int64_t splits_h, splits_w, slices_h;  // runs of dH's and dW's contractions at most
+    int cost16_h, cost16_w;
     // Offsets in the workspace.
     int64_t flag, rowmap, inv, ecol, eq, epos;           // both directions
     int64_t zsel, part, row_loss, gathered_forward;
@@ -1433,6 +1472,8 @@ static Layout layout_for(const B200VocabLossDesc& d, int64_t sms) {
     l.cta_group_h = T <= kRowsPerCta ? 1 : 2;
     l.tile_m_h = kRowsPerCta * l.cta_group_h;
     l.rows_pad = align_up(T, l.tile_m_h);
+    l.ld_gathered = align_up(D, 64);
+    l.ld_part = align_up(D, 32);
     // The forward pass gathers only to save products (its rows do not meet): not
     // where all tiles run at once anyway (2.5 us of a 17 us call).
     l.gather_forward = ceil_div(T, l.tile_m) * ceil_div(V, l.tile_n) > sms / l.cta_group && T > l.tile_m;
@@ -1453,11 +1494,12 @@ static Layout layout_for(const B200VocabLossDesc& d, int64_t sms) {
     const int64_t step = std::max<int64_t>(1, (most - least) / 64);
     const int64_t in_l2 = std::max<int64_t>(1, kL2Piece / (2 * kBN * l.rows_pad));
     const int64_t run_bytes = int64_t(1800) << 10;  // bytes in the time of a k-slice
-    auto splits_most = [&](int64_t tiles, int64_t slots_, int64_t rows, int64_t slices) -> int64_t {
+    auto splits_most = [&](int64_t tiles, int64_t slots_, int64_t rows) -> int64_t {
         if (tiles >= 4 * slots_) return 1;
-        return std::max<int64_t>(1, std::min<int64_t>({kMaxSplits, kPartialBytes / (4 * rows * D), slices}));
+        return std::max<int64_t>(1, std::min<int64_t>(kMaxSplits, kPartialBytes / (4 * rows * l.ld_part)));
     };
     auto rounds_of = [](int64_t tiles, int64_t slots_) { return ceil_div(tiles, slots_); };
+    auto cost16 = [&](int64_t rows) { return static_cast<int>(std::min<int64_t>(16 * 8 * rows * l.ld_part / run_bytes, 1 << 24)); };
     int64_t best = -1;
     for (int64_t i = in_l2 < least ? -1 : 0; least + i * step <= most; ++i) {
         const int64_t b = i < 0 ? in_l2 : least + i * step;
@@ -1468,36 +1510,36 @@ static Layout layout_for(const B200VocabLossDesc& d, int64_t sms) {
         const int64_t grad = both([&](int64_t n) {
             return std::max(rounds_of(ceil_div(T, l.tile_m) * ceil_div(n * kBN, l.tile_n), slots) * std::max<int64_t>(kd, 8), hbm(n)) + 8;
         });
-        int64_t best_h = -1, splits_h = 1, best_w = -1, splits_w = 1;
-        const int64_t most_h = splits_most(mb * nb, slots_h, l.rows_pad, std::min(ceil_div(V, kBK), b * (kBN / kBK)));
-        for (int64_t s = 1; s <= most_h; ++s) {
-            const int64_t c = both([&](int64_t n) {
-                return std::max(rounds_of(mb * nb * s, slots_h) * ceil_div(n * (kBN / kBK), s), hbm(n)) + 8 +
-                       4 * l.rows_pad * D * (s - 1) / run_bytes;
-            }) + 4 * l.rows_pad * D * (s - 1 + 2 * (pieces - 1)) / run_bytes;
-            if (best_h < 0 || c < best_h) {
-                best_h = c;
-                splits_h = s;
-            }
-        }
-        const int64_t most_w = pieces > 1 ? 1 : splits_most(b * nb, pairs, b * kBN, kt);
-        for (int64_t s = 1; s <= most_w; ++s) {
-            const int64_t c = both([&](int64_t n) { return std::max(rounds_of(n * nb * s, pairs) * ceil_div(kt, s), hbm(n)) + 8; }) +
-                              (s > 1 ? 4 + 8 * b * kBN * D * s / run_bytes : 0);
-            if (best_w < 0 || c < best_w) {
-                best_w = c;
-                splits_w = s;
-            }
-        }
-        const int64_t cost = grad + best_h + best_w;
+        const int64_t slices_h = std::min(ceil_div(V, kBK), b * (kBN / kBK));
+        const int64_t s_h = runs_for(static_cast<int>(mb * nb), static_cast<int>(slots_h), static_cast<int>(slices_h),
+                                     static_cast<int>(splits_most(mb * nb, slots_h, l.rows_pad)), cost16(l.rows_pad));
+        const int64_t dh = both([&](int64_t n) {
+            return std::max(rounds_of(mb * nb * s_h, slots_h) * ceil_div(n * (kBN / kBK), s_h), hbm(n)) + 8;
+        }) + 8 * l.rows_pad * l.ld_part * (s_h - 1 + pieces - 1) / run_bytes;
+        auto dw_of = [&](int64_t s) {
+            return both([&](int64_t n) { return std::max(rounds_of(n * nb * s, pairs) * ceil_div(kt, s), hbm(n)) + 8; }) +
+                   (s > 1 ? 6 + 8 * b * kBN * l.ld_part * s / run_bytes : 0);
+        };
+        int64_t s_w = pieces > 1 ? 1
+                                 : runs_for(static_cast<int>(b * nb), static_cast<int>(pairs), static_cast<int>(kt),
+                                            static_cast<int>(splits_most(b * nb, pairs, b * kBN)), cost16(b * kBN));
+        if (dw_of(1) <= dw_of(s_w)) s_w = 1;
+        const int64_t dw = dw_of(s_w);
+        const int64_t cost = grad + dh + dw;
         if (best < 0 || cost < best) {
             best = cost;
             l.piece = b * kBN;
             l.pieces = pieces;
-            l.splits_h = splits_h;
-            l.splits_w = splits_w;
+            l.splits_h = s_h;
+            l.splits_w = s_w;
+            l.slices_h = slices_h;
         }
     }
+    // Room for twice the runs of dH that all rows would take: fewer rows may carry a
+    // loss, which leaves clusters for more.
+    l.splits_h = std::min({2 * l.splits_h, splits_most(mb * nb, slots_h, l.rows_pad), l.slices_h});
+    l.cost16_h = cost16(l.rows_pad);
+    l.cost16_w = cost16(l.piece);
     int64_t at = 256;
     auto take = [&](int64_t bytes) {
         const int64_t here = at;
@@ -1516,8 +1558,6 @@ static Layout layout_for(const B200VocabLossDesc& d, int64_t sms) {
     l.zsel = take(4 * T * K);
     l.part = take(8 * ceil_div(V, l.tile_n / 2) * T);
     l.row_loss = take(4 * T);
-    l.ld_gathered = align_up(D, 64);
-    l.ld_part = align_up(D, 32);
     l.gathered_forward = take(l.gather_forward ? 2 * T * l.ld_gathered : 0);
     l.bytes_forward = at;
     at = common;
@@ -1785,6 +1825,8 @@ static int group_for(int64_t tile_m, int64_t k) {
     return std::max(2, std::min(32, static_cast<int>(rows / tile_m + 0.5)));
 }
 
+static int64_t slots_of(const Call& c, int cta_group) { return cta_group == 2 ? c.dev.pairs : c.dev.sms; }
+
 static int launch_gemm(const Call& c, int op, int cta_group, int tile_n, int64_t tiles, const CUtensorMap& a0,
                        const CUtensorMap& a1, const CUtensorMap& b0, const CUtensorMap& b1, const CUtensorMap& dmap,
                        const Params& p) {
@@ -1793,8 +1835,7 @@ static int launch_gemm(const Call& c, int op, int cta_group, int tile_n, int64_t
         set_error("internal error: no kernel for product %d with %d x %d tiles", op, kRowsPerCta * cta_group, tile_n);
         return B200_ERR_INTERNAL;
     }
-    const int64_t slots = cta_group == 2 ? c.dev.pairs : c.dev.sms;
-    const int grid = static_cast<int>(std::max<int64_t>(1, std::min(tiles, slots))) * cta_group;
+    const int grid = static_cast<int>(std::max<int64_t>(1, std::min(tiles, slots_of(c, cta_group)))) * cta_group;
     return launch(v->fn, grid, kThreads, v->smem, cta_group, true, c.stream, a0, a1, b0, b1, dmap, p);
 }
 
@@ -1952,6 +1993,9 @@ static int backward(const B200VocabLossDesc* d, const void* hidden, const void* 
             q.group_m = group_for(l.tile_m_h, l.piece);
             q.a_bytes = box_m_h * kBK * 2;
             q.splits = static_cast<int>(l.splits_h);
+            q.run_slots = static_cast<int>(slots_of(c, l.cta_group_h));
+            q.run_slices = static_cast<int>(l.slices_h);
+            q.run_cost16 = l.cost16_h;
             q.rows_pad = static_cast<int>(l.rows_pad);
             q.accumulate = v0 > 0;
             rc = launch_gemm(c, kDh, l.cta_group_h, kBN, l.rows_pad / l.tile_m_h * ceil_div(D, kBN) * l.splits_h, g_k, g_k,
@@ -1964,6 +2008,8 @@ static int backward(const B200VocabLossDesc* d, const void* hidden, const void* 
             q.group_m = group_for(2 * kRowsPerCta, T);
             q.a_bytes = kRowsPerCta * kBK * 2;
             q.splits = static_cast<int>(l.splits_w);
+            q.run_slots = static_cast<int>(slots_of(c, 2));
+            q.run_cost16 = l.cost16_w;
             q.rows_pad = static_cast<int>(l.piece);
             rc = launch_gemm(c, l.splits_w > 1 ? kDwParts : kDw, 2, kBN,
                              ceil_div(vp, 2 * kRowsPerCta) * ceil_div(D, kBN) * l.splits_w, g_mn, g_mn, h_mn, hg_mn, dw_st, q);
@@ -1980,6 +2026,12 @@ static int backward(const B200VocabLossDesc* d, const void* hidden, const void* 
     f.stride_w = l.piece * l.ld_part;
     f.splits_h = static_cast<int>(l.splits_h);
     f.splits_w = static_cast<int>(l.splits_w);
+    f.tile_m_h = static_cast<int>(l.tile_m_h);
+    f.slots_h = static_cast<int>(slots_of(c, l.cta_group_h));
+    f.slots_w = static_cast<int>(slots_of(c, 2));
+    f.slices_h = static_cast<int>(l.slices_h);
+    f.cost16_h = l.cost16_h;
+    f.cost16_w = l.cost16_w;
     f.rows = static_cast<int>(T);
     f.hidden = static_cast<int>(D);
     f.vocab = static_cast<int>(V);

@@ -436,8 +436,8 @@ typedef struct B200VocabLossInfo {
     int64_t tile_n;
     int64_t piece;         /* columns of the vocabulary per step of the backward pass */
     int64_t pieces;
-    int64_t splits_hidden; /* runs of the contraction over the vocabulary in d_hidden */
-    int64_t splits_weight; /* runs of the contraction over the rows in d_weight */
+    int64_t splits_hidden; /* runs of the contraction over the vocabulary in d_hidden, at most */
+    int64_t splits_weight; /* runs of the contraction over the rows in d_weight, at most */
     int64_t workspace_forward;  /* bytes, 256-byte aligned */
     int64_t workspace_backward;
     int64_t launches_forward;
