@@ -129,7 +129,7 @@ VocabLossDesc = _i64_struct(
 
 VocabLossInfo = _i64_struct(
     "B200VocabLossInfo",
-    ["cta_group", "tile_m", "tile_n", "piece", "pieces", "splits_hidden", "splits_weight",
+    ["cta_group", "tile_m", "tile_n", "tile_m_weight", "piece", "pieces", "splits_hidden", "splits_weight",
      "workspace_forward", "workspace_backward", "launches_forward", "launches_backward"],
 )
 

@@ -87,15 +87,24 @@ struct Head {
     float alpha;      // factor common to all rows of G, applied after the products
 };
 
-template <int kCtaGroup, int kTileN>
+// kSubM = 2 (Dw in pairs): a tile is two blocks of 256 rows that share their B
+// operand, one in each accumulator: 48 KiB of operands for 2 x 4.2 MFLOP of a CTA
+// instead of 32 KiB for 4.2. The start of a tile then waits for the last one's rows
+// to be read out of TMEM, which dW's short epilogue allows (8192 rows x 32000 x 4096:
+// 1312 against 1411 us) and G's exponentials do not (2000 x 50001 x 1024: 146 against
+// 134 us).
+template <int kCtaGroup, int kTileN, int kSubM = 1>
 struct Cfg {
     static_assert(kTileN == kBN || (kTileN == 128 && kCtaGroup == 1), "unsupported tile width");
-    static constexpr int kStages = kCtaGroup == 1 && kTileN == kBN ? 4 : 6;
-    static constexpr int kABytes = kRowsPerCta * kBK * 2;
+    static_assert(kSubM == 1 || (kSubM == 2 && kCtaGroup == 2), "unsupported tile height");
+    static constexpr int kStages = kSubM == 2 || (kCtaGroup == 1 && kTileN == kBN) ? 4 : 6;
+    static constexpr int kASubBytes = kRowsPerCta * kBK * 2;
+    static constexpr int kABytes = kASubBytes * kSubM;
     static constexpr int kBRows = kTileN / kCtaGroup;
     static constexpr int kBBytes = kBRows * kBK * 2;
     static constexpr int kStageBytes = kABytes + kBBytes;
-    static constexpr int kTileM = kRowsPerCta * kCtaGroup;
+    static constexpr int kSubRows = kRowsPerCta * kCtaGroup;
+    static constexpr int kTileM = kSubRows * kSubM;
     static constexpr int kEpiOffset = kStages * kStageBytes;
     static constexpr int kEpiBytes = kEpiWarps * kEpiBufBytes;
     static constexpr int kBarOffset = kEpiOffset + kEpiBytes;
@@ -137,7 +146,7 @@ struct Params {
     int k;                // contraction: D (Stats, Grad) or piece (Dh); Dw: from the head
     int v0;               // first vocabulary row of the piece
     int group_m;          // m-blocks per raster group
-    int a_bytes;          // bytes of an A tile: rows beyond the call's are not loaded
+    int a_bytes;          // bytes of a block of A: rows beyond the call's are not loaded
     int early;            // Stats: the operands are the call's own, all rows in their order
     int splits;           // Dh, DwParts: runs of the contraction at most
     int run_slots;        // clusters that they are chosen for
@@ -232,12 +241,13 @@ __device__ __forceinline__ float rescale(float from, float to, float c2) {
     return from == -INFINITY ? 0.0f : exp2_approx((finite_or_zero(from) - finite_or_zero(to)) * c2);
 }
 
-template <int kCtaGroup, int kTileN, int kOp, bool kHalf>
+template <int kCtaGroup, int kTileN, int kOp, bool kHalf, int kSubM>
 __global__ void __launch_bounds__(kThreads, 1)
 vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmA1,
                   const __grid_constant__ CUtensorMap tmB0, const __grid_constant__ CUtensorMap tmB1,
                   const __grid_constant__ CUtensorMap tmD, const Params p) {
-    using C = Cfg<kCtaGroup, kTileN>;
+    using C = Cfg<kCtaGroup, kTileN, kSubM>;
+    static_assert(kSubM == 1 || kOp == kDw, "one accumulator is read while the other is filled");
     constexpr int kStages = C::kStages;
     constexpr int kHalfN = kTileN / 2;
     constexpr int kTmemCols = 2 * kTileN;  // two accumulators
@@ -340,6 +350,7 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
     // the tiles in flight share rows of both operands in L2.
     struct Tile {
         int mb, nb, kb0, kb1, split;
+        int subs;  // blocks of rows that the tile has
     };
     auto tile_of = [&](int t) {
         Tile w;
@@ -359,6 +370,7 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
         const int r = t - g * per_group;
         w.mb = first + r % gsize;
         w.nb = r / gsize;
+        w.subs = kSubM == 1 || m_ext - w.mb * C::kTileM <= C::kSubRows ? 1 : 2;
         return w;
     };
     auto queue_wait = [&](uint32_t qs, uint32_t qph, int code) -> bool {
@@ -433,18 +445,24 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
                     const uint32_t sb = sa + C::kABytes;
                     const uint32_t fb = full0 + 8 * stage;
                     const uint32_t bar = kPair ? mapa_shared(fb, 0) : fb;
-                    if (rank == 0) mbar_arrive_expect_tx(fb, kCtaGroup * (p.a_bytes + C::kBBytes));
+                    if (rank == 0) mbar_arrive_expect_tx(fb, kCtaGroup * (p.a_bytes * w.subs + C::kBBytes));
                     auto load = [&](uint32_t dst, const CUtensorMap* map, int x, int y) {
                         if constexpr (kPair) tma_load_2d_pair(dst, map, bar, x, y);
                         else tma_load_2d(dst, map, bar, x, y);
                     };
                     const int kc = kb * kBK;
-                    if constexpr (kAMn) {
 #pragma unroll
-                        for (int i = 0; i < kRowsPerCta / 64; ++i)
-                            load(sa + i * kBoxBytes, tmA, a_m + 64 * i, kc);
-                    } else {
-                        load(sa, tmA, kc, a_m);
+                    for (int sm = 0; sm < kSubM; ++sm) {
+                        if (sm >= w.subs) break;
+                        const uint32_t dst = sa + sm * C::kASubBytes;
+                        const int row = a_m + sm * C::kSubRows;
+                        if constexpr (kAMn) {
+#pragma unroll
+                            for (int i = 0; i < kRowsPerCta / 64; ++i)
+                                load(dst + i * kBoxBytes, tmA, row + 64 * i, kc);
+                        } else {
+                            load(dst, tmA, kc, row);
+                        }
                     }
                     if constexpr (kBMn) {
                         const int y = kOp == kDh ? p.v0 + kc : kc;
@@ -495,54 +513,91 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
                 if (t < 0) break;
                 const Tile w = tile_of(t);
                 if (w.kb0 == w.kb1) continue;
-                for (int kb = w.kb0; kb < w.kb1; ++kb) {
-                    // A unit is what one accumulator sums up: the whole contraction, or
-                    // kDrain k-slices of it for the statistics.
-                    const int in_unit = kOp == kStats ? (kb - w.kb0) % kDrain : kb - w.kb0;
-                    const uint32_t slot = unit & 1;
-                    const uint32_t d_tmem = tmem_base + slot * kTileN;
-                    if (in_unit == 0) {
-                        if (!mbar_wait(tempty0 + 8 * slot, ((unit >> 1) & 1) ^ 1, status, p.timeout_ns,
-                                              B200_DEV_TIMEOUT_MMA_TMEM)) {
-                            ok = false;
-                            break;
-                        }
-                        tc_fence_after();
-                    }
-                    if (!mbar_wait(full0 + 8 * stage, phase, status, p.timeout_ns,
-                                   B200_DEV_TIMEOUT_MMA_FULL)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    const uint32_t sa = sbase + stage * C::kStageBytes;
-                    const uint32_t sb = sa + C::kABytes;
+                // The products of a block of rows with the k-slice in ring slot `st`.
+                auto multiply = [&](uint32_t slot, int sm, uint32_t st, bool first) {
+                    const uint32_t sa = sbase + st * C::kStageBytes + sm * C::kASubBytes;
+                    const uint32_t sb = sbase + st * C::kStageBytes + C::kABytes;
 #pragma unroll
                     for (int k = 0; k < kBK / 16; ++k) {
                         // 16 elements down the contraction: 32 bytes inside a K-major row,
                         // 16 rows of 128 bytes in an MN-major box.
                         const uint64_t da = kAMn ? smem_desc_mn_sw128(sa + 2048 * k) : smem_desc_sw128(sa + 32 * k);
                         const uint64_t db = kBMn ? smem_desc_mn_sw128(sb + 2048 * k) : smem_desc_sw128(sb + 32 * k);
-                        umma_bf16<kCtaGroup>(d_tmem, da, db, idesc, (in_unit != 0 || k != 0) ? 1u : 0u);
+                        umma_bf16<kCtaGroup>(tmem_base + slot * kTileN, da, db, idesc, !first || k != 0 ? 1u : 0u);
                     }
-                    const uint32_t eb = empty0 + 8 * stage;
+                };
+                auto commit = [&](uint32_t bar) {
                     if constexpr (!kPair) {
-                        umma_commit<1>(eb);
+                        umma_commit<1>(bar);
                     } else {
-                        umma_commit<2>(mapa_shared(eb, 0));
-                        umma_commit<2>(mapa_shared(eb, 1));
+                        umma_commit<2>(mapa_shared(bar, 0));
+                        umma_commit<2>(mapa_shared(bar, 1));
                     }
-                    if (++stage == kStages) { stage = 0; phase ^= 1; }
-                    if (kb + 1 == w.kb1 || (kOp == kStats && in_unit == kDrain - 1)) {
-                        const uint32_t tb = tfull0 + 8 * slot;
-                        if constexpr (!kPair) {
-                            umma_commit<1>(tb);
-                        } else {
-                            umma_commit<2>(mapa_shared(tb, 0));
-                            umma_commit<2>(mapa_shared(tb, 1));
+                };
+                auto wait_slot = [&](uint32_t u) -> bool {
+                    if (!mbar_wait(tempty0 + 8 * (u & 1), ((u >> 1) & 1) ^ 1, status, p.timeout_ns,
+                                   B200_DEV_TIMEOUT_MMA_TMEM)) {
+                        return false;
+                    }
+                    tc_fence_after();
+                    return true;
+                };
+                auto wait_full = [&](uint32_t st, uint32_t ph) -> bool {
+                    if (!mbar_wait(full0 + 8 * st, ph, status, p.timeout_ns, B200_DEV_TIMEOUT_MMA_FULL)) return false;
+                    tc_fence_after();
+                    return true;
+                };
+                auto next_stage = [&](uint32_t& st, uint32_t& ph) {
+                    if (++st == kStages) { st = 0; ph ^= 1; }
+                };
+                if (kSubM == 1 || w.subs == 1) {
+                    for (int kb = w.kb0; kb < w.kb1; ++kb) {
+                        // A unit is what one accumulator sums up: the whole contraction, or
+                        // kDrain k-slices of it for the statistics.
+                        const int in_unit = kOp == kStats ? (kb - w.kb0) % kDrain : kb - w.kb0;
+                        ok = (in_unit != 0 || wait_slot(unit)) && wait_full(stage, phase);
+                        if (!ok) break;
+                        multiply(unit & 1, 0, stage, in_unit == 0);
+                        commit(empty0 + 8 * stage);
+                        next_stage(stage, phase);
+                        if (kb + 1 == w.kb1 || (kOp == kStats && in_unit == kDrain - 1)) {
+                            commit(tfull0 + 8 * (unit & 1));
+                            ++unit;
                         }
-                        ++unit;
                     }
+                } else {
+                    // Two blocks of rows: the first one runs ahead over the ring while the
+                    // second one's accumulator is still being read; those ring slots are
+                    // held until the second has used them too.
+                    const int slices = w.kb1 - w.kb0, head = min(kStages, slices);
+                    const uint32_t slot0 = unit & 1, slot1 = slot0 ^ 1;
+                    uint32_t st = stage, ph = phase;
+                    ok = wait_slot(unit);
+                    for (int i = 0; ok && i < head; ++i) {
+                        ok = wait_full(st, ph);
+                        if (!ok) break;
+                        multiply(slot0, 0, st, i == 0);
+                        if (i == slices - 1) commit(tfull0 + 8 * slot0);
+                        next_stage(st, ph);
+                    }
+                    ok = ok && wait_slot(unit + 1);
+                    for (int i = 0; ok && i < head; ++i) {
+                        multiply(slot1, 1, stage, i == 0);
+                        if (i == slices - 1) commit(tfull0 + 8 * slot1);
+                        commit(empty0 + 8 * stage);
+                        next_stage(stage, phase);
+                    }
+                    for (int i = head; ok && i < slices; ++i) {
+                        ok = wait_full(stage, phase);
+                        if (!ok) break;
+                        multiply(slot0, 0, stage, false);
+                        if (i == slices - 1) commit(tfull0 + 8 * slot0);
+                        multiply(slot1, 1, stage, false);
+                        if (i == slices - 1) commit(tfull0 + 8 * slot1);
+                        commit(empty0 + 8 * stage);
+                        next_stage(stage, phase);
+                    }
+                    unit += 2;
                 }
                 if (status == nullptr) {
                     griddep_wait();
@@ -602,18 +657,23 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
                 bulk_commit_group();
             }
         };
+        Tile w{};
+        int sm = 0;  // block of rows of the tile that comes next
         auto pack = [](float lo, float hi) { return kHalf ? pack_half2(lo, hi) : pack_bf16x2(lo, hi); };
 
         while (true) {
-            if (!__all_sync(0xffffffffu, queue_wait(qs, qph, B200_DEV_TIMEOUT_EPILOGUE))) break;
-            const int t = ring[qs];
-            __syncwarp();
-            if (lane == 0) queue_release(qs);
-            if (++qs == kQueue) { qs = 0; qph ^= 1; }
-            if (t < 0) break;
-            const Tile w = tile_of(t);
-            if (w.kb0 == w.kb1) continue;
-            const int row0 = w.mb * C::kTileM + static_cast<int>(rank) * kRowsPerCta + q * 32;
+            if (sm == 0) {
+                if (!__all_sync(0xffffffffu, queue_wait(qs, qph, B200_DEV_TIMEOUT_EPILOGUE))) break;
+                const int t = ring[qs];
+                __syncwarp();
+                if (lane == 0) queue_release(qs);
+                if (++qs == kQueue) { qs = 0; qph ^= 1; }
+                if (t < 0) break;
+                w = tile_of(t);
+                if (w.kb0 == w.kb1) continue;
+            }
+            const int row0 = w.mb * C::kTileM + sm * C::kSubRows + static_cast<int>(rank) * kRowsPerCta + q * 32;
+            sm = sm + 1 < w.subs ? sm + 1 : 0;
             const int col0 = w.nb * kTileN + half * kHalfN;  // first column of this warp
             const uint32_t t_lane = tmem_base + half * kHalfN + (static_cast<uint32_t>(q * 32) << 16);
 
@@ -848,23 +908,29 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
                 }
                 release_unit();
             } else {
-#pragma unroll 1
+                // The whole block rounded into registers before any store: with two blocks
+                // per tile no other accumulator is free meanwhile.
+                uint32_t pk[kHalfN / 64][32];
+#pragma unroll
                 for (int c = 0; c < kHalfN / 64; ++c) {
-                    uint32_t r0[32], r1[32], pk[32];
+                    uint32_t r0[32], r1[32];
                     tmem_ld_32x32b_x32(t_row + c * 64, r0);
                     tmem_ld_32x32b_x32(t_row + c * 64 + 32, r1);
                     tmem_ld_wait();
-                    const int x = col0 + c * 64;
-                    if (x >= p.n || row0 >= p.m) break;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        pk[i] = pack(alpha * __uint_as_float(r0[2 * i]), alpha * __uint_as_float(r0[2 * i + 1]));
-                        pk[16 + i] = pack(alpha * __uint_as_float(r1[2 * i]), alpha * __uint_as_float(r1[2 * i + 1]));
+                        pk[c][i] = pack(alpha * __uint_as_float(r0[2 * i]), alpha * __uint_as_float(r0[2 * i + 1]));
+                        pk[c][16 + i] = pack(alpha * __uint_as_float(r1[2 * i]), alpha * __uint_as_float(r1[2 * i + 1]));
                     }
-                    stage_chunk(pk);
-                    store_chunk(x, p.v0 + row0, false);
                 }
                 release_unit();
+#pragma unroll
+                for (int c = 0; c < kHalfN / 64; ++c) {
+                    const int x = col0 + c * 64;
+                    if (x >= p.n || row0 >= p.m) break;
+                    stage_chunk(pk[c]);
+                    store_chunk(x, p.v0 + row0, false);
+                }
             }
         }
         if (lane == 0) bulk_wait_group<0>();
@@ -1359,6 +1425,7 @@ struct Layout {
     int64_t tile_m, tile_m_h, piece, pieces, rows_pad;
     int64_t splits_h, splits_w, slices_h;  // runs of dH's and dW's contractions at most
     int cost16_h, cost16_w;
+    int sub_w;                             // blocks of 256 rows per tile of dW
     // Offsets in the workspace.
     int64_t flag, rowmap, inv, ecol, eq, epos;           // both directions
     int64_t zsel, part, row_loss, gathered_forward;
@@ -1499,6 +1566,14 @@ static Layout layout_for(const B200VocabLossDesc& d, int64_t sms) {
         return std::max<int64_t>(1, std::min<int64_t>(kMaxSplits, kPartialBytes / (4 * rows * l.ld_part)));
     };
     auto rounds_of = [](int64_t tiles, int64_t slots_) { return ceil_div(tiles, slots_); };
+    // dW of n blocks of columns in tiles of one or two blocks: with two, a tile's start
+    // waits for TMEM (8 k-slices); with one, its operands keep all SMs 8 % below the
+    // products' rate over many rounds.
+    auto dw_blocks = [&](int64_t n, int64_t sub) {
+        const int64_t rounds = rounds_of(ceil_div(n, sub) * nb, pairs);
+        if (sub == 2) return rounds * (2 * kt + 8);
+        return rounds >= 4 ? rounds * kt * 27 / 25 : rounds * kt;
+    };
     auto cost16 = [&](int64_t rows) { return static_cast<int>(std::min<int64_t>(16 * 8 * rows * l.ld_part / run_bytes, 1 << 24)); };
     int64_t best = -1;
     for (int64_t i = in_l2 < least ? -1 : 0; least + i * step <= most; ++i) {
@@ -1517,7 +1592,10 @@ static Layout layout_for(const B200VocabLossDesc& d, int64_t sms) {
             return std::max(rounds_of(mb * nb * s_h, slots_h) * ceil_div(n * (kBN / kBK), s_h), hbm(n)) + 8;
         }) + 8 * l.rows_pad * l.ld_part * (s_h - 1 + pieces - 1) / run_bytes;
         auto dw_of = [&](int64_t s) {
-            return both([&](int64_t n) { return std::max(rounds_of(n * nb * s, pairs) * ceil_div(kt, s), hbm(n)) + 8; }) +
+            auto products = [&](int64_t n) {
+                return s > 1 ? rounds_of(n * nb * s, pairs) * ceil_div(kt, s) : std::min(dw_blocks(n, 1), dw_blocks(n, 2));
+            };
+            return both([&](int64_t n) { return std::max(products(n), hbm(n)) + 8; }) +
                    (s > 1 ? 6 + 8 * b * kBN * l.ld_part * s / run_bytes : 0);
         };
         int64_t s_w = pieces > 1 ? 1
@@ -1532,6 +1610,7 @@ static Layout layout_for(const B200VocabLossDesc& d, int64_t sms) {
             l.pieces = pieces;
             l.splits_h = s_h;
             l.splits_w = s_w;
+            l.sub_w = s_w == 1 && dw_blocks(b, 2) < dw_blocks(b, 1) ? 2 : 1;
             l.slices_h = slices_h;
         }
     }
@@ -1573,15 +1652,16 @@ static Layout layout_for(const B200VocabLossDesc& d, int64_t sms) {
 using KernelFn = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, Params);
 
 struct Variant {
-    int cta_group, tile_n, op;
+    int cta_group, tile_n, op, sub_m;
     bool fp16;
     KernelFn fn;
     int smem;
 };
 
-template <int kCtaGroup, int kTileN, int kOp, bool kHalf = false>
+template <int kCtaGroup, int kTileN, int kOp, bool kHalf = false, int kSubM = 1>
 static Variant variant() {
-    return {kCtaGroup, kTileN, kOp, kHalf, vocab_gemm_kernel<kCtaGroup, kTileN, kOp, kHalf>, Cfg<kCtaGroup, kTileN>::kSmemBytes};
+    return {kCtaGroup, kTileN, kOp, kSubM, kHalf, vocab_gemm_kernel<kCtaGroup, kTileN, kOp, kHalf, kSubM>,
+            Cfg<kCtaGroup, kTileN, kSubM>::kSmemBytes};
 }
 
 // Every product in the shapes that the layout can choose.
@@ -1593,17 +1673,20 @@ static const Variant* variants(int* count) {
         variant<2, 256, kGrad, true>(), variant<1, 256, kGrad, true>(), variant<1, 128, kGrad, true>(),
         variant<2, 256, kDh>(), variant<1, 256, kDh>(),
         variant<2, 256, kDw, false>(), variant<2, 256, kDw, true>(), variant<2, 256, kDwParts>(),
+        variant<2, 256, kDw, false, 2>(), variant<2, 256, kDw, true, 2>(),
     };
     *count = static_cast<int>(sizeof(all) / sizeof(all[0]));
     return all;
 }
 
-static const Variant* variant_of(int cta_group, int tile_n, int op, bool fp16) {
+static const Variant* variant_of(int cta_group, int tile_n, int op, bool fp16, int sub_m) {
     int n = 0;
     const Variant* all = variants(&n);
     const bool half = fp16 && (op == kGrad || op == kDw);
     for (int i = 0; i < n; ++i)
-        if (all[i].cta_group == cta_group && all[i].tile_n == tile_n && all[i].op == op && all[i].fp16 == half) return all + i;
+        if (all[i].cta_group == cta_group && all[i].tile_n == tile_n && all[i].op == op && all[i].fp16 == half &&
+            all[i].sub_m == sub_m)
+            return all + i;
     return nullptr;
 }
 
@@ -1827,12 +1910,13 @@ static int group_for(int64_t tile_m, int64_t k) {
 
 static int64_t slots_of(const Call& c, int cta_group) { return cta_group == 2 ? c.dev.pairs : c.dev.sms; }
 
-static int launch_gemm(const Call& c, int op, int cta_group, int tile_n, int64_t tiles, const CUtensorMap& a0,
+static int launch_gemm(const Call& c, int op, int cta_group, int tile_n, int sub_m, int64_t tiles, const CUtensorMap& a0,
                        const CUtensorMap& a1, const CUtensorMap& b0, const CUtensorMap& b1, const CUtensorMap& dmap,
                        const Params& p) {
-    const Variant* v = variant_of(cta_group, tile_n, op, p.fp16);
+    const Variant* v = variant_of(cta_group, tile_n, op, p.fp16, sub_m);
     if (v == nullptr) {
-        set_error("internal error: no kernel for product %d with %d x %d tiles", op, kRowsPerCta * cta_group, tile_n);
+        set_error("internal error: no kernel for product %d with %d x %d tiles", op, kRowsPerCta * cta_group * sub_m,
+                  tile_n);
         return B200_ERR_INTERNAL;
     }
     const int grid = static_cast<int>(std::max<int64_t>(1, std::min(tiles, slots_of(c, cta_group)))) * cta_group;
@@ -1902,7 +1986,7 @@ static int forward(const B200VocabLossDesc* d, const void* hidden, const void* w
     p.early = !l.gather_forward;
     p.part_ld = ceil_div(d->vocab, l.tile_n / 2);
     p.a_bytes = box_m * kBK * 2;
-    rc = launch_gemm(c, d->hidden <= kDrainMost * kBK ? kStatsShort : kStats, l.cta_group, l.tile_n,
+    rc = launch_gemm(c, d->hidden <= kDrainMost * kBK ? kStatsShort : kStats, l.cta_group, l.tile_n, 1,
                      ceil_div(d->rows, l.tile_m) * ceil_div(d->vocab, l.tile_n), a0, a1, b, b, b, p);
     if (rc != B200_OK) return rc;
     MergeParams m{};
@@ -1984,8 +2068,8 @@ static int backward(const B200VocabLossDesc* d, const void* hidden, const void* 
         p.k = static_cast<int>(D);
         p.group_m = group_for(l.tile_m, D);
         p.a_bytes = box_m * kBK * 2;
-        rc = launch_gemm(c, kGrad, l.cta_group, l.tile_n, ceil_div(T, l.tile_m) * ceil_div(vp, l.tile_n), h_k, hg_k, w_k, w_k,
-                         g_st, p);
+        rc = launch_gemm(c, kGrad, l.cta_group, l.tile_n, 1, ceil_div(T, l.tile_m) * ceil_div(vp, l.tile_n), h_k, hg_k, w_k,
+                         w_k, g_st, p);
         if (rc == B200_OK && d_hidden != nullptr) {
             Params q = p;
             q.n = static_cast<int>(D);
@@ -1998,21 +2082,21 @@ static int backward(const B200VocabLossDesc* d, const void* hidden, const void* 
             q.run_cost16 = l.cost16_h;
             q.rows_pad = static_cast<int>(l.rows_pad);
             q.accumulate = v0 > 0;
-            rc = launch_gemm(c, kDh, l.cta_group_h, kBN, l.rows_pad / l.tile_m_h * ceil_div(D, kBN) * l.splits_h, g_k, g_k,
+            rc = launch_gemm(c, kDh, l.cta_group_h, kBN, 1, l.rows_pad / l.tile_m_h * ceil_div(D, kBN) * l.splits_h, g_k, g_k,
                              w_mn, w_mn, dh_st, q);
         }
         if (rc == B200_OK && d_weight != nullptr) {
             Params q = p;
             q.m = static_cast<int>(vp);
             q.n = static_cast<int>(D);
-            q.group_m = group_for(2 * kRowsPerCta, T);
+            q.group_m = group_for(2 * kRowsPerCta * l.sub_w, T);
             q.a_bytes = kRowsPerCta * kBK * 2;
             q.splits = static_cast<int>(l.splits_w);
             q.run_slots = static_cast<int>(slots_of(c, 2));
             q.run_cost16 = l.cost16_w;
             q.rows_pad = static_cast<int>(l.piece);
-            rc = launch_gemm(c, l.splits_w > 1 ? kDwParts : kDw, 2, kBN,
-                             ceil_div(vp, 2 * kRowsPerCta) * ceil_div(D, kBN) * l.splits_w, g_mn, g_mn, h_mn, hg_mn, dw_st, q);
+            rc = launch_gemm(c, l.splits_w > 1 ? kDwParts : kDw, 2, kBN, l.sub_w,
+                             ceil_div(vp, 2 * kRowsPerCta * l.sub_w) * ceil_div(D, kBN) * l.splits_w, g_mn, g_mn, h_mn, hg_mn, dw_st, q);
         }
     }
     if (rc != B200_OK) return rc;
@@ -2065,6 +2149,7 @@ int b200_vocab_loss_info(const B200VocabLossDesc* desc, int sm_count, B200VocabL
     out->cta_group = l.cta_group;
     out->tile_m = l.tile_m;
     out->tile_n = l.tile_n;
+    out->tile_m_weight = 2 * b200::vl::kRowsPerCta * l.sub_w;
     out->piece = l.piece;
     out->pieces = l.pieces;
     out->splits_hidden = l.splits_h;

@@ -434,6 +434,7 @@ typedef struct B200VocabLossInfo {
     int64_t cta_group;     /* CTAs per tile of the logits */
     int64_t tile_m;        /* rows and columns of such a tile */
     int64_t tile_n;
+    int64_t tile_m_weight; /* rows of a tile of d_weight */
     int64_t piece;         /* columns of the vocabulary per step of the backward pass */
     int64_t pieces;
     int64_t splits_hidden; /* runs of the contraction over the vocabulary in d_hidden, at most */

@@ -173,6 +173,15 @@ def test_weight_gradient_in_runs():
     ce(5000, 300, 64, reduction="sum", ignored=0.995)
 
 
+@pytest.mark.parametrize("rows,vocab,dtype", [(4096, 28990, BF16), (4090, 56976, FP16)])
+def test_weight_gradient_two_blocks_per_tile(rows, vocab, dtype):
+    """Tiles of 512 rows of dW, the last of them with one block or less; one piece and two."""
+    from b200gemm import vocab_loss
+    assert vocab_loss.policy(rows, vocab, 264)["tile_m_weight"] == 512
+    ce(rows, vocab, 264, dtype, reduction="sum")
+    ce(rows, vocab, 264, dtype, reduction="sum", ignored=0.97)
+
+
 def test_hidden_gradient_in_runs():
     from b200gemm import vocab_loss
     assert vocab_loss.policy(130, 20000, 64)["splits_hidden"] > 1
