@@ -978,23 +978,26 @@ struct TeacherParams {
     int* flag;
 };
 
-// A warp turns one row of a teacher's logits into its target distribution:
+// A block turns one row of a teacher's logits into its target distribution:
 // softmax over the entries that are there, sorted by column, entries of one
 // column added up in the order given. 2 x 8 bytes per entry in, 8 out. It also
-// leaves where in the row each half tile of the vocabulary begins.
-constexpr int kTeacherWarps = 8;
-__global__ void __launch_bounds__(kTeacherWarps * 32) teacher_kernel(const TeacherParams p, int pad) {
-    extern __shared__ unsigned long long teacher_smem[];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    unsigned long long* key = teacher_smem + static_cast<size_t>(warp) * pad;
-    float* prob = reinterpret_cast<float*>(teacher_smem + static_cast<size_t>(kTeacherWarps) * pad) +
-                  static_cast<size_t>(warp) * pad;
-    const int t = blockIdx.x * kTeacherWarps + warp;
+// leaves where in the row each half tile of the vocabulary begins. What it takes is
+// latency: sorting steps and, for every half tile, a search (two rows of 109 over
+// 108645 columns: 20 us with a warp per row, 8 with four). Many rows of few entries
+// take a warp each instead (7844 rows of 6: 10 against 16 us).
+template <int kTeacherThreads>
+__global__ void __launch_bounds__(kTeacherThreads) teacher_kernel(const TeacherParams p, int pad) {
+    constexpr int kWarps = kTeacherThreads / 32;
+    __shared__ unsigned long long key[kMaxTop];
+    __shared__ float prob[kMaxTop];
+    __shared__ unsigned cols[kMaxTop];
+    __shared__ float red[2][kWarps];
+    __shared__ int heads_of[kWarps];
     griddep_launch_dependents();
-    if (t >= p.rows) return;
+    const int t = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     float mx = -INFINITY;
     bool any = false, bad = false, nan = false;
-    for (int k = lane; k < pad; k += 32) {
+    for (int k = tid; k < pad; k += kTeacherThreads) {
         float l = -INFINITY;
         unsigned col = kNoCol;
         if (k < p.top) {
@@ -1013,23 +1016,28 @@ __global__ void __launch_bounds__(kTeacherWarps * 32) teacher_kernel(const Teach
         prob[k] = l;
         mx = fmaxf(mx, l);
     }
-    any = __any_sync(0xffffffffu, any);
-    bad = __any_sync(0xffffffffu, bad);
-    nan = __any_sync(0xffffffffu, nan);
     for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    if (lane == 0) red[0][warp] = mx;
+    any = __syncthreads_or(any);
+    bad = __syncthreads_or(bad);
+    nan = __syncthreads_or(nan);
+    for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, red[0][w]);
     float sum = 0.0f;
-    for (int k = lane; k < pad; k += 32) {
+    for (int k = tid; k < pad; k += kTeacherThreads) {
         const float e = prob[k] == -INFINITY ? 0.0f : expf(prob[k] - mx);
         prob[k] = e;
         sum += e;
     }
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) red[1][warp] = sum;
+    __syncthreads();
+    sum = red[1][0];
+    for (int w = 1; w < kWarps; ++w) sum += red[1][w];
     const float inv = nan ? NAN : 1.0f / sum;
-    __syncwarp();
     // Bitonic sort of (column, position).
     for (int size = 2; size <= pad; size <<= 1) {
         for (int stride = size >> 1; stride; stride >>= 1) {
-            for (int i = lane; i < pad / 2; i += 32) {
+            for (int i = tid; i < pad / 2; i += kTeacherThreads) {
                 const int lo = 2 * i - (i & (stride - 1));
                 const int hi = lo + stride;
                 const unsigned long long a = key[lo], b = key[hi];
@@ -1038,15 +1046,14 @@ __global__ void __launch_bounds__(kTeacherWarps * 32) teacher_kernel(const Teach
                     key[hi] = a;
                 }
             }
-            __syncwarp();
+            __syncthreads();
         }
     }
     int out = 0;
-    unsigned* cols = reinterpret_cast<unsigned*>(prob + static_cast<size_t>(kTeacherWarps) * pad);
     int* ecol = p.ecol + static_cast<long long>(t) * p.top;
     float* eq = p.eq + static_cast<long long>(t) * p.top;
-    for (int base = 0; base < pad; base += 32) {
-        const int i = base + lane;
+    for (int base = 0; base < pad; base += kTeacherThreads) {
+        const int i = base + tid;
         unsigned col = kNoCol;
         bool first = false;
         if (i < pad) {
@@ -1054,25 +1061,30 @@ __global__ void __launch_bounds__(kTeacherWarps * 32) teacher_kernel(const Teach
             first = col != kNoCol && (i == 0 || static_cast<unsigned>(key[i - 1] >> 32) != col);
         }
         const unsigned heads = __ballot_sync(0xffffffffu, first);
+        if (lane == 0) heads_of[warp] = __popc(heads);
+        __syncthreads();
+        int o = out + __popc(heads & ((1u << lane) - 1));
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) o += heads_of[w];
+            out += heads_of[w];
+        }
         if (first) {
             float v = 0.0f;
             for (int j = i; j < pad && static_cast<unsigned>(key[j] >> 32) == col; ++j)
                 v += prob[static_cast<unsigned>(key[j])];
-            const int o = out + __popc(heads & ((1u << lane) - 1));
             ecol[o] = static_cast<int>(col);
             cols[o] = col;
             eq[o] = v * inv;
         }
-        out += __popc(heads);
+        __syncthreads();
     }
-    for (int i = out + lane; i < p.top; i += 32) {
+    for (int i = out + tid; i < p.top; i += kTeacherThreads) {
         ecol[i] = kNoCol;
         eq[i] = 0.0f;
     }
-    if (lane == 0) p.flag[t] = bad ? kBad : (any ? kLoss : kNoLoss);
-    __syncwarp();
+    if (tid == 0) p.flag[t] = bad ? kBad : (any ? kLoss : kNoLoss);
     unsigned short* epos = p.epos + t * p.epos_ld;
-    for (long long j = lane; j < p.epos_ld; j += 32) {
+    for (long long j = tid; j < p.epos_ld; j += kTeacherThreads) {
         const long long col = j * p.half;
         int lo = 0, hi = out;
         while (lo < hi) {
@@ -1121,23 +1133,32 @@ __global__ void __launch_bounds__(1024) rows_kernel(const RowsParams p) {
     __syncthreads();
     for (int r0 = 0; r0 < p.rows; r0 += 1024 * kPer) {
         const int t0 = r0 + tid * kPer;
+        // Four rows as one access wherever all four are there: one row at a time, 16
+        // bytes apart between lanes, took 14 us for 8192 rows.
+        const bool four = t0 + kPer <= p.rows;
         int f[kPer], col[kPer], count = 0;
+        if (p.target == nullptr && four) {
+            const int4 v = *reinterpret_cast<const int4*>(p.flag + t0);
+            f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+        }
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
             const int t = t0 + j;
-            f[j] = kNoLoss;
+            col[j] = kNoCol;
+            if (p.target != nullptr || !four) f[j] = kNoLoss;
             if (t < p.rows) {
                 if (p.target != nullptr) {
                     const long long c = index_at(p.target, p.index_bytes, t);
                     f[j] = c == p.ignore ? kNoLoss : (c >= 0 && c < p.vocab ? kLoss : kBad);
                     col[j] = f[j] == kLoss ? static_cast<int>(c) : kNoCol;
-                    p.flag[t] = f[j];
-                } else {
+                    if (!four) p.flag[t] = f[j];
+                } else if (!four) {
                     f[j] = p.flag[t];
                 }
             }
             count += f[j] != kNoLoss;
         }
+        if (p.target != nullptr && four) *reinterpret_cast<int4*>(p.flag + t0) = make_int4(f[0], f[1], f[2], f[3]);
         // Rows with a loss before this thread's first one: scan in the warp, then
         // over the warps.
         int upto = count;
@@ -1157,23 +1178,34 @@ __global__ void __launch_bounds__(1024) rows_kernel(const RowsParams p) {
         }
         __syncthreads();
         int at = base + (warp ? warp_sum[warp - 1] : 0) + upto - count;
+        const int at0 = p.gather ? at : t0;
+        const bool together = four && (at0 & 3) == 0 && (count == kPer || !p.gather);
+        int inv[kPer];
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
             const int t = t0 + j;
-            if (t >= p.rows) break;
             const bool in = f[j] != kNoLoss;
             const int i = p.gather ? at : t;
             at += in;
-            p.inv[t] = in ? i : -1;
+            inv[j] = in ? i : -1;
+            if (t >= p.rows) continue;
+            if (!four) p.inv[t] = inv[j];
             if (p.gather && !in) continue;
-            p.rowmap[i] = t;
-            if (p.target != nullptr) p.ecol[i] = col[j];
+            if (!together) {
+                p.rowmap[i] = t;
+                if (p.target != nullptr) p.ecol[i] = col[j];
+            }
             if (p.rgrad == nullptr) continue;
             const float g = p.reduction == B200_VL_NONE ? p.grad[t] : 1.0f;
             // p - 1 at the one target, without the difference of two numbers near 1.
             const float below = p.target != nullptr ? expm1f(p.target_logp[t]) : 0.0f;
             p.rgrad[i] = f[j] == kBad ? make_float4(NAN, NAN, NAN, 0.0f) : make_float4(g, -p.lse[t] * kLog2e, g * below, 0.0f);
             gmax = fabsf(g) > gmax || g != g ? fabsf(g) : gmax;  // a NaN stays
+        }
+        if (four) *reinterpret_cast<int4*>(p.inv + t0) = make_int4(inv[0], inv[1], inv[2], inv[3]);
+        if (together) {
+            *reinterpret_cast<int4*>(p.rowmap + at0) = make_int4(t0, t0 + 1, t0 + 2, t0 + 3);
+            if (p.target != nullptr) *reinterpret_cast<int4*>(p.ecol + at0) = make_int4(col[0], col[1], col[2], col[3]);
         }
         __syncthreads();
         if (tid == 0) base += warp_sum[31];
@@ -1723,7 +1755,8 @@ static int device_state(DeviceState* out) {
                                                cudaFuncAttributeMaxDynamicSharedMemorySize, all[i].smem));
         // Loaded now, not at a first launch that a stream capture may hold.
         cudaFuncAttributes loaded;
-        for (const void* fn : {reinterpret_cast<const void*>(teacher_kernel), reinterpret_cast<const void*>(rows_kernel),
+        for (const void* fn : {reinterpret_cast<const void*>(teacher_kernel<32>), reinterpret_cast<const void*>(teacher_kernel<128>),
+                               reinterpret_cast<const void*>(rows_kernel),
                                reinterpret_cast<const void*>(gather_kernel), reinterpret_cast<const void*>(merge_kernel),
                                reinterpret_cast<const void*>(finish_kernel)})
             B200_CUDA_TRY(cudaFuncGetAttributes(&loaded, fn));
@@ -1850,8 +1883,9 @@ static int launch_rows(const Call& c, const void* index, const void* teacher, co
         t.flag = c.at<int>(l.flag);
         int pad = 2;
         while (pad < t.top) pad *= 2;
-        const int rc = launch(teacher_kernel, static_cast<int>(ceil_div(d.rows, kTeacherWarps)), kTeacherWarps * 32,
-                              kTeacherWarps * pad * 16, 1, false, c.stream, t, pad);
+        const int rc = pad <= 32 && d.rows > 8 * c.dev.sms
+                           ? launch(teacher_kernel<32>, static_cast<int>(d.rows), 32, 0, 1, false, c.stream, t, pad)
+                           : launch(teacher_kernel<128>, static_cast<int>(d.rows), 128, 0, 1, false, c.stream, t, pad);
         if (rc != B200_OK) return rc;
     }
     RowsParams r{};
