@@ -1200,7 +1200,8 @@ __global__ void __launch_bounds__(1024) rows_kernel(const RowsParams p) {
             // p - 1 at the one target, without the difference of two numbers near 1.
             const float below = p.target != nullptr ? expm1f(p.target_logp[t]) : 0.0f;
             p.rgrad[i] = f[j] == kBad ? make_float4(NAN, NAN, NAN, 0.0f) : make_float4(g, -p.lse[t] * kLog2e, g * below, 0.0f);
-            gmax = fabsf(g) > gmax || g != g ? fabsf(g) : gmax;  // a NaN stays
+            // What is infinite or NaN from above stays in its own row.
+            if (isfinite(g)) gmax = fmaxf(gmax, fabsf(g));
         }
         if (four) *reinterpret_cast<int4*>(p.inv + t0) = make_int4(inv[0], inv[1], inv[2], inv[3]);
         if (together) {
@@ -1213,13 +1214,10 @@ __global__ void __launch_bounds__(1024) rows_kernel(const RowsParams p) {
     }
     const int n_valid = base;
     if (p.rgrad != nullptr && p.reduction == B200_VL_NONE) {
-        for (int o = 16; o; o >>= 1) {
-            const float u = __shfl_xor_sync(0xffffffffu, gmax, o);
-            gmax = u > gmax || u != u ? u : gmax;
-        }
+        for (int o = 16; o; o >>= 1) gmax = fmaxf(gmax, __shfl_xor_sync(0xffffffffu, gmax, o));
         if (lane == 0) warp_max[warp] = gmax;
         __syncthreads();
-        for (int i = 0; i < 32; ++i) gmax = warp_max[i] > gmax || warp_max[i] != warp_max[i] ? warp_max[i] : gmax;
+        for (int i = 0; i < 32; ++i) gmax = fmaxf(gmax, warp_max[i]);
         // At most 1, so that G fits half precision whatever the loss is scaled by.
         const float unit = gmax > 0.0f ? gmax : 1.0f;
         for (int i = tid; i < n_valid; i += 1024) {
@@ -1237,7 +1235,7 @@ __global__ void __launch_bounds__(1024) rows_kernel(const RowsParams p) {
         h.compact = h.n_rows != p.rows || p.copy_all;
         h.alpha = 1.0f;
         if (p.rgrad != nullptr) {
-            if (p.reduction == B200_VL_NONE) h.alpha = gmax > 0.0f || gmax != gmax ? gmax * p.tau : p.tau;
+            if (p.reduction == B200_VL_NONE) h.alpha = gmax > 0.0f ? gmax * p.tau : p.tau;
             else h.alpha = p.grad[0] * p.tau / (p.reduction == B200_VL_MEAN ? static_cast<float>(max(n_valid, 1)) : 1.0f);
         }
         *p.head = h;

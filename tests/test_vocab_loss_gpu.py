@@ -393,6 +393,20 @@ def test_upstream_zeros_and_scales():
                   ref.reference(h, w, kept, idx, q, 1.0, "none", up))
 
 
+def test_upstream_infinities_stay_in_their_rows():
+    from b200gemm import vocab_loss
+    g, h, w = make(140, 400, 64)
+    t = torch.randint(0, 400, (140,), generator=g, device="cuda")
+    up = torch.ones(140, device="cuda")
+    _, want, _ = run(vocab_loss.linear_cross_entropy, h, w, (t,), up, reduction="none")
+    up[7], up[130] = math.inf, math.nan
+    _, dh, dw = run(vocab_loss.linear_cross_entropy, h, w, (t,), up, reduction="none")
+    other = torch.ones(140, dtype=torch.bool, device="cuda")
+    other[[7, 130]] = False
+    assert torch.equal(dh[other], want[other]) and not dh[~other].isfinite().any()
+    assert not dw.isfinite().any()
+
+
 @pytest.mark.parametrize("std", [0.0, 3.0])
 def test_flat_and_peaked_logits(std):
     """All logits equal; logits hundreds apart, where all but one probability vanish."""
