@@ -1482,6 +1482,13 @@ static int check_desc(const B200VocabLossDesc* d) {
                   (long long)d->rows, (long long)d->vocab, (long long)d->hidden);
         return B200_ERR_UNSUPPORTED;
     }
+    // Byte counts are in 64 bits, with room for what is kept of each.
+    if (d->rows > (int64_t(1) << 46) / d->hidden || d->vocab > (int64_t(1) << 46) / d->hidden ||
+        d->rows > (int64_t(1) << 50) / d->vocab) {
+        set_error("(rows,vocab,hidden)=(%lld,%lld,%lld): operands must be below 2^46 elements, logits below 2^50",
+                  (long long)d->rows, (long long)d->vocab, (long long)d->hidden);
+        return B200_ERR_UNSUPPORTED;
+    }
     if (d->hidden % 8 != 0) {
         set_error("hidden=%lld: rows must be whole 16-byte units for TMA (hidden %% 8 == 0)", (long long)d->hidden);
         return B200_ERR_UNSUPPORTED;

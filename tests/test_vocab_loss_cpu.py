@@ -93,6 +93,8 @@ def desc(**change):
     (dict(rows=-1), _lib.ERR_INVALID_ARGUMENT), (dict(vocab=0), _lib.ERR_INVALID_ARGUMENT),
     (dict(hidden=0), _lib.ERR_INVALID_ARGUMENT), (dict(rows=2 ** 31), _lib.ERR_UNSUPPORTED),
     (dict(vocab=2 ** 31 - 512), _lib.ERR_UNSUPPORTED), (dict(hidden=100, ld_hidden=104), _lib.ERR_UNSUPPORTED),
+    (dict(rows=2 ** 30, hidden=2 ** 20, ld_hidden=2 ** 20, ld_weight=2 ** 20), _lib.ERR_UNSUPPORTED),
+    (dict(rows=2 ** 28, vocab=2 ** 28, hidden=8, ld_hidden=8, ld_weight=8), _lib.ERR_UNSUPPORTED),
     (dict(ld_hidden=120), _lib.ERR_INVALID_ARGUMENT), (dict(ld_weight=130), _lib.ERR_UNSUPPORTED),
     (dict(dtype=2), _lib.ERR_INVALID_ARGUMENT), (dict(index_bytes=2), _lib.ERR_INVALID_ARGUMENT),
     (dict(reduction=3), _lib.ERR_INVALID_ARGUMENT), (dict(top=257, ld_index=257, ld_teacher=257), _lib.ERR_UNSUPPORTED),
