@@ -222,8 +222,9 @@ __device__ __forceinline__ void tma_reduce_add_2d(const void* tmap, uint32_t src
         : "memory");
 }
 
-// 2^x by the hardware's approximation (absolute error about 2^-22 of the
-// result): every use is a term of a sum of exponentials or a probability.
+// 2^x by the hardware's approximation (off by about 2^-22 of the result, results
+// below 2^-126 are zeros): every use is a term of a sum of exponentials or a
+// probability.
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -324,7 +325,7 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
     // (early), the first tile is loaded and multiplied meanwhile. The kernels before
     // this one in the call write neither, and the first of them began when everything
     // before the call was done. Each role then waits before it touches the workspace, the
-    // status word included (one token over 128256 x 4096: 3 us of 187).
+    // status word included (a 512^3 forward pass as a graph: 16.5 -> 14.5 us).
     const bool early = is_stats(kOp) && p.early;
     int* status = early ? nullptr : status_word;
     if (!early) griddep_wait();
@@ -1460,7 +1461,8 @@ struct Layout {
     int64_t flag, rowmap, inv, ecol, eq, epos;           // both directions
     int64_t zsel, part, row_loss, gathered_forward;
     int64_t rgrad, gathered_backward, g, part_h, part_w;
-    int64_t epos_ld, ld_gathered, ld_part;                        // row pitches on 128-byte lines
+    int64_t epos_ld;
+    int64_t ld_gathered, ld_part;                        // row pitches on 128-byte lines
     int64_t bytes_forward, bytes_backward;
     bool gather_forward;
 };

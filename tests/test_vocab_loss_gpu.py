@@ -303,6 +303,10 @@ def test_no_rows():
         assert loss.shape == ((0,) if reduction == "none" else ()) and not loss.any()
         dh, dw = torch.autograd.grad(loss.sum(), (h, w))
         assert dh.shape == h.shape and dw.shape == w.shape and not dw.any()
+    h = torch.empty(3, 0, 64, dtype=BF16, device="cuda")
+    loss = vocab_loss.linear_distillation(h, w, torch.empty(3, 0, 5, device="cuda"),
+                                          torch.empty(3, 0, 5, dtype=torch.int32, device="cuda"), reduction="none")
+    assert loss.shape == (3, 0)
 
 
 def test_two_streams_at_once():
