@@ -79,7 +79,8 @@ __host__ __device__ constexpr bool is_dw(int op) { return op == kDw || op == kDw
 // What the first kernels of a call leave in the workspace for the others.
 struct Head {
     int status;       // device status word
-    int counter[2];   // tile scheduler: next tile, finished clusters
+    int counter[4];   // tile scheduler: next tile, finished clusters; dW's own pair
+    int g_piece;      // the last piece whose G is known to be complete, from 1
     int ticket;       // finished blocks of the merge kernel
     int n_rows;       // rows that the products run over
     int n_valid;      // rows with a loss
@@ -154,6 +155,7 @@ struct Params {
     int run_cost16;
     int rows_pad;         // Dh, DwParts: rows between two splits' partial sums
     int accumulate;       // Dh: 1 add to the partial sums, 0 write them
+    int piece_no;         // Dh, Dw, DwParts: the piece, from 1
     // Stats, Grad. One target per row (cross entropy): ecol and zsel (Stats) go by
     // the gathered row, rowmap and eq are null. A teacher's: by the row of the call.
     const int* rowmap;    // gathered row -> row
@@ -221,6 +223,13 @@ __device__ __forceinline__ void tma_reduce_add_2d(const void* tmap, uint32_t src
         ::"l"(reinterpret_cast<uint64_t>(tmap)), "r"(src), "r"(x), "r"(y)
         : "memory");
 }
+
+__device__ __forceinline__ void st_release_gpu(int* addr, int v) {
+    asm volatile("st.release.gpu.global.b32 [%0], %1;" ::"l"(addr), "r"(v) : "memory");
+}
+
+// Global memory seen by ordinary loads so far is seen by TMA loads from here on.
+__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.global;" ::: "memory"); }
 
 // 2^x by the hardware's approximation (off by about 2^-22 of the result, results
 // below 2^-126 are zeros): every use is a term of a sum of exponentials or a
@@ -328,7 +337,23 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
     // status word included (a 512^3 forward pass as a graph: 16.5 -> 14.5 us).
     const bool early = is_stats(kOp) && p.early;
     int* status = early ? nullptr : status_word;
-    if (!early) griddep_wait();
+    if constexpr (is_dw(kOp)) {
+        // dW needs G and not the product before it, which is dH: it fills the SMs that
+        // dH leaves, and waits for dH's end at its own (512^3 step as a graph: 43.1 ->
+        // 39.0 us; 8192 x 128256 x 4096: 25.15-25.33 -> 24.99 ms). dH is launched first, waits for G and says so; without its word, dW
+        // waits for all that came before.
+        if (ld_acquire_gpu(&p.head->g_piece) != p.piece_no) griddep_wait();
+        fence_proxy_async();
+    } else if (!early) {
+        griddep_wait();
+    }
+    if constexpr (kOp == kDh) {
+        if (threadIdx.x == 0) {
+            if (blockIdx.x == 0) st_release_gpu(&p.head->g_piece, p.piece_no);
+            griddep_launch_dependents();
+        }
+    }
+    int* const counter = p.head->counter + (is_dw(kOp) ? 2 : 0);
 
     const int n_rows = early ? p.rows : p.head->n_rows;
     const bool compact = !early && p.head->compact != 0;
@@ -404,10 +429,10 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
                         t = -1;
                         if (!waited) griddep_wait();
                         __threadfence();
-                        if (atomicAdd(&p.head->counter[1], 1) == num_clusters - 1) {
+                        if (atomicAdd(&counter[1], 1) == num_clusters - 1) {
                             // Every cluster has made its last fetch: ready for the next launch.
-                            atomicExch(&p.head->counter[0], 0);
-                            atomicExch(&p.head->counter[1], 0);
+                            atomicExch(&counter[0], 0);
+                            atomicExch(&counter[1], 0);
                         }
                     }
                     ring[qs] = t;
@@ -434,9 +459,9 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
                 // early enough to hide the round trip, late enough that a fast cluster
                 // does not take two tiles while a slow one has none.
                 const int fetch_kb = max(w.kb0, w.kb1 - 2 * kStages);
-                if (rank == 0 && w.kb0 == w.kb1) next = atomicAdd(&p.head->counter[0], 1) + num_clusters;
+                if (rank == 0 && w.kb0 == w.kb1) next = atomicAdd(&counter[0], 1) + num_clusters;
                 for (int kb = w.kb0; kb < w.kb1; ++kb) {
-                    if (rank == 0 && kb == fetch_kb && waited) next = atomicAdd(&p.head->counter[0], 1) + num_clusters;
+                    if (rank == 0 && kb == fetch_kb && waited) next = atomicAdd(&counter[0], 1) + num_clusters;
                     if (!mbar_wait(empty0 + 8 * stage, phase ^ 1, status, p.timeout_ns,
                                    B200_DEV_TIMEOUT_PRODUCER)) {
                         ok = false;
@@ -480,7 +505,7 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
                     griddep_wait();
                     status = status_word;
                     waited = true;
-                    if (rank == 0) next = atomicAdd(&p.head->counter[0], 1) + num_clusters;
+                    if (rank == 0) next = atomicAdd(&counter[0], 1) + num_clusters;
                 }
             }
             if (!waited) griddep_wait();
@@ -938,6 +963,9 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
         __syncwarp();
     }
 
+    // Whatever follows dW waits for dW alone, and needs dH too.
+    if constexpr (is_dw(kOp)) griddep_wait();
+
     // Teardown: every role is done with TMEM and with the peer's barriers.
     tc_fence_before();
     if constexpr (kPair) cluster_sync(); else __syncthreads();
@@ -1229,7 +1257,8 @@ __global__ void __launch_bounds__(1024) rows_kernel(const RowsParams p) {
     if (tid == 0) {
         Head h;
         h.status = 0;
-        h.counter[0] = h.counter[1] = 0;
+        for (int i = 0; i < 4; ++i) h.counter[i] = 0;
+        h.g_piece = 0;
         h.ticket = 0;
         h.n_valid = n_valid;
         h.n_rows = p.gather ? n_valid : p.rows;
@@ -2109,6 +2138,7 @@ static int backward(const B200VocabLossDesc* d, const void* hidden, const void* 
         p.k = static_cast<int>(D);
         p.group_m = group_for(l.tile_m, D);
         p.a_bytes = box_m * kBK * 2;
+        p.piece_no = static_cast<int>(v0 / l.piece) + 1;
         rc = launch_gemm(c, kGrad, l.cta_group, l.tile_n, 1, ceil_div(T, l.tile_m) * ceil_div(vp, l.tile_n), h_k, hg_k, w_k,
                          w_k, g_st, p);
         if (rc == B200_OK && d_hidden != nullptr) {
