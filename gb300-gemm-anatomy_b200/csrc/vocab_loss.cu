@@ -1143,51 +1143,91 @@ struct RowsParams {
     const float* target_logp;
     float4* rgrad;        // see Params
     float tau;
+    const uint4* hidden;  // gather: H, and where its copy goes
+    uint4* copy;
+    long long ld, ld_copy;
+    int vecs;             // 16-byte units of a row
 };
 
-// One block numbers the rows that have a loss, in order, and leaves the
-// factors of the backward pass. Four rows per thread and step.
+// Numbers the rows that have a loss, in order, leaves the factors of the backward
+// pass, and copies the rows of H that have a loss (a block of rows of zeros follows
+// the last one) unless every row has one and starts on a 128-byte line. Four rows
+// per thread and step. Every block counts all rows, so that none waits for another;
+// of each group of four rows one block writes what is written, and copies. Latency
+// and the copy bound it (2048 of 4096 rows of 8 KiB: 13 us, where a block that numbers
+// and a launch that copies took 17 and a launch more).
 __global__ void __launch_bounds__(1024) rows_kernel(const RowsParams p) {
-    constexpr int kPer = 4;
+    constexpr int kPer = 4, kChunk = 1024 * kPer;
     __shared__ int warp_sum[32];
     __shared__ float warp_max[32];
     __shared__ int base;
+    __shared__ int4 numbers[1024];  // inv of a chunk
     // What follows may set itself up, and load what the call was given, from the
     // start; it waits for this kernel's end before it looks at the workspace.
     griddep_launch_dependents();
     griddep_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    if (tid == 0) base = 0;
-    float gmax = 0.0f;
-    __syncthreads();
-    for (int r0 = 0; r0 < p.rows; r0 += 1024 * kPer) {
-        const int t0 = r0 + tid * kPer;
-        // Four rows as one access wherever all four are there: one row at a time, 16
-        // bytes apart between lanes, took 14 us for 8192 rows.
-        const bool four = t0 + kPer <= p.rows;
-        int f[kPer], col[kPer], count = 0;
-        if (p.target == nullptr && four) {
+    // Four rows as one access wherever all four are there: one row at a time, 16
+    // bytes apart between lanes, took 14 us for 8192 rows.
+    auto classify = [&](int t0, int (&f)[kPer], int (&col)[kPer]) {
+        const bool four = p.target == nullptr && t0 + kPer <= p.rows;
+        if (four) {
             const int4 v = *reinterpret_cast<const int4*>(p.flag + t0);
             f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
         }
+        int count = 0;
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
-            const int t = t0 + j;
             col[j] = kNoCol;
-            if (p.target != nullptr || !four) f[j] = kNoLoss;
-            if (t < p.rows) {
+            if (!four) f[j] = kNoLoss;
+            if (!four && t0 + j < p.rows) {
                 if (p.target != nullptr) {
-                    const long long c = index_at(p.target, p.index_bytes, t);
+                    const long long c = index_at(p.target, p.index_bytes, t0 + j);
                     f[j] = c == p.ignore ? kNoLoss : (c >= 0 && c < p.vocab ? kLoss : kBad);
                     col[j] = f[j] == kLoss ? static_cast<int>(c) : kNoCol;
-                    if (!four) p.flag[t] = f[j];
-                } else if (!four) {
-                    f[j] = p.flag[t];
+                } else {
+                    f[j] = p.flag[t0 + j];
                 }
             }
             count += f[j] != kNoLoss;
         }
-        if (p.target != nullptr && four) *reinterpret_cast<int4*>(p.flag + t0) = make_int4(f[0], f[1], f[2], f[3]);
+        return count;
+    };
+    // What must be known of all rows first: whether one is left out, and the largest
+    // finite gradient (what is infinite or NaN stays in its own row).
+    bool copying = p.gather && p.copy_all;
+    const bool per_row = p.rgrad != nullptr && p.reduction == B200_VL_NONE;
+    const bool counting = p.gather && !copying && p.rows > kChunk;
+    float gmax = 0.0f;
+    if (per_row || counting) {
+        int left_out = 0;
+        for (int t0 = tid * kPer; t0 < p.rows; t0 += kChunk) {
+            int f[kPer], col[kPer];
+            left_out += classify(t0, f, col) != min(kPer, p.rows - t0);
+            if (per_row) {
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) {
+                    const float g = f[j] != kNoLoss ? fabsf(p.grad[t0 + j]) : 0.0f;
+                    if (isfinite(g)) gmax = fmaxf(gmax, g);
+                }
+            }
+        }
+        for (int o = 16; o; o >>= 1) gmax = fmaxf(gmax, __shfl_xor_sync(0xffffffffu, gmax, o));
+        if (lane == 0) warp_max[warp] = gmax;
+        left_out = __syncthreads_or(left_out);
+        if (counting) copying = left_out != 0;
+        for (int i = 0; i < 32; ++i) gmax = fmaxf(gmax, warp_max[i]);
+    }
+    // At most 1, so that G fits half precision whatever the loss is scaled by.
+    const float unit = gmax > 0.0f ? gmax : 1.0f;
+    if (tid == 0) base = 0;
+    __syncthreads();
+    for (int r0 = 0; r0 < p.rows; r0 += kChunk) {
+        const int t0 = r0 + tid * kPer;
+        const bool four = t0 + kPer <= p.rows;
+        const bool mine = t0 < p.rows && (t0 / kPer) % gridDim.x == blockIdx.x;
+        int f[kPer], col[kPer];
+        const int count = classify(t0, f, col);
         // Rows with a loss before this thread's first one: scan in the warp, then
         // over the warps.
         int upto = count;
@@ -1206,55 +1246,86 @@ __global__ void __launch_bounds__(1024) rows_kernel(const RowsParams p) {
             warp_sum[lane] = v;
         }
         __syncthreads();
+        if (p.gather && !copying && !counting) copying = warp_sum[31] != p.rows;
         int at = base + (warp ? warp_sum[warp - 1] : 0) + upto - count;
         const int at0 = p.gather ? at : t0;
-        const bool together = four && (at0 & 3) == 0 && (count == kPer || !p.gather);
         int inv[kPer];
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
-            const int t = t0 + j;
             const bool in = f[j] != kNoLoss;
-            const int i = p.gather ? at : t;
+            inv[j] = in ? (p.gather ? at : t0 + j) : -1;
             at += in;
-            inv[j] = in ? i : -1;
-            if (t >= p.rows) continue;
-            if (!four) p.inv[t] = inv[j];
-            if (p.gather && !in) continue;
-            if (!together) {
-                p.rowmap[i] = t;
-                if (p.target != nullptr) p.ecol[i] = col[j];
-            }
-            if (p.rgrad == nullptr) continue;
-            const float g = p.reduction == B200_VL_NONE ? p.grad[t] : 1.0f;
-            // p - 1 at the one target, without the difference of two numbers near 1.
-            const float below = p.target != nullptr ? expm1f(p.target_logp[t]) : 0.0f;
-            p.rgrad[i] = f[j] == kBad ? make_float4(NAN, NAN, NAN, 0.0f) : make_float4(g, -p.lse[t] * kLog2e, g * below, 0.0f);
-            // What is infinite or NaN from above stays in its own row.
-            if (isfinite(g)) gmax = fmaxf(gmax, fabsf(g));
         }
-        if (four) *reinterpret_cast<int4*>(p.inv + t0) = make_int4(inv[0], inv[1], inv[2], inv[3]);
-        if (together) {
-            *reinterpret_cast<int4*>(p.rowmap + at0) = make_int4(t0, t0 + 1, t0 + 2, t0 + 3);
-            if (p.target != nullptr) *reinterpret_cast<int4*>(p.ecol + at0) = make_int4(col[0], col[1], col[2], col[3]);
+        const int4 quad = make_int4(inv[0], inv[1], inv[2], inv[3]);
+        if (copying) numbers[tid] = quad;
+        if (mine) {
+            const bool together = four && (at0 & 3) == 0 && (count == kPer || !p.gather);
+            if (four) {
+                *reinterpret_cast<int4*>(p.inv + t0) = quad;
+                if (p.target != nullptr) *reinterpret_cast<int4*>(p.flag + t0) = make_int4(f[0], f[1], f[2], f[3]);
+            }
+            if (together) {
+                *reinterpret_cast<int4*>(p.rowmap + at0) = make_int4(t0, t0 + 1, t0 + 2, t0 + 3);
+                if (p.target != nullptr) *reinterpret_cast<int4*>(p.ecol + at0) = make_int4(col[0], col[1], col[2], col[3]);
+            }
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) {
+                const int t = t0 + j;
+                if (t >= p.rows) continue;
+                if (!four) {
+                    p.inv[t] = inv[j];
+                    if (p.target != nullptr) p.flag[t] = f[j];
+                }
+                const int i = p.gather ? inv[j] : t;
+                if (i < 0) continue;
+                if (!together) {
+                    p.rowmap[i] = t;
+                    if (p.target != nullptr) p.ecol[i] = col[j];
+                }
+                if (p.rgrad == nullptr) continue;
+                const float g = per_row ? p.grad[t] / unit : 1.0f;
+                // p - 1 at the one target, without the difference of two numbers near 1.
+                const float below = p.target != nullptr ? expm1f(p.target_logp[t]) : 0.0f;
+                p.rgrad[i] = f[j] == kBad ? make_float4(NAN, NAN, NAN, 0.0f)
+                                          : make_float4(g, -p.lse[t] * kLog2e, g * below, 0.0f);
+            }
         }
         __syncthreads();
+        if (copying) {
+            // A warp per row: of the block's groups of four in this chunk, the e-th row.
+            const int first = r0 / kPer;
+            const int own = first + (blockIdx.x + gridDim.x - first % gridDim.x) % gridDim.x;
+            for (int e = warp;; e += 32) {
+                const int quad_no = own + (e >> 2) * static_cast<int>(gridDim.x) - first;
+                const int t = r0 + quad_no * kPer + (e & 3);
+                if (quad_no >= 1024 || t >= p.rows) break;
+                const int i = reinterpret_cast<const int*>(numbers)[quad_no * kPer + (e & 3)];
+                if (i < 0) continue;
+                const uint4* src = p.hidden + t * p.ld;
+                uint4* dst = p.copy + i * p.ld_copy;
+                for (int v0 = lane; v0 < p.vecs; v0 += 32 * 8) {
+                    uint4 x[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (v0 + 32 * j < p.vecs) x[j] = __ldg(src + v0 + 32 * j);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (v0 + 32 * j < p.vecs) dst[v0 + 32 * j] = x[j];
+                }
+            }
+        }
         if (tid == 0) base += warp_sum[31];
         __syncthreads();
     }
     const int n_valid = base;
-    if (p.rgrad != nullptr && p.reduction == B200_VL_NONE) {
-        for (int o = 16; o; o >>= 1) gmax = fmaxf(gmax, __shfl_xor_sync(0xffffffffu, gmax, o));
-        if (lane == 0) warp_max[warp] = gmax;
-        __syncthreads();
-        for (int i = 0; i < 32; ++i) gmax = fmaxf(gmax, warp_max[i]);
-        // At most 1, so that G fits half precision whatever the loss is scaled by.
-        const float unit = gmax > 0.0f ? gmax : 1.0f;
-        for (int i = tid; i < n_valid; i += 1024) {
-            p.rgrad[i].x /= unit;
-            p.rgrad[i].z /= unit;
+    if (copying) {
+        const int end = min(p.rows, (max(n_valid, 1) + 255) / 256 * 256);
+        for (int i = n_valid + blockIdx.x * 32 + warp; i < end; i += gridDim.x * 32) {
+            uint4* dst = p.copy + i * p.ld_copy;
+            for (int v = lane; v < p.vecs; v += 32) dst[v] = make_uint4(0, 0, 0, 0);
         }
     }
-    if (tid == 0) {
+    if (blockIdx.x == 0 && tid == 0) {
         Head h;
         h.status = 0;
         for (int i = 0; i < 4; ++i) h.counter[i] = 0;
@@ -1262,29 +1333,13 @@ __global__ void __launch_bounds__(1024) rows_kernel(const RowsParams p) {
         h.ticket = 0;
         h.n_valid = n_valid;
         h.n_rows = p.gather ? n_valid : p.rows;
-        h.compact = h.n_rows != p.rows || p.copy_all;
+        h.compact = copying;
         h.alpha = 1.0f;
         if (p.rgrad != nullptr) {
-            if (p.reduction == B200_VL_NONE) h.alpha = gmax > 0.0f ? gmax * p.tau : p.tau;
+            if (per_row) h.alpha = unit * p.tau;
             else h.alpha = p.grad[0] * p.tau / (p.reduction == B200_VL_MEAN ? static_cast<float>(max(n_valid, 1)) : 1.0f);
         }
         *p.head = h;
-    }
-}
-
-// Gathers the rows that have a loss; a block of rows of zeros follows the last
-// one. Nothing to do where every row has one and starts on a 128-byte line.
-__global__ void __launch_bounds__(256) gather_kernel(const Head* head, const int* rowmap, const uint4* src,
-                                                     long long ld, uint4* dst, long long ld_dst, int rows, int vecs) {
-    griddep_wait();
-    griddep_launch_dependents();
-    if (!head->compact) return;
-    const int n = head->n_rows;
-    const int end = min(rows, (max(n, 1) + 255) / 256 * 256);
-    for (int i = blockIdx.x; i < end; i += gridDim.x) {
-        const uint4* s = i < n ? src + rowmap[i] * ld : nullptr;
-        uint4* d = dst + i * ld_dst;
-        for (int v = threadIdx.x; v < vecs; v += 256) d[v] = s != nullptr ? __ldg(s + v) : make_uint4(0, 0, 0, 0);
     }
 }
 
@@ -1508,8 +1563,8 @@ static int check_desc(const B200VocabLossDesc* d) {
         return B200_ERR_INVALID_ARGUMENT;
     }
     // Tile arithmetic is in 32 bits: leave room for a block behind the end.
-    if (d->rows > kMax - 1024 || d->vocab > kMax - 1024 || d->hidden > kMax - 1024) {
-        set_error("(rows,vocab,hidden)=(%lld,%lld,%lld): every extent must be below 2^31 - 1024",
+    if (d->rows > kMax - 8192 || d->vocab > kMax - 8192 || d->hidden > kMax - 8192) {
+        set_error("(rows,vocab,hidden)=(%lld,%lld,%lld): every extent must be below 2^31 - 8192",
                   (long long)d->rows, (long long)d->vocab, (long long)d->hidden);
         return B200_ERR_UNSUPPORTED;
     }
@@ -1793,7 +1848,7 @@ static int device_state(DeviceState* out) {
         cudaFuncAttributes loaded;
         for (const void* fn : {reinterpret_cast<const void*>(teacher_kernel<32>), reinterpret_cast<const void*>(teacher_kernel<128>),
                                reinterpret_cast<const void*>(rows_kernel),
-                               reinterpret_cast<const void*>(gather_kernel), reinterpret_cast<const void*>(merge_kernel),
+                               reinterpret_cast<const void*>(merge_kernel),
                                reinterpret_cast<const void*>(finish_kernel)})
             B200_CUDA_TRY(cudaFuncGetAttributes(&loaded, fn));
         cudaLaunchConfig_t cfg = {};
@@ -1945,13 +2000,13 @@ static int launch_rows(const Call& c, const void* index, const void* teacher, co
     r.target_logp = target_logp;
     r.rgrad = grad != nullptr ? c.at<float4>(l.rgrad) : nullptr;
     r.tau = static_cast<float>(d.temperature);
-    int rc = launch(rows_kernel, 1, 1024, 0, 1, d.top > 0, c.stream, r);
-    if (rc != B200_OK || !gather) return rc;
-    const int vecs = static_cast<int>(d.hidden / 8);
-    return launch(gather_kernel, static_cast<int>(std::min<int64_t>(d.rows, 8 * c.dev.sms)), 256, 0, 1, true, c.stream,
-                  static_cast<const Head*>(c.head()), static_cast<const int*>(c.at<int>(l.rowmap)),
-                  static_cast<const uint4*>(hidden), static_cast<long long>(d.ld_hidden / 8), c.at<uint4>(gathered),
-                  static_cast<long long>(l.ld_gathered / 8), static_cast<int>(d.rows), vecs);
+    r.hidden = static_cast<const uint4*>(hidden);
+    r.copy = c.at<uint4>(gathered);
+    r.ld = d.ld_hidden / 8;
+    r.ld_copy = l.ld_gathered / 8;
+    r.vecs = static_cast<int>(d.hidden / 8);
+    const int64_t blocks = gather ? std::min<int64_t>(ceil_div(d.rows, 8), c.dev.sms) : 1;
+    return launch(rows_kernel, static_cast<int>(blocks), 1024, 0, 1, d.top > 0, c.stream, r);
 }
 
 static Params base_params(const Call& c) {
@@ -2228,8 +2283,8 @@ int b200_vocab_loss_info(const B200VocabLossDesc* desc, int sm_count, B200VocabL
     out->workspace_forward = l.bytes_forward;
     out->workspace_backward = l.bytes_backward;
     const int64_t teacher = desc->top > 0 ? 1 : 0;
-    out->launches_forward = desc->rows == 0 ? 0 : 3 + teacher + (l.gather_forward ? 1 : 0);
-    out->launches_backward = desc->rows == 0 ? 0 : 3 + teacher + 3 * l.pieces;
+    out->launches_forward = desc->rows == 0 ? 0 : 3 + teacher;
+    out->launches_backward = desc->rows == 0 ? 0 : 2 + teacher + 3 * l.pieces;
     return B200_OK;
     B200_ABI_GUARD_END
 }

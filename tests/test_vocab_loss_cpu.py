@@ -164,7 +164,7 @@ def test_policy_invariants(sms):
         pad = -(-rows // 256) * 256
         assert 2 * rows * p["piece"] <= max(256 << 20, 2 * pad * hidden, 2 * pad * 256)
         assert p["workspace_forward"] % 256 == 0 and p["workspace_backward"] >= 2 * rows * (p["piece"] + hidden)
-        assert p["launches_backward"] == 3 + (top > 0) + 3 * p["pieces"]
+        assert p["launches_backward"] == 2 + (top > 0) + 3 * p["pieces"]
 
 
 def test_policy_of_known_sizes():

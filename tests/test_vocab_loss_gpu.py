@@ -66,6 +66,14 @@ def test_cross_entropy(rows, vocab, hidden, dtype):
     ce(rows, vocab, hidden, dtype)
 
 
+@pytest.mark.parametrize("rows,hidden,ignored,reduction", [(4097, 64, 1 / 4097, "mean"), (8192, 64, 0.0, "none"),
+                                                           (9001, 72, 0.4, "none"), (12291, 72, 0.0, "sum"),
+                                                           (4096, 136, 0.999, "none"), (9001, 64, 1.0, "mean")])
+def test_many_rows_left_out(rows, hidden, ignored, reduction):
+    """Rows beyond one step of their numbering (4096), one of them or nearly all left out."""
+    ce(rows, 300, hidden, BF16 if rows % 2 else FP16, reduction, ignored, seed=rows)
+
+
 @pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
 @pytest.mark.parametrize("ignored", [0.0, 0.3, 1.0])
 @pytest.mark.parametrize("rows", [1, 5, 100, 257, 700])
