@@ -5,8 +5,8 @@
 //
 // b200gemm::vocab_loss is the losses at the vocabulary projection
 // (b200_vocab_loss_forward / _backward) as one differentiable operator. A small
-// training step is bound by the host: 230 us as a Python autograd.Function,
-// of which 60 us on the GPU; see b200gemm/vocab_loss.py for its public form.
+// call is bound by the host: a training step took 230 us as a Python
+// autograd.Function, 87 as this one, 38 on the GPU; a loss alone takes 15; see b200gemm/vocab_loss.py for its public form.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -69,47 +69,60 @@ Problem unpack(const c10::IValue& v) {
 
 Tensor workspace(int64_t bytes, const Tensor& like) { return at::empty({bytes}, like.options().dtype(at::kByte)); }
 
+int64_t align_up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
+
+// The loss, and in `saved` what the backward pass reads again: per row the
+// logarithm of the sum of exponentials, then the log-probabilities at the targets.
+// Without a backward pass (null) they lie behind the workspace: an allocation is
+// 0.8 us of a small call's 16.
+Tensor forward_pass(Problem& p, const Tensor& hidden, const Tensor& weight, const Tensor& index,
+                    const std::optional<Tensor>& teacher, int64_t ignore_index, int64_t reduction, double temperature,
+                    Tensor* saved) {
+    const int64_t rows = hidden.size(0);
+    const bool per_row = reduction == B200_VL_NONE;
+    const auto f32 = hidden.options().dtype(at::kFloat);
+    if (rows == 0) return per_row ? at::empty({0}, f32) : at::zeros({}, f32);
+    B200VocabLossDesc& d = p.desc;
+    d.rows = rows;
+    d.vocab = weight.size(0);
+    d.hidden = weight.size(1);
+    d.ld_hidden = row_pitch(hidden, "hidden");
+    d.ld_weight = row_pitch(weight, "weight");
+    d.dtype = operand_code(hidden.scalar_type());
+    d.index_bytes = index.element_size();
+    d.ignore_index = ignore_index;
+    d.reduction = reduction;
+    d.temperature = temperature;
+    if (teacher) {
+        d.top = d.ld_index = d.ld_teacher = teacher->size(1);
+        d.teacher_dtype = teacher->scalar_type() == at::kFloat ? static_cast<int64_t>(B200_VL_F32)
+                                                               : operand_code(teacher->scalar_type());
+    }
+    const c10::cuda::CUDAGuard guard(hidden.device());
+    check_rc(g_api.info(&d, at::cuda::getCurrentDeviceProperties()->multiProcessorCount, &p.info),
+             "b200_vocab_loss_info");
+    const int64_t kept = rows * (1 + (teacher ? d.top : 1)), behind = align_up(p.info.workspace_forward, 256);
+    Tensor loss = per_row ? at::empty({rows}, f32) : at::empty({}, f32);
+    if (saved != nullptr) *saved = at::empty({kept}, f32);
+    Tensor ws = workspace(saved != nullptr ? p.info.workspace_forward : behind + kept * 4, hidden);
+    uint8_t* base = ws.mutable_data_ptr<uint8_t>();
+    float* lse = saved != nullptr ? saved->mutable_data_ptr<float>() : reinterpret_cast<float*>(base + behind);
+    check_rc(g_api.forward(&d, hidden.const_data_ptr(), weight.const_data_ptr(), index.const_data_ptr(),
+                           teacher ? teacher->const_data_ptr() : nullptr, loss.mutable_data_ptr<float>(), lse, lse + rows,
+                           base, p.info.workspace_forward, c10::cuda::getCurrentCUDAStream().stream()),
+             "b200_vocab_loss_forward");
+    return loss;
+}
+
 struct VocabLoss : public torch::autograd::Function<VocabLoss> {
     static Tensor forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& index,
                           const std::optional<Tensor>& teacher, int64_t ignore_index, int64_t reduction,
                           double temperature) {
-        const int64_t rows = hidden.size(0);
-        const bool per_row = reduction == B200_VL_NONE;
-        const auto f32 = hidden.options().dtype(at::kFloat);
-        ctx->saved_data["empty"] = rows == 0;
-        if (rows == 0) {
-            ctx->save_for_backward({hidden, weight});
-            return per_row ? at::empty({0}, f32) : at::zeros({}, f32);
-        }
         Problem p{};
-        B200VocabLossDesc& d = p.desc;
-        d.rows = rows;
-        d.vocab = weight.size(0);
-        d.hidden = weight.size(1);
-        d.ld_hidden = row_pitch(hidden, "hidden");
-        d.ld_weight = row_pitch(weight, "weight");
-        d.dtype = operand_code(hidden.scalar_type());
-        d.index_bytes = index.element_size();
-        d.ignore_index = ignore_index;
-        d.reduction = reduction;
-        d.temperature = temperature;
-        if (teacher) {
-            d.top = d.ld_index = d.ld_teacher = teacher->size(1);
-            d.teacher_dtype = teacher->scalar_type() == at::kFloat ? static_cast<int64_t>(B200_VL_F32)
-                                                                   : operand_code(teacher->scalar_type());
-        }
-        const c10::cuda::CUDAGuard guard(hidden.device());
-        check_rc(g_api.info(&d, at::cuda::getCurrentDeviceProperties()->multiProcessorCount, &p.info),
-                 "b200_vocab_loss_info");
-        Tensor loss = per_row ? at::empty({rows}, f32) : at::empty({}, f32);
-        Tensor lse = at::empty({rows}, f32), target_logp = at::empty({rows, teacher ? d.top : 1}, f32);
-        Tensor ws = workspace(p.info.workspace_forward, hidden);
-        check_rc(g_api.forward(&d, hidden.const_data_ptr(), weight.const_data_ptr(), index.const_data_ptr(),
-                               teacher ? teacher->const_data_ptr() : nullptr, loss.mutable_data_ptr<float>(),
-                               lse.mutable_data_ptr<float>(), target_logp.mutable_data_ptr<float>(), ws.mutable_data_ptr(), p.info.workspace_forward,
-                               c10::cuda::getCurrentCUDAStream().stream()),
-                 "b200_vocab_loss_forward");
-        ctx->save_for_backward({hidden, weight, index, teacher.value_or(Tensor()), lse, target_logp});
+        Tensor saved;
+        const Tensor loss =
+            forward_pass(p, hidden, weight, index, teacher, ignore_index, reduction, temperature, &saved);
+        ctx->save_for_backward({hidden, weight, index, teacher.value_or(Tensor()), saved});
         ctx->saved_data["problem"] = pack(p);
         return loss;
     }
@@ -121,13 +134,14 @@ struct VocabLoss : public torch::autograd::Function<VocabLoss> {
         const Tensor &hidden = saved[0], &weight = saved[1];
         const bool want_h = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
         Tensor dh, dw;
-        if (ctx->saved_data["empty"].toBool()) {
+        const Problem p = unpack(ctx->saved_data["problem"]);
+        if (p.desc.rows == 0) {
             if (want_h) dh = at::zeros(hidden.sizes(), hidden.options());
             if (want_w) dw = at::zeros(weight.sizes(), weight.options());
             return {dh, dw, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
         }
-        const Problem p = unpack(ctx->saved_data["problem"]);
-        const Tensor &index = saved[2], &teacher = saved[3], &lse = saved[4], &target_logp = saved[5];
+        const Tensor &index = saved[2], &teacher = saved[3];
+        const float* lse = saved[4].const_data_ptr<float>();
         const c10::cuda::CUDAGuard guard(hidden.device());
         const Tensor grad = grads[0].to(at::kFloat).contiguous();
         if (want_h) dh = at::empty(hidden.sizes(), hidden.options());
@@ -136,8 +150,7 @@ struct VocabLoss : public torch::autograd::Function<VocabLoss> {
             Tensor ws = workspace(p.info.workspace_backward, hidden);
             check_rc(g_api.backward(&p.desc, hidden.const_data_ptr(), weight.const_data_ptr(), index.const_data_ptr(),
                                     teacher.defined() ? teacher.const_data_ptr() : nullptr,
-                                    lse.const_data_ptr<float>(), target_logp.const_data_ptr<float>(),
-                                    grad.const_data_ptr<float>(),
+                                    lse, lse + p.desc.rows, grad.const_data_ptr<float>(),
                                     want_h ? dh.mutable_data_ptr() : nullptr, want_w ? dw.mutable_data_ptr() : nullptr,
                                     ws.mutable_data_ptr(), p.info.workspace_backward,
                                     c10::cuda::getCurrentCUDAStream().stream()),
@@ -193,15 +206,23 @@ Tensor vocab_loss(const Tensor& hidden, const Tensor& weight, const Tensor& inde
     for (const Tensor* t : {&h, &weight})
         TORCH_CHECK_VALUE(reinterpret_cast<uintptr_t>(t->const_data_ptr()) % 16 == 0, t == &h ? "hidden" : "weight",
                           " must start on a 16-byte boundary");
-    Tensor loss;
+    Tensor rows_index;
+    std::optional<Tensor> rows_teacher;
     if (teacher) {
         const int64_t k = teacher->size(-1);
-        loss = VocabLoss::apply(h, weight, index.reshape({-1, k}).contiguous(),
-                                std::optional<Tensor>(teacher->reshape({-1, k}).contiguous()), ignore_index, reduction,
-                                temperature);
+        rows_index = index.reshape({-1, k}).contiguous();
+        rows_teacher = teacher->reshape({-1, k}).contiguous();
     } else {
-        loss = VocabLoss::apply(h, weight, index.dim() == 1 ? index.contiguous() : index.reshape({-1}).contiguous(),
-                                std::optional<Tensor>(), ignore_index, reduction, temperature);
+        rows_index = (index.dim() == 1 ? index : index.reshape({-1})).contiguous();
+    }
+    Tensor loss;
+    // Forward mode has to go through autograd too, which refuses it.
+    const bool tangents = h._fw_grad(0).defined() || weight._fw_grad(0).defined();
+    if (tangents || (at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad()))) {
+        loss = VocabLoss::apply(h, weight, rows_index, rows_teacher, ignore_index, reduction, temperature);
+    } else {
+        Problem p{};
+        loss = forward_pass(p, h, weight, rows_index, rows_teacher, ignore_index, reduction, temperature, nullptr);
     }
     return reduction == B200_VL_NONE && hidden.dim() != 2 ? loss.reshape(lead) : loss;
 }

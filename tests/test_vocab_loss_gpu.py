@@ -317,6 +317,27 @@ def test_no_rows():
     assert loss.shape == (3, 0)
 
 
+def test_loss_alone_is_the_loss_of_a_step():
+    """Without a backward pass another path allocates; forward mode is refused."""
+    from b200gemm import vocab_loss
+    g, h, w = make(301, 700, 72)
+    t = torch.randint(0, 700, (301,), generator=g, device="cuda")
+    q = torch.randn(301, 5, generator=g, device="cuda")
+    idx = torch.randint(-1, 700, (301, 5), generator=g, device="cuda")
+    for fn, args in ((vocab_loss.linear_cross_entropy, (t,)), (vocab_loss.linear_distillation, (q, idx))):
+        for reduction in ("none", "mean", "sum"):
+            step = fn(h.detach().requires_grad_(), w, *args, reduction=reduction)
+            alone = fn(h, w, *args, reduction=reduction)
+            with torch.no_grad():
+                quiet = fn(h.detach().requires_grad_(), w, *args, reduction=reduction)
+            with torch.inference_mode():
+                inferred = fn(h, w, *args, reduction=reduction)
+            assert step.requires_grad and not alone.requires_grad and not quiet.requires_grad
+            assert torch.equal(step, alone) and torch.equal(step, quiet) and torch.equal(step, inferred)
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(lambda x: fn(x, w, *args), (h,), (h,))
+
+
 def test_two_streams_at_once():
     from b200gemm import vocab_loss
     jobs = []
