@@ -137,6 +137,29 @@ __device__ __forceinline__ int runs_for_warp(int tiles, int slots, int slices, i
     return __ffs(__ballot_sync(0xffffffffu, cost == least));
 }
 
+enum RowFlag { kNoLoss = 0, kLoss = 1, kBad = 2 };  // kBad: a target outside the vocabulary
+
+constexpr int kMergeWarps = 8;
+
+struct MergeParams {
+    Head* head;
+    const float2* part;
+    long long part_ld;
+    int tiles;            // half tiles
+    int warps_per_row;    // merge_kernel: 1 or kMergeWarps
+    int lanes;            // 0: merge_kernel follows; otherwise the product's last block merges, so many lanes a row
+    int rows, top, reduction;
+    const int* inv;
+    const int* flag;
+    const float* eq;
+    const float* zsel;
+    float c2, inv_tau, tau2;
+    float* lse;
+    float* target_logp;    // [rows][top]
+    float* row_loss;   // reduction none: the result
+    float* loss;
+};
+
 struct Params {
     Head* head;
     unsigned long long timeout_ns;
@@ -169,6 +192,7 @@ struct Params {
     const float4* rgrad;  // Grad: [gathered row] (g_t, -lse_t log2(e), g_t (p - 1) at the one target, 0)
     int top;
     float c2;             // log2(e) / tau
+    MergeParams merge;    // Stats
 };
 
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
@@ -251,6 +275,80 @@ __device__ __forceinline__ float finite_or_zero(float m) { return fabsf(m) == IN
 // A sum against -inf is empty: nothing, not 0 times the overflow of exp(0 - to).
 __device__ __forceinline__ float rescale(float from, float to, float c2) {
     return from == -INFINITY ? 0.0f : exp2_approx((finite_or_zero(from) - finite_or_zero(to)) * c2);
+}
+
+// Half tiles j0, j0 + step, ... of a row: the maximum first, then the sums against
+// it, eight at a time. What other blocks wrote is read from L2.
+__device__ __forceinline__ void merge_parts(const MergeParams& p, int i, int j0, int step, float& m, float& s) {
+    const float2* part = p.part + i * p.part_ld;
+    for (; j0 < p.tiles; j0 += 8 * step) {
+        float2 v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            v[j] = j0 + j * step < p.tiles ? __ldcg(part + j0 + j * step) : make_float2(-INFINITY, 0.0f);
+        float mx = m;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) mx = fmaxf(mx, v[j].x);
+        s *= rescale(m, mx, p.c2);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s += v[j].y * rescale(v[j].x, mx, p.c2);
+        m = mx;
+    }
+}
+
+// The same over groups of `lanes` lanes.
+__device__ __forceinline__ void merge_lanes(const MergeParams& p, int lanes, float& m, float& s) {
+    float mx = m;
+    for (int o = lanes / 2; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    s *= rescale(m, mx, p.c2);
+    for (int o = lanes / 2; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    m = mx;
+}
+
+// A row's results by a group of lanes from its flag, its gathered number and the
+// logit at its one target; `row` beyond the last: nothing to write.
+__device__ __forceinline__ void merge_row(const MergeParams& p, int row, int f, float z_one, int i, bool failed, float m,
+                                          float s, int lane, int lanes) {
+    // Log-probabilities at the targets as differences from the maximum: next to lse,
+    // which is rounded to its own size, those near 0 would be lost.
+    const float ref = finite_or_zero(m), logs = logf(s);
+    const bool there = row < p.rows;
+    if (there && lane == 0) p.lse[row] = i >= 0 ? logs + ref * p.inv_tau : 0.0f;
+    float v = 0.0f;
+    if (f == kLoss && p.eq == nullptr) {
+        v = logs - (z_one - ref);
+        if (lane == 0) p.target_logp[row] = -v;
+    } else if (f == kLoss) {
+        const long long e = static_cast<long long>(row) * p.top;
+        for (int k = lane; k < p.top; k += lanes) {
+            const float qv = p.eq[e + k];
+            const float logp = (__ldcg(p.zsel + e + k) - ref) * p.inv_tau - logs;
+            p.target_logp[e + k] = logp;
+            if (qv != 0.0f) v += qv * (logf(qv) - logp);
+        }
+    }
+    if (p.eq != nullptr) {
+        for (int o = lanes / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        v *= p.tau2;
+    }
+    // A target outside the vocabulary, or a launch that was given up, is no number.
+    if (f == kBad || failed) v = NAN;
+    if (there && lane == 0) p.row_loss[row] = v;
+}
+
+// The rows' sum by one block, in 64 bits: over many rows it keeps the rows' own precision.
+template <int kBlock>
+__device__ __forceinline__ void merge_sum(const MergeParams& p, double* sums) {
+    double sum = 0.0;
+    for (int r = threadIdx.x; r < p.rows; r += kBlock) sum += static_cast<double>(__ldcg(p.row_loss + r));
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (threadIdx.x % 32 == 0) sums[threadIdx.x / 32] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < kBlock / 32; ++w) sum += sums[w];
+        if (p.reduction == B200_VL_MEAN) sum /= max(p.head->n_valid, 1);
+        *p.loss = static_cast<float>(sum);
+    }
 }
 
 template <int kCtaGroup, int kTileN, int kOp, bool kHalf, int kSubM>
@@ -1009,18 +1107,44 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
     if constexpr (is_dw(kOp)) griddep_wait();
 
     // Teardown: every role is done with TMEM and with the peer's barriers.
+    if (is_stats(kOp) && p.merge.lanes != 0) __threadfence();
     tc_fence_before();
     if constexpr (kPair) cluster_sync(); else __syncthreads();
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc<kCtaGroup>(tmem_base, kTmemCols);
     }
+    if constexpr (is_stats(kOp)) {
+        // Little to merge: the block that finishes last does it.
+        const MergeParams& mp = p.merge;
+        if (mp.lanes == 0) return;
+        __shared__ double sums[kThreads / 32];
+        __shared__ int last;
+        if (threadIdx.x == 0) last = atomicAdd(&p.head->ticket, 1) == static_cast<int>(gridDim.x) - 1;
+        __syncthreads();
+        if (!last) return;
+        __threadfence();
+        const bool failed = __ldcg(&p.head->status) != 0;
+        const int sub = threadIdx.x & (mp.lanes - 1);
+        for (int r0 = 0; r0 < mp.rows; r0 += kThreads / mp.lanes) {
+            const int row = r0 + threadIdx.x / mp.lanes;
+            const int i = row < mp.rows ? mp.inv[row] : -1;
+            const int f = row < mp.rows ? mp.flag[row] : kNoLoss;
+            const float z_one = i >= 0 && mp.eq == nullptr ? __ldcg(mp.zsel + i) : 0.0f;
+            float m = -INFINITY, s = 0.0f;
+            if (i >= 0) merge_parts(mp, i, sub, mp.lanes, m, s);
+            merge_lanes(mp, mp.lanes, m, s);
+            merge_row(mp, row, f, z_one, i, failed, m, s, sub, mp.lanes);
+        }
+        if (mp.reduction == B200_VL_NONE) return;
+        __syncthreads();
+        merge_sum<kThreads>(mp, sums);
+    }
 }
 
 // ---------------------------------------------------------------------------
 // Rows, targets, teachers
 // ---------------------------------------------------------------------------
-enum RowFlag { kNoLoss = 0, kLoss = 1, kBad = 2 };  // kBad: a target outside the vocabulary
 
 __device__ __forceinline__ long long index_at(const void* idx, int bytes, long long i) {
     return bytes == 8 ? __ldg(static_cast<const long long*>(idx) + i)
@@ -1385,28 +1509,9 @@ __global__ void __launch_bounds__(1024) rows_kernel(const RowsParams p) {
     }
 }
 
-struct MergeParams {
-    Head* head;
-    const float2* part;
-    long long part_ld;
-    int tiles;            // half tiles
-    int warps_per_row;    // 1 or kMergeWarps
-    int rows, top, reduction;
-    const int* inv;
-    const int* flag;
-    const float* eq;
-    const float* zsel;
-    float c2, inv_tau, tau2;
-    float* lse;
-    float* target_logp;    // [rows][top]
-    float* row_loss;   // reduction none: the result
-    float* loss;
-};
-
 // A warp, or all eight of a block where there are few rows, merges a row's half
 // tiles in a fixed order and forms its loss; the last block to finish adds the
 // rows in order. Reads 8 bytes per (row, half tile).
-constexpr int kMergeWarps = 8;
 __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const MergeParams p) {
     __shared__ float sm[kMergeWarps], ss[kMergeWarps];
     __shared__ double sums[kMergeWarps];
@@ -1417,32 +1522,10 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const MergePara
     const int i = row < p.rows ? p.inv[row] : -1;
     const int f = row < p.rows ? p.flag[row] : kNoLoss;
     const bool failed = p.head->status != 0;
-    const float z_one = i >= 0 && p.eq == nullptr ? p.zsel[i] : 0.0f;
-    // The maximum first, then the sums against it: eight parts of a lane at a time,
-    // then the lanes, then the warps.
+    const float z_one = i >= 0 && p.eq == nullptr ? __ldcg(p.zsel + i) : 0.0f;
     float m = -INFINITY, s = 0.0f;
-    auto scale = [&](float from, float to) { return rescale(from, to, p.c2); };
-    if (i >= 0) {
-        const float2* part = p.part + i * p.part_ld;
-        const int step = 32 * p.warps_per_row;
-        for (int j0 = (warp % p.warps_per_row) * 32 + lane; j0 < p.tiles; j0 += 8 * step) {
-            float2 v[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = j0 + j * step < p.tiles ? part[j0 + j * step] : make_float2(-INFINITY, 0.0f);
-            float mx = m;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) mx = fmaxf(mx, v[j].x);
-            s *= scale(m, mx);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) s += v[j].y * scale(v[j].x, mx);
-            m = mx;
-        }
-    }
-    float mx = m;
-    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    s *= scale(m, mx);
-    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    m = mx;
+    if (i >= 0) merge_parts(p, i, (warp % p.warps_per_row) * 32 + lane, 32 * p.warps_per_row, m, s);
+    merge_lanes(p, 32, m, s);
     if (p.warps_per_row > 1) {
         if (lane == 0) {
             sm[warp] = m;
@@ -1451,33 +1534,10 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const MergePara
         __syncthreads();
         for (int w = 0; w < kMergeWarps; ++w) m = fmaxf(m, sm[w]);
         s = 0.0f;
-        for (int w = 0; w < kMergeWarps; ++w) s += ss[w] * scale(sm[w], m);
+        for (int w = 0; w < kMergeWarps; ++w) s += ss[w] * rescale(sm[w], m, p.c2);
     }
-    // Log-probabilities at the targets as differences from the maximum: next to lse,
-    // which is rounded to its own size, those near 0 would be lost.
-    const float ref = finite_or_zero(m), logs = logf(s);
     const bool leader = row < p.rows && warp % p.warps_per_row == 0;
-    if (leader && lane == 0) p.lse[row] = i >= 0 ? logs + ref * p.inv_tau : 0.0f;
-    if (leader) {
-        float v = 0.0f;
-        if (f == kLoss && p.eq == nullptr) {
-            v = logs - (z_one - ref);
-            if (lane == 0) p.target_logp[row] = -v;
-        } else if (f == kLoss) {
-            const long long e = static_cast<long long>(row) * p.top;
-            for (int k = lane; k < p.top; k += 32) {
-                const float qv = p.eq[e + k];
-                const float logp = (p.zsel[e + k] - ref) * p.inv_tau - logs;
-                p.target_logp[e + k] = logp;
-                if (qv != 0.0f) v += qv * (logf(qv) - logp);
-            }
-            for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-            v *= p.tau2;
-        }
-        // A target outside the vocabulary, or a launch that was given up, is no number.
-        if (f == kBad || failed) v = NAN;
-        if (lane == 0) p.row_loss[row] = v;
-    }
+    merge_row(p, leader ? row : p.rows, leader ? f : kNoLoss, z_one, i, failed, m, s, lane, 32);
     if (p.reduction == B200_VL_NONE) return;
     __threadfence();
     __syncthreads();
@@ -1485,17 +1545,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const MergePara
     __syncthreads();
     if (!last) return;
     __threadfence();
-    // In 64 bits: the sum over many rows keeps the rows' own precision.
-    double sum = 0.0;
-    for (int r = threadIdx.x; r < p.rows; r += 32 * kMergeWarps) sum += static_cast<double>(__ldcg(p.row_loss + r));
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) sums[warp] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < kMergeWarps; ++w) sum += sums[w];
-        if (p.reduction == B200_VL_MEAN) sum /= max(p.head->n_valid, 1);
-        *p.loss = static_cast<float>(sum);
-    }
+    merge_sum<32 * kMergeWarps>(p, sums);
 }
 
 struct FinishParams {
@@ -1573,6 +1623,11 @@ static int64_t align_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
 // Room for G: this, or as much as H itself takes (one 256-column block at least).
 constexpr int64_t kPieceBytes = int64_t(256) << 20;
 constexpr int64_t kPartialBytes = int64_t(256) << 20;
+// What the last block of the product merges in the time of a launch: rows x (half
+// tiles or targets), and those of one row. (26 rows over 718 columns 15.7 -> 13.0 us,
+// 8 over 32000 17.2 -> 16.0, 512 over 512 16.5 -> 15.9; beyond: 64 over 32000 16.4 ->
+// 22.4, one over 128256 181 -> 184.)
+constexpr int64_t kMergeHere = 4096, kMergeRowHere = 512;
 // A piece of G that is still in L2 (126 MB) when the second product reads it.
 constexpr int64_t kL2Piece = int64_t(48) << 20;
 
@@ -1591,6 +1646,7 @@ struct Layout {
     int64_t ld_gathered, ld_part;                        // row pitches on 128-byte lines
     int64_t bytes_forward, bytes_backward;
     bool gather_forward;
+    int merge_lanes;      // of MergeParams
 };
 
 static int check_desc(const B200VocabLossDesc* d) {
@@ -1708,6 +1764,10 @@ static Layout layout_for(const B200VocabLossDesc& d, int64_t sms) {
     l.ld_part = align_up(D, 32);
     // The forward pass gathers only to save products (its rows do not meet): not
     // where all tiles run at once anyway (2.5 us of a 17 us call).
+    const int64_t parts = ceil_div(V, l.tile_n / 2), longest = std::max(parts, d.top);
+    l.merge_lanes = 0;
+    if (T * longest <= kMergeHere && longest <= kMergeRowHere)
+        for (l.merge_lanes = 1; l.merge_lanes < 32 && 8 * l.merge_lanes < longest;) l.merge_lanes *= 2;
     l.gather_forward = ceil_div(T, l.tile_m) * ceil_div(V, l.tile_n) > sms / l.cta_group && T > l.tile_m;
     // Piece of the vocabulary (in blocks of 256) and runs of the contractions of dH
     // and dW: the least k-slices on the longest cluster, over the three products of
@@ -2153,9 +2213,6 @@ static int forward(const B200VocabLossDesc* d, const void* hidden, const void* w
     p.early = !l.gather_forward;
     p.part_ld = ceil_div(d->vocab, l.tile_n / 2);
     p.a_bytes = box_m * kBK * 2;
-    rc = launch_gemm(c, d->hidden <= kDrainMost * kBK ? kStatsShort : kStats, l.cta_group, l.tile_n, 1,
-                     ceil_div(d->rows, l.tile_m) * ceil_div(d->vocab, l.tile_n), a0, a1, b, b, b, p);
-    if (rc != B200_OK) return rc;
     MergeParams m{};
     m.head = c.head();
     m.part = p.part;
@@ -2163,6 +2220,7 @@ static int forward(const B200VocabLossDesc* d, const void* hidden, const void* w
     m.tiles = static_cast<int>(p.part_ld);
     // A block for each row up to eight blocks per SM.
     m.warps_per_row = d->rows <= 8 * c.dev.sms ? kMergeWarps : 1;
+    m.lanes = l.merge_lanes;
     m.rows = static_cast<int>(d->rows);
     m.top = p.top;
     m.reduction = static_cast<int>(d->reduction);
@@ -2177,6 +2235,10 @@ static int forward(const B200VocabLossDesc* d, const void* hidden, const void* w
     m.target_logp = target_logp;
     m.row_loss = d->reduction == B200_VL_NONE ? loss : c.at<float>(l.row_loss);
     m.loss = loss;
+    p.merge = m;
+    rc = launch_gemm(c, d->hidden <= kDrainMost * kBK ? kStatsShort : kStats, l.cta_group, l.tile_n, 1,
+                     ceil_div(d->rows, l.tile_m) * ceil_div(d->vocab, l.tile_n), a0, a1, b, b, b, p);
+    if (rc != B200_OK || m.lanes != 0) return rc;
     return launch(merge_kernel, static_cast<int>(ceil_div(d->rows, kMergeWarps / m.warps_per_row)), 32 * kMergeWarps, 0, 1,
                   true, c.stream, m);
 }
@@ -2325,7 +2387,7 @@ int b200_vocab_loss_info(const B200VocabLossDesc* desc, int sm_count, B200VocabL
     out->workspace_forward = l.bytes_forward;
     out->workspace_backward = l.bytes_backward;
     const int64_t teacher = desc->top > 0 ? 1 : 0;
-    out->launches_forward = desc->rows == 0 ? 0 : 3 + teacher;
+    out->launches_forward = desc->rows == 0 ? 0 : 2 + teacher + (l.merge_lanes == 0 ? 1 : 0);
     out->launches_backward = desc->rows == 0 ? 0 : 2 + teacher + 3 * l.pieces;
     return B200_OK;
     B200_ABI_GUARD_END

@@ -173,6 +173,10 @@ def test_policy_of_known_sizes():
     p = vocab_loss.policy(1, 128256, 4096)  # one token: the weight is read in narrow tiles, H not gathered
     assert (p["cta_group"], p["tile_n"], p["pieces"], p["launches_forward"]) == (1, 128, 1, 3)
     assert vocab_loss.policy(8192, 256, 512)["splits_weight"] > 1
+    # A small call's rows are merged by the product's last block.
+    assert vocab_loss.policy(26, 718, 120)["launches_forward"] == 2
+    assert vocab_loss.policy(64, 1000, 256, top=8)["launches_forward"] == 3
+    assert vocab_loss.policy(64, 32000, 256)["launches_forward"] == 3
     assert vocab_loss.policy(0, 10, 8)["launches_forward"] == 0
     with pytest.raises(ValueError):
         vocab_loss.policy(1, 1, 8, dtype=torch.float32)

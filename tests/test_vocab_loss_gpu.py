@@ -74,6 +74,18 @@ def test_many_rows_left_out(rows, hidden, ignored, reduction):
     ce(rows, 300, hidden, BF16 if rows % 2 else FP16, reduction, ignored, seed=rows)
 
 
+@pytest.mark.parametrize("rows,vocab,top", [(1, 512 * 64, 0), (1, 512 * 64 + 1, 0), (8, 32000, 0), (26, 718, 0),
+                                            (512, 500, 0), (513, 500, 0), (33, 5000, 0), (4000, 60, 0), (4097, 60, 0),
+                                            (16, 300, 256), (17, 300, 256), (320, 400, 12), (70, 3000, 3)])
+@pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
+def test_merged_by_the_last_block(rows, vocab, top, reduction):
+    """Both sides of the rule, and every number of lanes per row."""
+    if top:
+        kd(rows, vocab, 72, top, reduction=reduction)
+    else:
+        ce(rows, vocab, 72, FP16, reduction, 0.2, seed=rows)
+
+
 @pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
 @pytest.mark.parametrize("ignored", [0.0, 0.3, 1.0])
 @pytest.mark.parametrize("rows", [1, 5, 100, 257, 700])
