@@ -83,7 +83,7 @@ struct Head {
     int g_piece;      // the last piece whose G is known to be complete, from 1
     int ticket;       // finished blocks of the merge kernel
     int n_rows;       // rows that the products run over
-    int n_valid;      // rows with a loss
+    int n_valid;      // rows with a loss, if the rows' kernel ran
     int compact;      // 1: the rows are those of the gathered copy of H
     float alpha;      // factor common to all rows of G, applied after the products
 };
@@ -149,6 +149,7 @@ struct MergeParams {
     int warps_per_row;    // merge_kernel: 1 or kMergeWarps
     int lanes;            // 0: merge_kernel follows; otherwise the product's last block merges, so many lanes a row
     int rows, top, reduction;
+    int count;            // 1: nobody has counted the rows with a loss
     const int* inv;
     const int* flag;
     const float* eq;
@@ -336,17 +337,29 @@ __device__ __forceinline__ void merge_row(const MergeParams& p, int row, int f, 
     if (there && lane == 0) p.row_loss[row] = v;
 }
 
-// The rows' sum by one block, in 64 bits: over many rows it keeps the rows' own precision.
+// The rows' sum, and their mean over those with a loss, by one block; in 64 bits,
+// which over many rows keeps the rows' own precision.
 template <int kBlock>
-__device__ __forceinline__ void merge_sum(const MergeParams& p, double* sums) {
+__device__ __forceinline__ void merge_sum(const MergeParams& p, double (&sums)[kBlock / 32], int (&counts)[kBlock / 32]) {
     double sum = 0.0;
     for (int r = threadIdx.x; r < p.rows; r += kBlock) sum += static_cast<double>(__ldcg(p.row_loss + r));
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (threadIdx.x % 32 == 0) sums[threadIdx.x / 32] = sum;
+    int n = 0;
+    if (p.count) {
+        for (int r = threadIdx.x; r < p.rows; r += kBlock) n += p.flag[r] != kNoLoss;
+        n = __reduce_add_sync(0xffffffffu, n);
+    }
+    if (threadIdx.x % 32 == 0) {
+        sums[threadIdx.x / 32] = sum;
+        counts[threadIdx.x / 32] = n;
+    }
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int w = 1; w < kBlock / 32; ++w) sum += sums[w];
-        if (p.reduction == B200_VL_MEAN) sum /= max(p.head->n_valid, 1);
+        for (int w = 1; w < kBlock / 32; ++w) {
+            sum += sums[w];
+            n += counts[w];
+        }
+        if (p.reduction == B200_VL_MEAN) sum /= max(p.count ? n : p.head->n_valid, 1);
         *p.loss = static_cast<float>(sum);
     }
 }
@@ -1119,6 +1132,7 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
         const MergeParams& mp = p.merge;
         if (mp.lanes == 0) return;
         __shared__ double sums[kThreads / 32];
+        __shared__ int counts[kThreads / 32];
         __shared__ int last;
         if (threadIdx.x == 0) last = atomicAdd(&p.head->ticket, 1) == static_cast<int>(gridDim.x) - 1;
         __syncthreads();
@@ -1138,7 +1152,7 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
         }
         if (mp.reduction == B200_VL_NONE) return;
         __syncthreads();
-        merge_sum<kThreads>(mp, sums);
+        merge_sum<kThreads>(mp, sums, counts);
     }
 }
 
@@ -1171,6 +1185,10 @@ struct TeacherParams {
     float* eq;
     unsigned short* epos;
     int* flag;
+    // Where the products run over all rows in their order: nothing is left to number.
+    Head* head;           // or null: the rows' kernel follows
+    int* rowmap;
+    int* inv;
 };
 
 // A block turns one row of a teacher's logits into its target distribution:
@@ -1277,7 +1295,19 @@ __global__ void __launch_bounds__(kTeacherThreads) teacher_kernel(const TeacherP
         ecol[i] = kNoCol;
         eq[i] = 0.0f;
     }
-    if (tid == 0) p.flag[t] = bad ? kBad : (any ? kLoss : kNoLoss);
+    if (tid == 0) {
+        p.flag[t] = bad ? kBad : (any ? kLoss : kNoLoss);
+        if (p.head != nullptr) {
+            p.rowmap[t] = t;
+            p.inv[t] = bad || any ? t : -1;
+            if (t == 0) {
+                Head h = {};
+                h.n_rows = p.rows;
+                h.alpha = 1.0f;
+                *p.head = h;
+            }
+        }
+    }
     unsigned short* epos = p.epos + t * p.epos_ld;
     for (long long j = tid; j < p.epos_ld; j += kTeacherThreads) {
         const long long col = j * p.half;
@@ -1515,6 +1545,7 @@ __global__ void __launch_bounds__(1024) rows_kernel(const RowsParams p) {
 __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const MergeParams p) {
     __shared__ float sm[kMergeWarps], ss[kMergeWarps];
     __shared__ double sums[kMergeWarps];
+    __shared__ int counts[kMergeWarps];
     __shared__ int last;
     griddep_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -1545,7 +1576,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const MergePara
     __syncthreads();
     if (!last) return;
     __threadfence();
-    merge_sum<32 * kMergeWarps>(p, sums);
+    merge_sum<32 * kMergeWarps>(p, sums, counts);
 }
 
 struct FinishParams {
@@ -2074,12 +2105,17 @@ static int launch_rows(const Call& c, const void* index, const void* teacher, co
         t.ecol = c.at<int>(l.ecol);
         t.eq = c.at<float>(l.eq);
         t.flag = c.at<int>(l.flag);
+        if (!gather) {
+            t.head = c.head();
+            t.rowmap = c.at<int>(l.rowmap);
+            t.inv = c.at<int>(l.inv);
+        }
         int pad = 2;
         while (pad < t.top) pad *= 2;
         const int rc = pad <= 32 && d.rows > 8 * c.dev.sms
                            ? launch(teacher_kernel<32>, static_cast<int>(d.rows), 32, 0, 1, false, c.stream, t, pad)
                            : launch(teacher_kernel<128>, static_cast<int>(d.rows), 128, 0, 1, false, c.stream, t, pad);
-        if (rc != B200_OK) return rc;
+        if (rc != B200_OK || !gather) return rc;
     }
     RowsParams r{};
     r.head = c.head();
@@ -2224,6 +2260,7 @@ static int forward(const B200VocabLossDesc* d, const void* hidden, const void* w
     m.rows = static_cast<int>(d->rows);
     m.top = p.top;
     m.reduction = static_cast<int>(d->reduction);
+    m.count = d->reduction == B200_VL_MEAN && d->top > 0 && !l.gather_forward;
     m.inv = c.at<int>(l.inv);
     m.flag = c.at<int>(l.flag);
     m.eq = p.eq;
@@ -2387,7 +2424,7 @@ int b200_vocab_loss_info(const B200VocabLossDesc* desc, int sm_count, B200VocabL
     out->workspace_forward = l.bytes_forward;
     out->workspace_backward = l.bytes_backward;
     const int64_t teacher = desc->top > 0 ? 1 : 0;
-    out->launches_forward = desc->rows == 0 ? 0 : 2 + teacher + (l.merge_lanes == 0 ? 1 : 0);
+    out->launches_forward = desc->rows == 0 ? 0 : 2 + (l.gather_forward ? teacher : 0) + (l.merge_lanes == 0 ? 1 : 0);
     out->launches_backward = desc->rows == 0 ? 0 : 2 + teacher + 3 * l.pieces;
     return B200_OK;
     B200_ABI_GUARD_END

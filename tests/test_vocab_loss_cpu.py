@@ -175,7 +175,9 @@ def test_policy_of_known_sizes():
     assert vocab_loss.policy(8192, 256, 512)["splits_weight"] > 1
     # A small call's rows are merged by the product's last block.
     assert vocab_loss.policy(26, 718, 120)["launches_forward"] == 2
-    assert vocab_loss.policy(64, 1000, 256, top=8)["launches_forward"] == 3
+    assert vocab_loss.policy(64, 1000, 256, top=8)["launches_forward"] == 2
+    assert vocab_loss.policy(64, 32000, 256, top=8)["launches_forward"] == 3
+    assert vocab_loss.policy(2048, 32000, 256, top=8)["launches_forward"] == 4
     assert vocab_loss.policy(64, 32000, 256)["launches_forward"] == 3
     assert vocab_loss.policy(0, 10, 8)["launches_forward"] == 0
     with pytest.raises(ValueError):
