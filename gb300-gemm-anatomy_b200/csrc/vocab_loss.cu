@@ -1539,7 +1539,7 @@ __global__ void __launch_bounds__(1024) rows_kernel(const RowsParams p) {
     }
 }
 
-// A warp, or all eight of a block where there are few rows, merges a row's half
+// A warp, or all eight of a block where there are few long rows, merges a row's half
 // tiles in a fixed order and forms its loss; the last block to finish adds the
 // rows in order. Reads 8 bytes per (row, half tile).
 __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const MergeParams p) {
@@ -2254,8 +2254,9 @@ static int forward(const B200VocabLossDesc* d, const void* hidden, const void* w
     m.part = p.part;
     m.part_ld = p.part_ld;
     m.tiles = static_cast<int>(p.part_ld);
-    // A block for each row up to eight blocks per SM.
-    m.warps_per_row = d->rows <= 8 * c.dev.sms ? kMergeWarps : 1;
+    // A block for each row pays where there are few rows of many half tiles (one row of
+    // 2004: 21.0 against 21.9 us; 1000 of 235 33.1 and 37.4, 1021 of 391 41.4 and 45.0).
+    m.warps_per_row = d->rows <= c.dev.sms && m.tiles > 512 ? kMergeWarps : 1;
     m.lanes = l.merge_lanes;
     m.rows = static_cast<int>(d->rows);
     m.top = p.top;
