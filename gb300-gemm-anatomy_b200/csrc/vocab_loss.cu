@@ -14,7 +14,8 @@
 // tiles of z in TMEM; its epilogue keeps, for every row and tile, the running
 // maximum m and s = sum exp((z - m) / tau) and copies out the logits at the
 // row's targets. 8 bytes per (row, tile) leave the SM instead of 1024. A small
-// kernel merges the tiles in order and forms the loss.
+// kernel, in a small call the last block of the product, merges the tiles in order
+// and forms the loss.
 //
 // Backward: the vocabulary is walked in pieces. For each piece, the logits are
 // recomputed and turned into G = g_t (p - q) in 16 bits (T x piece), then
@@ -65,7 +66,7 @@ constexpr int kDrain = kCtaGroup == 1 ? 4 : kDrainMost;
 constexpr int kQueue = 4;
 constexpr int kNoCol = INT_MAX;
 constexpr int kMaxTop = 256;      // teacher logits per row
-constexpr int kMaxSplits = 16;    // runs of the contraction of dH
+constexpr int kMaxSplits = 16;    // runs of the contraction of dH or dW
 constexpr float kLog2e = 1.4426950408889634f;
 
 // The products. Operands: Stats, Grad: A = H, B = W (both K-major); Dh: A = G
@@ -453,8 +454,9 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
     if constexpr (is_dw(kOp)) {
         // dW needs G and not the product before it, which is dH: it fills the SMs that
         // dH leaves, and waits for dH's end at its own (512^3 step as a graph: 43.1 ->
-        // 39.0 us; 8192 x 128256 x 4096: 25.15-25.33 -> 24.99 ms). dH is launched first, waits for G and says so; without its word, dW
-        // waits for all that came before.
+        // 39.0 us; 8192 x 128256 x 4096: 25.15-25.33 -> 24.99 ms). dH is launched
+        // first, waits for G and says so; without its word, dW waits for all that came
+        // before.
         if (ld_acquire_gpu(&p.head->g_piece) != p.piece_no) griddep_wait();
         fence_proxy_async();
     } else if (!early) {
