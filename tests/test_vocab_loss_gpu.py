@@ -350,6 +350,45 @@ def test_loss_alone_is_the_loss_of_a_step():
             torch.func.jvp(lambda x: fn(x, w, *args), (h,), (h,))
 
 
+@pytest.mark.parametrize("rows,vocab,hidden,top", [(512, 512, 512, 0), (130, 5000, 72, 0), (4096, 40007, 64, 0),
+                                                   (700, 3000, 1000, 9), (8, 700, 64, 3)])
+def test_overlapping_kernels_give_the_same_bits(rows, vocab, hidden, top):
+    """Steps close behind one another, eager and as a graph that is replayed: the kernels of a step
+    start while others end, on a workspace that the step before has used."""
+    from b200gemm import vocab_loss
+    g, h, w = make(rows, vocab, hidden)
+    up = torch.rand(rows, generator=g, device="cuda")
+    if top:
+        fn = vocab_loss.linear_distillation
+        args = (torch.randn(rows, top, generator=g, device="cuda"),
+                torch.randint(-1, vocab, (rows, top), generator=g, device="cuda"))
+    else:
+        fn = vocab_loss.linear_cross_entropy
+        args = (torch.randint(0, vocab, (rows,), generator=g, device="cuda"),)
+        args[0][::5] = IGNORE
+    first = run(fn, h, w, args, up, reduction="none")
+    torch.cuda.synchronize()
+    differ = torch.zeros((), dtype=torch.bool, device="cuda")
+    for _ in range(30):
+        for x, y in zip(run(fn, h, w, args, up, reduction="none"), first):
+            differ |= (x != y).any()
+    assert not differ
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        run(fn, h, w, args, up, reduction="none")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        out = run(fn, h, w, args, up, reduction="none")
+    for _ in range(30):
+        graph.replay()
+        graph.replay()
+        for x, y in zip(out, first):
+            differ |= (x != y).any()
+    assert not differ
+
+
 def test_two_streams_at_once():
     from b200gemm import vocab_loss
     jobs = []
