@@ -12,6 +12,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <cstring>
 #include <optional>
 
@@ -43,12 +44,30 @@ void check_rc(int rc, const char* what) {
 }
 
 // Rows of the operand: contiguous inside, a multiple of 16 bytes apart.
+bool rows_fit(const Tensor& t) { return t.size(0) <= 1 || (t.stride(0) >= t.size(1) && t.stride(0) % 8 == 0); }
+bool starts_on_unit(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0; }
 int64_t row_pitch(const Tensor& t, const char* name) {
-    const int64_t rows = t.size(0), d = t.size(1);
-    if (rows <= 1) return d;
-    TORCH_CHECK_VALUE(t.stride(0) >= d && t.stride(0) % 8 == 0, name,
-                      " rows must be a multiple of 8 elements apart and not overlap, strides ", t.strides());
-    return t.stride(0);
+    TORCH_CHECK_VALUE(rows_fit(t), name, " rows must be a multiple of 8 elements apart and not overlap, strides ",
+                      t.strides());
+    return t.size(0) <= 1 ? t.size(1) : t.stride(0);
+}
+
+// A tensor that the backward pass reads again. Saved-tensor hooks
+// (torch.autograd.graph.save_on_cpu, a checkpoint) may give back the same values in
+// another layout: the kernels go by the layout that is there now.
+void check_saved(const Tensor& t, const char* name, at::IntArrayRef sizes, at::ScalarType type, at::Device device) {
+    TORCH_CHECK(t.defined() && t.sizes() == sizes && t.scalar_type() == type && t.device() == device, name,
+                " came back to the backward pass as another tensor than was saved: expected ", sizes, " ", type, " on ",
+                device);
+}
+Tensor as_saved(const Tensor& t, const char* name, at::IntArrayRef sizes, at::ScalarType type, at::Device device) {
+    check_saved(t, name, sizes, type, device);
+    return t.contiguous();
+}
+// The same for an operand, which may keep a pitch that the kernels can take.
+Tensor as_saved_operand(const Tensor& t, const char* name, at::IntArrayRef sizes, at::ScalarType type, at::Device device) {
+    check_saved(t, name, sizes, type, device);
+    return t.stride(1) == 1 && rows_fit(t) && starts_on_unit(t) ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
 int64_t operand_code(at::ScalarType t) { return t == at::kHalf ? B200_VL_F16 : B200_VL_BF16; }
@@ -58,8 +77,10 @@ struct Problem {
     B200VocabLossInfo info;
 };
 
-// The description travels from the forward to the backward pass in saved_data,
-// as bytes: the sizes and pitches are those that the forward pass checked.
+// The description travels from the forward to the backward pass in saved_data, as
+// bytes. Its sizes hold there; its pitches are those of the tensors that the forward
+// pass was given, and the backward pass takes its own from what comes back (see
+// as_saved).
 c10::IValue pack(const Problem& p) { return std::string(reinterpret_cast<const char*>(&p), sizeof(p)); }
 Problem unpack(const c10::IValue& v) {
     Problem p;
@@ -131,18 +152,37 @@ struct VocabLoss : public torch::autograd::Function<VocabLoss> {
         TORCH_CHECK(!at::GradMode::is_enabled(),
                     "the losses at the vocabulary projection are differentiable once (create_graph=True)");
         const variable_list saved = ctx->get_saved_variables();
-        const Tensor &hidden = saved[0], &weight = saved[1];
         const bool want_h = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
         Tensor dh, dw;
-        const Problem p = unpack(ctx->saved_data["problem"]);
+        Problem p = unpack(ctx->saved_data["problem"]);
         if (p.desc.rows == 0) {
+            const Tensor &hidden = saved[0], &weight = saved[1];
             if (want_h) dh = at::zeros(hidden.sizes(), hidden.options());
             if (want_w) dw = at::zeros(weight.sizes(), weight.options());
             return {dh, dw, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
         }
-        const Tensor &index = saved[2], &teacher = saved[3];
-        const float* lse = saved[4].const_data_ptr<float>();
-        const c10::cuda::CUDAGuard guard(hidden.device());
+        B200VocabLossDesc& d = p.desc;
+        const at::Device device = grads[0].device();
+        const c10::cuda::CUDAGuard guard(device);
+        const at::ScalarType type = d.dtype == B200_VL_F16 ? at::kHalf : at::kBFloat16;
+        const Tensor hidden = as_saved_operand(saved[0], "hidden", {d.rows, d.hidden}, type, device);
+        const Tensor weight = as_saved_operand(saved[1], "weight", {d.vocab, d.hidden}, type, device);
+        d.ld_hidden = row_pitch(hidden, "hidden");
+        d.ld_weight = row_pitch(weight, "weight");
+        const at::ScalarType index_type = d.index_bytes == 8 ? at::kLong : at::kInt;
+        Tensor index, teacher;
+        if (d.top > 0) {
+            const at::ScalarType teacher_type = d.teacher_dtype == B200_VL_F32   ? at::kFloat
+                                                : d.teacher_dtype == B200_VL_F16 ? at::kHalf
+                                                                                 : at::kBFloat16;
+            index = as_saved(saved[2], "teacher_index", {d.rows, d.top}, index_type, device);
+            teacher = as_saved(saved[3], "teacher_logits", {d.rows, d.top}, teacher_type, device);
+        } else {
+            index = as_saved(saved[2], "target", {d.rows}, index_type, device);
+        }
+        const Tensor kept = as_saved(saved[4], "a result of the forward pass", {d.rows * (1 + std::max<int64_t>(d.top, 1))},
+                                     at::kFloat, device);
+        const float* lse = kept.const_data_ptr<float>();
         const Tensor grad = grads[0].to(at::kFloat).contiguous();
         if (want_h) dh = at::empty(hidden.sizes(), hidden.options());
         if (want_w) dw = at::empty(weight.sizes(), weight.options());
@@ -204,7 +244,7 @@ Tensor vocab_loss(const Tensor& hidden, const Tensor& weight, const Tensor& inde
                       " like hidden, got ", teacher ? teacher->device() : hidden.device());
     const Tensor h = hidden.dim() == 2 ? hidden : hidden.reshape({-1, d});
     for (const Tensor* t : {&h, &weight})
-        TORCH_CHECK_VALUE(reinterpret_cast<uintptr_t>(t->const_data_ptr()) % 16 == 0, t == &h ? "hidden" : "weight",
+        TORCH_CHECK_VALUE(starts_on_unit(*t), t == &h ? "hidden" : "weight",
                           " must start on a 16-byte boundary");
     Tensor rows_index;
     std::optional<Tensor> rows_teacher;
