@@ -68,6 +68,9 @@ constexpr int kNoCol = INT_MAX;
 constexpr int kMaxTop = 256;      // teacher logits per row
 constexpr int kMaxSplits = 16;    // runs of the contraction of dH or dW
 constexpr float kLog2e = 1.4426950408889634f;
+// Limits of what a CTA waits for before it leaves: loads and products that it has
+// started end within microseconds.
+constexpr unsigned long long kLeaveNs = 10000000, kSettleNs = 50000;
 
 // The products. Operands: Stats, Grad: A = H, B = W (both K-major); Dh: A = G
 // (K-major), B = W (MN-major); Dw: A = G, B = H (both MN-major). StatsShort is
@@ -110,7 +113,7 @@ struct Cfg {
     static constexpr int kEpiOffset = kStages * kStageBytes;
     static constexpr int kEpiBytes = kEpiWarps * kEpiBufBytes;
     static constexpr int kBarOffset = kEpiOffset + kEpiBytes;
-    static constexpr int kBarCount = 2 * kStages + 4 + 2 * kQueue;
+    static constexpr int kBarCount = 2 * kStages + 5 + 2 * kQueue;
     static constexpr int kBarBytes = kBarCount * 8 + 16 + 4 * kQueue;
     static constexpr int kSmemBytes = kBarOffset + kBarBytes + 1024;
     static_assert(kStageBytes % 1024 == 0, "ring slots must keep 1024-byte alignment");
@@ -259,6 +262,12 @@ __device__ __forceinline__ void st_release_gpu(int* addr, int v) {
 // Global memory seen by ordinary loads so far is seen by TMA loads from here on.
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.global;" ::: "memory"); }
 
+// Time for what went to the other CTA of the pair, or is counted there, to land.
+__device__ __forceinline__ void settle() {
+    const uint64_t t0 = globaltimer_ns();
+    for (int i = 0; i < 100000 && globaltimer_ns() - t0 < kSettleNs; ++i) __nanosleep(1000);
+}
+
 // 2^x by the hardware's approximation (off by about 2^-22 of the result, results
 // below 2^-126 are zeros): every use is a term of a sum of exponentials or a
 // probability.
@@ -315,7 +324,8 @@ __device__ __forceinline__ void merge_row(const MergeParams& p, int row, int f, 
     // which is rounded to its own size, those near 0 would be lost.
     const float ref = finite_or_zero(m), logs = logf(s);
     const bool there = row < p.rows;
-    if (there && lane == 0) p.lse[row] = i >= 0 ? logs + ref * p.inv_tau : 0.0f;
+    // A launch that was given up leaves no number that a backward pass could go on from.
+    if (there && lane == 0) p.lse[row] = failed ? NAN : (i >= 0 ? logs + ref * p.inv_tau : 0.0f);
     float v = 0.0f;
     if (f == kLoss && p.eq == nullptr) {
         v = logs - (z_one - ref);
@@ -399,6 +409,7 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
     const uint32_t tempty0 = tfull0 + 16;
     const uint32_t qfull0 = tempty0 + 16;
     const uint32_t qempty0 = qfull0 + 8 * kQueue;
+    const uint32_t done0 = qempty0 + 8 * kQueue;  // the products' end, for their issuer alone
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kBarOffset + C::kBarCount * 8);
     volatile int* ring = reinterpret_cast<volatile int*>(smem + C::kBarOffset + C::kBarCount * 8 + 16);
     const uint32_t ring_addr = smem_u32(const_cast<int*>(ring));
@@ -424,6 +435,7 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
             mbar_init(qfull0 + 8 * q, 1);
             mbar_init(qempty0 + 8 * q, (kEpiWarps + 1) * kCtaGroup);
         }
+        mbar_init(done0, 1);
         fence_barrier_init();
         // The peer's slots are filled by asynchronous stores, each armed before the
         // leader may write it.
@@ -532,6 +544,7 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
             // launch-wide counter.
             int next = cluster;
             bool waited = !early;
+            bool ended = false;  // every tile has been loaded
             while (ok) {
                 int t;
                 if (rank == 0) {
@@ -564,6 +577,7 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
                 }
                 if (++qs == kQueue) { qs = 0; qph ^= 1; }
                 if (t < 0) {
+                    ended = true;
                     griddep_launch_dependents();
                     break;
                 }
@@ -631,17 +645,19 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
                 }
             }
             if (!waited) griddep_wait();
-            if (status_failed(status_word) && rank == 0) {
-                // The launch is being abandoned: before this CTA (pair) exits, wait
-                // (bounded) for the loads it still has in flight into its ring.
-                const unsigned long long drain_ns = min(p.timeout_ns, 100000000ull);
+            // This CTA (pair) leaves only when the loads into its ring have landed. At a
+            // normal end the other roles wait longer than that anyway; where one of them
+            // has given up, perhaps without a status word to say so, this is the only wait.
+            if (rank == 0) {
                 for (int s = 0; s < kStages; ++s) {
                     if (issued <= s) continue;
                     const long long last = ((issued - 1 - s) / kStages) * kStages + s;
-                    mbar_wait(full0 + 8 * s, static_cast<uint32_t>((last / kStages) & 1), nullptr,
-                              drain_ns, 0);
+                    mbar_wait(full0 + 8 * s, static_cast<uint32_t>((last / kStages) & 1), nullptr, kLeaveNs, 0);
                 }
             }
+            // A peer that has run ahead of a leader that gave up has loads that no barrier
+            // counts, and a leader may have sent it a tile id just now.
+            if (kPair && (!ended || status_failed(status_word))) settle();
         }
         __syncwarp();
     } else if (warp == 1) {
@@ -752,6 +768,10 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
                     status = status_word;
                 }
             }
+            // The products read the rings and write the accumulators of the CTA (pair): it
+            // leaves when they have ended, although an epilogue that gave up does not wait.
+            umma_commit<kCtaGroup>(kPair ? mapa_shared(done0, 0) : done0);
+            mbar_wait(done0, 0, nullptr, kLeaveNs, 0);
         }
         __syncwarp();
     } else {
