@@ -21,10 +21,11 @@
 // recomputed and turned into G = g_t (p - q) in 16 bits (T x piece), then
 //   dH += G W_piece     (fp32, added piece after piece in stream order)
 //   dW_piece = G^T H    (rounded once)
-// G is the operand both products read, so it stays the operands' type: with
-// |G| <= 1 (the factor common to all rows is applied after the products) its
-// rounding is half a step of the type for each term, no more than the
-// operands' own.
+// G is the operand both products read, so it stays the operands' type: its
+// rounding is half a step of the type for each term. The factor common to all rows
+// is applied after the products, in 32 bits, so that |G| <= 1; half precision holds
+// G times 2^14 (kHalfScale), since its steps below 2^-14 are 2^-24 wide whatever the
+// value and most probabilities over a large vocabulary are there.
 //
 // Rows without a target are gathered out first: they cost nothing, and what
 // they hold (padding, infinities, NaN) meets no other row. W and H keep their
@@ -68,6 +69,10 @@ constexpr int kNoCol = INT_MAX;
 constexpr int kMaxTop = 256;      // teacher logits per row
 constexpr int kMaxSplits = 16;    // runs of the contraction of dH or dW
 constexpr float kLog2e = 1.4426950408889634f;
+// G in half precision: 2^14 of its 65504 for 1, so full precision from 2^-28 on. 128256
+// flat logits without it: dW of tokens that are no target off by a relative 2.1e-3
+// instead of 2.2e-4.
+constexpr float kHalfScale = 16384.0f;
 // Limits of what a CTA waits for before it leaves: loads and products that it has
 // started end within microseconds.
 constexpr unsigned long long kLeaveNs = 10000000, kSettleNs = 50000;
@@ -194,7 +199,7 @@ struct Params {
     float* zsel;          // Stats: [rows][top] logits at the targets; Grad: their log-probabilities
     float2* part;         // Stats: [gathered row][part_ld half tiles] (maximum, sum of exponentials)
     long long part_ld;
-    const float4* rgrad;  // Grad: [gathered row] (g_t, -lse_t log2(e), g_t (p - 1) at the one target, 0)
+    const float4* rgrad;  // Grad: [gathered row] (g_t, -lse_t log2(e), g_t (p - 1) at the one target, 0), g_t in G's scale
     int top;
     float c2;             // log2(e) / tau
     MergeParams merge;    // Stats
@@ -1368,6 +1373,7 @@ struct RowsParams {
     const float* target_logp;
     float4* rgrad;        // see Params
     float tau;
+    float scale;          // of G
     const uint4* hidden;  // gather: H, and where its copy goes
     uint4* copy;
     long long ld, ld_copy;
@@ -1443,7 +1449,8 @@ __global__ void __launch_bounds__(1024) rows_kernel(const RowsParams p) {
         if (counting) copying = left_out != 0;
         for (int i = 0; i < 32; ++i) gmax = fmaxf(gmax, warp_max[i]);
     }
-    // At most 1, so that G fits half precision whatever the loss is scaled by.
+    // At most 1 (times the scale), so that G fits half precision whatever the loss is
+    // scaled by.
     const float unit = gmax > 0.0f ? gmax : 1.0f;
     if (tid == 0) base = 0;
     __syncthreads();
@@ -1508,7 +1515,7 @@ __global__ void __launch_bounds__(1024) rows_kernel(const RowsParams p) {
                     if (p.target != nullptr) p.ecol[i] = col[j];
                 }
                 if (p.rgrad == nullptr) continue;
-                const float g = per_row ? p.grad[t] / unit : 1.0f;
+                const float g = (per_row ? p.grad[t] / unit : 1.0f) * p.scale;
                 // p - 1 at the one target, without the difference of two numbers near 1.
                 const float below = p.target != nullptr ? expm1f(p.target_logp[t]) : 0.0f;
                 p.rgrad[i] = f[j] == kBad ? make_float4(NAN, NAN, NAN, 0.0f)
@@ -1563,6 +1570,7 @@ __global__ void __launch_bounds__(1024) rows_kernel(const RowsParams p) {
         if (p.rgrad != nullptr) {
             if (per_row) h.alpha = unit * p.tau;
             else h.alpha = p.grad[0] * p.tau / (p.reduction == B200_VL_MEAN ? static_cast<float>(max(n_valid, 1)) : 1.0f);
+            h.alpha /= p.scale;
         }
         *p.head = h;
     }
@@ -2172,6 +2180,7 @@ static int launch_rows(const Call& c, const void* index, const void* teacher, co
     r.target_logp = target_logp;
     r.rgrad = grad != nullptr ? c.at<float4>(l.rgrad) : nullptr;
     r.tau = static_cast<float>(d.temperature);
+    r.scale = d.dtype == B200_VL_F16 ? kHalfScale : 1.0f;
     r.hidden = static_cast<const uint4*>(hidden);
     r.copy = c.at<uint4>(gathered);
     r.ld = d.ld_hidden / 8;
