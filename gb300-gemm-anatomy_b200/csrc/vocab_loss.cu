@@ -335,7 +335,11 @@ __device__ __forceinline__ void merge_row(const MergeParams& p, int row, int f, 
     if (f == kLoss && p.eq == nullptr) {
         v = logs - (z_one - ref);
         if (lane == 0) p.target_logp[row] = -v;
-    } else if (f == kLoss) {
+    } else if (f != kLoss) {
+        // Nothing reads these, but no output keeps what was in its memory.
+        if (there)
+            for (int k = lane; k < p.top; k += lanes) p.target_logp[static_cast<long long>(row) * p.top + k] = 0.0f;
+    } else {
         const long long e = static_cast<long long>(row) * p.top;
         for (int k = lane; k < p.top; k += lanes) {
             const float qv = p.eq[e + k];
@@ -1219,6 +1223,7 @@ struct TeacherParams {
     float* eq;
     unsigned short* epos;
     int* flag;
+    float* zsel;          // forward: logits at the targets, zeros behind a row's last
     // Where the products run over all rows in their order: nothing is left to number.
     Head* head;           // or null: the rows' kernel follows
     int* rowmap;
@@ -1328,6 +1333,7 @@ __global__ void __launch_bounds__(kTeacherThreads) teacher_kernel(const TeacherP
     for (int i = out + tid; i < p.top; i += kTeacherThreads) {
         ecol[i] = kNoCol;
         eq[i] = 0.0f;
+        if (p.zsel != nullptr) p.zsel[static_cast<long long>(t) * p.top + i] = 0.0f;
     }
     if (tid == 0) {
         p.flag[t] = bad ? kBad : (any ? kLoss : kNoLoss);
@@ -2147,6 +2153,7 @@ static int launch_rows(const Call& c, const void* index, const void* teacher, co
         t.ecol = c.at<int>(l.ecol);
         t.eq = c.at<float>(l.eq);
         t.flag = c.at<int>(l.flag);
+        t.zsel = grad == nullptr ? c.at<float>(l.zsel) : nullptr;
         if (!gather) {
             t.head = c.head();
             t.rowmap = c.at<int>(l.rowmap);

@@ -454,7 +454,8 @@ int b200_vocab_loss_info(const B200VocabLossDesc* desc, int sm_count, B200VocabL
 /* Asynchronous on `stream`, on the current device. loss: fp32, rows values
  * (NONE) or one. For the backward pass: lse, fp32, rows values (log sum
  * exp(z / tau)); target_logp, fp32, rows x max(top, 1) values, the
- * log-probabilities of the targets in an order of its own. The workspace is
+ * log-probabilities of the targets in an order of its own, zeros where a row
+ * has fewer. Every value is written. The workspace is
  * scratch for this call alone. A wait that runs out in a kernel leaves NaN in
  * loss and lse. */
 int b200_vocab_loss_forward(const B200VocabLossDesc* desc, const void* hidden, const void* weight,
