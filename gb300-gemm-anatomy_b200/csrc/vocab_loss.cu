@@ -25,7 +25,10 @@
 // rounding is half a step of the type for each term. The factor common to all rows
 // is applied after the products, in 32 bits, so that |G| <= 1; half precision holds
 // G times 2^14 (kHalfScale), since its steps below 2^-14 are 2^-24 wide whatever the
-// value and most probabilities over a large vocabulary are there.
+// value and most probabilities over a large vocabulary are there. Weights of the rows
+// (a gradient for each row's loss) leave G as powers of two: bf16 has the exponents to
+// hold them all the same; half precision does not, so there a row's power of two goes
+// to its row of dH in 32 bits, and to dW on a copy of H (weigh_kernel).
 //
 // Rows without a target are gathered out first: they cost nothing, and what
 // they hold (padding, infinities, NaN) meets no other row. W and H keep their
@@ -95,6 +98,8 @@ struct Head {
     int n_valid;      // rows with a loss, if the rows' kernel ran
     int compact;      // 1: the rows are those of the gathered copy of H
     float alpha;      // factor common to all rows of G, applied after the products
+    int g_exponent;   // weights of rows: the exponent of the largest finite one
+    unsigned h_most;  // and of the largest finite |h| 2^(row's exponent - g_exponent), its bits
 };
 
 // kSubM = 2 (Dw in pairs): a tile is two blocks of 256 rows that share their B
@@ -199,7 +204,7 @@ struct Params {
     float* zsel;          // Stats: [rows][top] logits at the targets; Grad: their log-probabilities
     float2* part;         // Stats: [gathered row][part_ld half tiles] (maximum, sum of exponentials)
     long long part_ld;
-    const float4* rgrad;  // Grad: [gathered row] (g_t, -lse_t log2(e), g_t (p - 1) at the one target, 0), g_t in G's scale
+    const float4* rgrad;  // Grad: [gathered row] (g_t, -lse_t log2(e), g_t (p - 1) at the one target, its exponent), g_t in G's scale
     int top;
     float c2;             // log2(e) / tau
     MergeParams merge;    // Stats
@@ -1380,6 +1385,7 @@ struct RowsParams {
     float4* rgrad;        // see Params
     float tau;
     float scale;          // of G
+    int split;            // weights of rows: 1 leaves their exponents out of G
     const uint4* hidden;  // gather: H, and where its copy goes
     uint4* copy;
     long long ld, ld_copy;
@@ -1455,9 +1461,9 @@ __global__ void __launch_bounds__(1024) rows_kernel(const RowsParams p) {
         if (counting) copying = left_out != 0;
         for (int i = 0; i < 32; ++i) gmax = fmaxf(gmax, warp_max[i]);
     }
-    // At most 1 (times the scale), so that G fits half precision whatever the loss is
-    // scaled by.
-    const float unit = gmax > 0.0f ? gmax : 1.0f;
+    // G holds the weights over the largest one's power of two, below 2 (times the scale),
+    // or each over its own: exact, and no row's gradient depends on another row's weight.
+    const int g_exponent = gmax > 0.0f ? ilogbf(gmax) : 0;
     if (tid == 0) base = 0;
     __syncthreads();
     for (int r0 = 0; r0 < p.rows; r0 += kChunk) {
@@ -1521,11 +1527,20 @@ __global__ void __launch_bounds__(1024) rows_kernel(const RowsParams p) {
                     if (p.target != nullptr) p.ecol[i] = col[j];
                 }
                 if (p.rgrad == nullptr) continue;
-                const float g = (per_row ? p.grad[t] / unit : 1.0f) * p.scale;
+                float g = 1.0f;
+                int exponent = g_exponent;
+                if (per_row) {
+                    g = p.grad[t];
+                    // A weight of 0 is no reason to scale H by anything.
+                    if (p.split && isfinite(g) && f[j] != kBad) exponent = g != 0.0f ? ilogbf(g) : g_exponent - 200;
+                    g = scalbnf(g, -exponent);
+                }
+                g *= p.scale;
+                const float own = __int_as_float(exponent);
                 // p - 1 at the one target, without the difference of two numbers near 1.
                 const float below = p.target != nullptr ? expm1f(p.target_logp[t]) : 0.0f;
-                p.rgrad[i] = f[j] == kBad ? make_float4(NAN, NAN, NAN, 0.0f)
-                                          : make_float4(g, -p.lse[t] * kLog2e, g * below, 0.0f);
+                p.rgrad[i] = f[j] == kBad ? make_float4(NAN, NAN, NAN, own)
+                                          : make_float4(g, -p.lse[t] * kLog2e, g * below, own);
             }
         }
         __syncthreads();
@@ -1574,11 +1589,94 @@ __global__ void __launch_bounds__(1024) rows_kernel(const RowsParams p) {
         h.compact = copying;
         h.alpha = 1.0f;
         if (p.rgrad != nullptr) {
-            if (per_row) h.alpha = unit * p.tau;
+            if (per_row) h.alpha = scalbnf(p.tau, g_exponent);
             else h.alpha = p.grad[0] * p.tau / (p.reduction == B200_VL_MEAN ? static_cast<float>(max(n_valid, 1)) : 1.0f);
             h.alpha /= p.scale;
         }
+        h.g_exponent = g_exponent;
+        h.h_most = 0;
         *p.head = h;
+    }
+}
+
+// Weights of rows in half precision: dW = sum_t g_t (p - q)_t h_t runs over a copy of H
+// that holds each row's power of two, so that G is free of it. The copy is scaled by one
+// more power of two for all rows, its largest element then at 2^14 or above: rows of
+// 2^-24 of that weight keep what is left of half precision's 40 binades. Exact but for
+// elements below 2^-14, which lose less than 2^-39 of the largest. Weights folded
+// into G instead cost rows of 1/1000 of the largest weight a third of their dW and 0.4 %
+// of their dH at 32064 tokens. The copy takes one more pass over H for its
+// largest element; both are bound by reading H.
+struct WeighParams {
+    Head* head;
+    const float4* rgrad;
+    const uint4* hidden;  // H, and the gathered copy of it
+    const uint4* copy;
+    uint4* weighed;
+    long long ld, ld_copy;
+    int rows, vecs;
+    float tau;            // in G's scale
+};
+
+constexpr int kWeighWarps = 8;
+
+__device__ __forceinline__ const uint4* weigh_source(const WeighParams& p, int i) {
+    return p.head->compact ? p.copy + i * p.ld_copy : p.hidden + i * p.ld;
+}
+
+__global__ void __launch_bounds__(32 * kWeighWarps) weigh_most_kernel(const WeighParams p) {
+    __shared__ unsigned mosts[kWeighWarps];
+    griddep_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int n = p.head->n_rows, g_exponent = p.head->g_exponent;
+    unsigned most = 0;
+    for (int i = blockIdx.x * kWeighWarps + warp; i < n; i += gridDim.x * kWeighWarps) {
+        const uint4* src = weigh_source(p, i);
+        unsigned m = 0;  // magnitudes order like their bits
+        auto finite = [&](unsigned bits) { if (bits < 0x7c00u) m = max(m, bits); };
+        for (int v = lane; v < p.vecs; v += 32) {
+            const uint4 x = __ldg(src + v);
+            for (const unsigned w : {x.x, x.y, x.z, x.w}) {
+                finite(w & 0x7fffu);
+                finite((w >> 16) & 0x7fffu);
+            }
+        }
+        m = __reduce_max_sync(0xffffffffu, m);
+        const float h = __half2float(__ushort_as_half(static_cast<unsigned short>(m)));
+        most = max(most, __float_as_uint(scalbnf(h, __float_as_int(p.rgrad[i].w) - g_exponent)));
+    }
+    if (lane == 0) mosts[warp] = most;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    for (int w = 0; w < kWeighWarps; ++w) most = max(most, mosts[w]);
+    atomicMax(&p.head->h_most, most);  // a maximum: whatever the order
+}
+
+__global__ void __launch_bounds__(32 * kWeighWarps) weigh_kernel(const WeighParams p) {
+    griddep_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int n = p.head->n_rows, g_exponent = p.head->g_exponent;
+    const float most = __uint_as_float(p.head->h_most);
+    const int up = most > 0.0f ? max(0, min(60, 14 - ilogbf(most))) : 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0) p.head->alpha = scalbnf(p.tau, g_exponent - up);
+    // Rows of zeros behind the last one: dW's contraction runs over whole k-slices.
+    const int end = min(p.rows, (max(n, 1) + 255) / 256 * 256);
+    for (int i = blockIdx.x * kWeighWarps + warp; i < end; i += gridDim.x * kWeighWarps) {
+        uint4* dst = p.weighed + i * p.ld_copy;
+        if (i >= n) {
+            for (int v = lane; v < p.vecs; v += 32) dst[v] = make_uint4(0, 0, 0, 0);
+            continue;
+        }
+        const uint4* src = weigh_source(p, i);
+        const float factor = scalbnf(1.0f, __float_as_int(p.rgrad[i].w) - g_exponent + up);
+        auto times = [&](uint32_t w) {
+            const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w));
+            return pack_half2(x.x * factor, x.y * factor);
+        };
+        for (int v = lane; v < p.vecs; v += 32) {
+            const uint4 x = __ldg(src + v);
+            dst[v] = make_uint4(times(x.x), times(x.y), times(x.z), times(x.w));
+        }
     }
 }
 
@@ -1631,11 +1729,13 @@ struct FinishParams {
     int splits_h, splits_w, rows, hidden, vocab, fp16;
     int width;            // threads of a row: 32 to 256
     int tile_m_h, slots_h, slots_w, slices_h, cost16_h, cost16_w;  // of runs_for, as in the products
+    const float4* rgrad;  // weights of rows: their exponents, where G is free of them
+    float tau;            // in G's scale
     void* d_hidden;
     void* d_weight;
 };
 
-// Adds the splits of dH (and of dW) in order, applies the common factor, rounds,
+// Adds the splits of dH (and of dW) in order, applies the common (or the row's) factor, rounds,
 // and puts the rows of dH back in their places; rows without a loss get zeros.
 // 4 bytes read per split and 2 written for each element. Short rows share a block
 // (step of 4000 x 8000 x 256 as a graph: 111 us, 123 with a block for each row).
@@ -1662,6 +1762,7 @@ __global__ void __launch_bounds__(256) finish_kernel(const FinishParams p) {
         const int splits = is_h ? splits_h : splits_w;
         const long long stride = is_h ? p.stride_h : p.stride_w;
         const float* part = (is_h ? p.part_h : p.part_w) + max(i, 0) * p.ld_part;
+        const float factor = is_h && p.rgrad != nullptr ? scalbnf(p.tau, __float_as_int(p.rgrad[max(i, 0)].w)) : alpha;
         uint4* out = static_cast<uint4*>(is_h ? p.d_hidden : p.d_weight) + static_cast<long long>(t) * vecs;
         for (int v = at; v < vecs; v += p.width) {
             float x[8] = {};
@@ -1677,8 +1778,8 @@ __global__ void __launch_bounds__(256) finish_kernel(const FinishParams p) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 // Never a silent half of a gradient: a launch that was given up leaves NaN.
-                const float lo = failed ? NAN : (i >= 0 ? alpha * x[2 * j] : 0.0f);
-                const float hi = failed ? NAN : (i >= 0 ? alpha * x[2 * j + 1] : 0.0f);
+                const float lo = failed ? NAN : (i >= 0 ? factor * x[2 * j] : 0.0f);
+                const float hi = failed ? NAN : (i >= 0 ? factor * x[2 * j + 1] : 0.0f);
                 o[j] = p.fp16 ? pack_half2(lo, hi) : pack_bf16x2(lo, hi);
             }
             out[v] = make_uint4(o[0], o[1], o[2], o[3]);
@@ -1720,11 +1821,12 @@ struct Layout {
     // Offsets in the workspace.
     int64_t flag, rowmap, inv, ecol, eq, epos;           // both directions
     int64_t zsel, part, row_loss, gathered_forward;
-    int64_t rgrad, gathered_backward, g, part_h, part_w;
+    int64_t rgrad, gathered_backward, weighed, g, part_h, part_w;
     int64_t epos_ld;
     int64_t ld_gathered, ld_part;                        // row pitches on 128-byte lines
     int64_t bytes_forward, bytes_backward;
     bool gather_forward;
+    bool split;           // weights of rows leave G (RowsParams)
     int merge_lanes;      // of MergeParams
 };
 
@@ -1946,6 +2048,8 @@ static Layout layout_for(const B200VocabLossDesc& d, int64_t sms) {
     at = common;
     l.rgrad = take(16 * T);
     l.gathered_backward = take(2 * T * l.ld_gathered);
+    l.split = d.dtype == B200_VL_F16 && d.reduction == B200_VL_NONE;
+    l.weighed = take(l.split ? 2 * T * l.ld_gathered : 0);
     l.g = take(2 * T * l.piece);
     l.part_h = take(4 * l.splits_h * l.rows_pad * l.ld_part);
     l.part_w = take(l.splits_w > 1 ? 4 * l.splits_w * l.piece * l.ld_part : 0);
@@ -2029,6 +2133,7 @@ static int device_state(DeviceState* out) {
         cudaFuncAttributes loaded;
         for (const void* fn : {reinterpret_cast<const void*>(teacher_kernel<32>), reinterpret_cast<const void*>(teacher_kernel<128>),
                                reinterpret_cast<const void*>(rows_kernel),
+                               reinterpret_cast<const void*>(weigh_most_kernel), reinterpret_cast<const void*>(weigh_kernel),
                                reinterpret_cast<const void*>(merge_kernel),
                                reinterpret_cast<const void*>(finish_kernel)})
             B200_CUDA_TRY(cudaFuncGetAttributes(&loaded, fn));
@@ -2129,6 +2234,8 @@ static int map_2d(const Call& c, CUtensorMap* map, const void* base, int64_t row
     return encode_tmap_2d(map, c.type, 2, base, rows, cols, ld, box_rows, box_cols, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+static float g_scale(const B200VocabLossDesc& d) { return d.dtype == B200_VL_F16 ? kHalfScale : 1.0f; }
+
 // Targets, row numbers and the gathered copy of H.
 static int launch_rows(const Call& c, const void* index, const void* teacher, const void* hidden, bool gather,
                        int64_t gathered, const float* grad, const float* lse,
@@ -2187,7 +2294,8 @@ static int launch_rows(const Call& c, const void* index, const void* teacher, co
     r.target_logp = target_logp;
     r.rgrad = grad != nullptr ? c.at<float4>(l.rgrad) : nullptr;
     r.tau = static_cast<float>(d.temperature);
-    r.scale = d.dtype == B200_VL_F16 ? kHalfScale : 1.0f;
+    r.scale = g_scale(d);
+    r.split = l.split;
     r.hidden = static_cast<const uint4*>(hidden);
     r.copy = c.at<uint4>(gathered);
     r.ld = d.ld_hidden / 8;
@@ -2195,6 +2303,26 @@ static int launch_rows(const Call& c, const void* index, const void* teacher, co
     r.vecs = static_cast<int>(d.hidden / 8);
     const int64_t blocks = gather ? std::min<int64_t>(ceil_div(d.rows, 8), c.dev.sms) : 1;
     return launch(rows_kernel, static_cast<int>(blocks), 1024, 0, 1, d.top > 0, c.stream, r);
+}
+
+// The copy of H with the rows' weights.
+static int launch_weigh(const Call& c, const void* hidden) {
+    const B200VocabLossDesc& d = *c.d;
+    const Layout& l = c.l;
+    WeighParams w{};
+    w.head = c.head();
+    w.rgrad = c.at<float4>(l.rgrad);
+    w.hidden = static_cast<const uint4*>(hidden);
+    w.copy = c.at<uint4>(l.gathered_backward);
+    w.weighed = c.at<uint4>(l.weighed);
+    w.ld = d.ld_hidden / 8;
+    w.ld_copy = l.ld_gathered / 8;
+    w.rows = static_cast<int>(d.rows);
+    w.vecs = static_cast<int>(d.hidden / 8);
+    w.tau = static_cast<float>(d.temperature) / g_scale(d);
+    const int blocks = static_cast<int>(std::min<int64_t>(ceil_div(d.rows, kWeighWarps), 4 * c.dev.sms));
+    const int rc = launch(weigh_most_kernel, blocks, 32 * kWeighWarps, 0, 1, true, c.stream, w);
+    return rc != B200_OK ? rc : launch(weigh_kernel, blocks, 32 * kWeighWarps, 0, 1, true, c.stream, w);
 }
 
 static Params base_params(const Call& c) {
@@ -2354,13 +2482,16 @@ static int backward(const B200VocabLossDesc* d, const void* hidden, const void* 
     void* hg = c.at<void>(l.gathered_backward);
     void* g = c.at<void>(l.g);
     CUtensorMap h_k, hg_k, h_mn, hg_mn, w_k, w_mn, g_st, g_k, g_mn, dh_st, dw_st;
+    const bool weigh = l.split && d_weight != nullptr;
     std::memset(&dw_st, 0, sizeof(dw_st));
     const int64_t T = d->rows, V = d->vocab, D = d->hidden;
     const int box_m = a_rows(*d, l.cta_group), box_m_h = a_rows(*d, l.cta_group_h);
     rc = map_2d(c, &h_k, hidden, T, D, d->ld_hidden, box_m, kBK);
     if (rc == B200_OK) rc = map_2d(c, &hg_k, hg, T, D, l.ld_gathered, box_m, kBK);
-    if (rc == B200_OK) rc = map_2d(c, &h_mn, hidden, T, D, d->ld_hidden, kBK, 64);
-    if (rc == B200_OK) rc = map_2d(c, &hg_mn, hg, T, D, l.ld_gathered, kBK, 64);
+    if (rc == B200_OK)
+        rc = weigh ? map_2d(c, &h_mn, c.at<void>(l.weighed), T, D, l.ld_gathered, kBK, 64)
+                   : map_2d(c, &h_mn, hidden, T, D, d->ld_hidden, kBK, 64);
+    if (rc == B200_OK) rc = weigh ? (hg_mn = h_mn, B200_OK) : map_2d(c, &hg_mn, hg, T, D, l.ld_gathered, kBK, 64);
     if (rc == B200_OK) rc = map_2d(c, &w_k, weight, V, D, d->ld_weight, l.tile_n / l.cta_group, kBK);
     if (rc == B200_OK) rc = map_2d(c, &w_mn, weight, V, D, d->ld_weight, kBK, 64);
     if (rc == B200_OK) rc = map_2d(c, &g_st, g, T, l.piece, l.piece, 32, 64);
@@ -2375,6 +2506,7 @@ static int backward(const B200VocabLossDesc* d, const void* hidden, const void* 
         rc = l.splits_w > 1 ? partial_map(&dw_st, l.part_w, l.splits_w * l.piece) : map_2d(c, &dw_st, d_weight, V, D, D, 32, 64);
     if (rc != B200_OK) return rc;
     rc = launch_rows(c, index, teacher, hidden, true, l.gathered_backward, grad_loss, lse, target_logp);
+    if (rc == B200_OK && weigh) rc = launch_weigh(c, hidden);
     for (int64_t v0 = 0; rc == B200_OK && v0 < V; v0 += l.piece) {
         const int64_t vp = std::min(l.piece, V - v0);
         Params p = base_params(c);
@@ -2438,6 +2570,8 @@ static int backward(const B200VocabLossDesc* d, const void* hidden, const void* 
     f.hidden = static_cast<int>(D);
     f.vocab = static_cast<int>(V);
     f.fp16 = d->dtype == B200_VL_F16;
+    f.rgrad = l.split ? c.at<float4>(l.rgrad) : nullptr;
+    f.tau = static_cast<float>(d->temperature) / g_scale(*d);
     f.d_hidden = d_hidden;
     f.d_weight = d_weight;
     for (f.width = 256; f.width > 32 && f.width / 2 >= D / 8;) f.width /= 2;
@@ -2477,7 +2611,7 @@ int b200_vocab_loss_info(const B200VocabLossDesc* desc, int sm_count, B200VocabL
     out->workspace_backward = l.bytes_backward;
     const int64_t teacher = desc->top > 0 ? 1 : 0;
     out->launches_forward = desc->rows == 0 ? 0 : 2 + (l.gather_forward ? teacher : 0) + (l.merge_lanes == 0 ? 1 : 0);
-    out->launches_backward = desc->rows == 0 ? 0 : 2 + teacher + 3 * l.pieces;
+    out->launches_backward = desc->rows == 0 ? 0 : 2 + teacher + (l.split ? 2 : 0) + 3 * l.pieces;
     return B200_OK;
     B200_ABI_GUARD_END
 }

@@ -4,9 +4,12 @@ vocab_loss_reference grants every element of G what the largest row's weight cos
 is held to its own size, element by element, from the roundings that the kernels make:
 
 * a logit is off by dz, p and q by a relative 2 dz / tau + 2^-18 (see vocab_loss_reference);
-* G = p - q, times the row's weight, is rounded to half a step h of the
-  operands' type. bf16 reaches to 2^-126. In half precision G is held times 2^14, where steps below 2^-14
+* G = p - q, times the row's weight or the part of it in [1, 2), is rounded to half a step h of the
+  operands' type. bf16 reaches 2^-126 of the largest row's weight: 2^-100 for weights up to 2^26 apart. In half precision G is held times 2^14, where steps below 2^-14
   are 2^-24 wide: off by 2^-25 of that, 2^-39 |g_t| of its own;
+* weights of rows that differ in half precision: the row's power of two goes to d_hidden in 32 bits, and to
+  d_weight on a copy of hidden that is scaled until its largest element is 2^14 or more. What that copy loses
+  below 2^-14 is 2^-25 of that: 2^-39 A for A = max_t |g_t| max_d |h_td|, times the part of G in [1, 2);
 * the products add n terms in 32 bits, at most (n / 16 + 32) 2^-23 of the magnitudes' sum, and round to the
   operands' type once, in half precision by no less than 2^-25.
 """
@@ -28,7 +31,7 @@ def gradients(hidden, weight, kept, index, q, tau, up):
     dense = torch.zeros(n, V, dtype=f64, device=dev).scatter_add_(1, index[kept], q[kept])
     p = torch.softmax(z / tau, 1)
     P = tau * (p - dense)  # G without the row's weight
-    tiny = 2.0 ** -39 if half else 2.0 ** -126
+    tiny = 2.0 ** -39 if half else 2.0 ** -100
     E = hs * P.abs() + tau * (p * (2 * dz / tau + 2.0 ** -18) + dense * 2.0 ** -18 + tiny)
     least = 2.0 ** -25 if half else 2.0 ** -126
 
@@ -41,5 +44,7 @@ def gradients(hidden, weight, kept, index, q, tau, up):
     dh_off[kept] = bound(gh * (P.abs() @ w.abs()), gh * (E @ w.abs()), dh[kept], V)
     dw = (g[:, None] * P).T @ h
     off = (gh * E).T @ h.abs()
+    if half and n:
+        off = off + 2.0 ** -39 * float((gh * h.abs()).max()) * 2 * (P.abs() + E).sum(0)[:, None]
     dw_off = bound((gh * P.abs()).T @ h.abs(), off, dw, n)
     return dh, dh_off, dw, dw_off
