@@ -1261,7 +1261,7 @@ __global__ void __launch_bounds__(kTeacherThreads) teacher_kernel(const TeacherP
             const long long c = index_at(p.index, p.index_bytes, t * p.ld_index + k);
             if (c >= p.vocab) bad = true;
             else if (c >= 0) {
-                l = teacher_at(p.teacher, p.teacher_dtype, t * p.ld_teacher + k) * p.inv_tau;
+                l = teacher_at(p.teacher, p.teacher_dtype, t * p.ld_teacher + k);
                 if (l != -INFINITY) {
                     col = static_cast<unsigned>(c);
                     any = true;
@@ -1281,7 +1281,8 @@ __global__ void __launch_bounds__(kTeacherThreads) teacher_kernel(const TeacherP
     for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, red[0][w]);
     float sum = 0.0f;
     for (int k = tid; k < pad; k += kTeacherThreads) {
-        const float e = prob[k] == -INFINITY ? 0.0f : expf(prob[k] - mx);
+        // The difference first: a logit of the type's lowest value is one, whatever tau.
+        const float e = prob[k] == -INFINITY ? 0.0f : expf((prob[k] - mx) * p.inv_tau);
         prob[k] = e;
         sum += e;
     }
