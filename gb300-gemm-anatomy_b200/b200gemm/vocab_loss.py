@@ -14,6 +14,10 @@ is alive.) Results do not depend on the order in which tiles run: the same call
 gives the same bits.
 
 A kernel wait that runs out (``B200_WAIT_TIMEOUT_MS``) leaves NaN in the results.
+
+Tensors without storage of their own are refused, so ``torch.compile`` cannot trace these losses:
+call them through ``torch.compiler.disable``. Autocast does not cast for them: an fp32 operand is
+refused under it as without it.
 """
 from __future__ import annotations
 

@@ -52,6 +52,15 @@ int64_t row_pitch(const Tensor& t, const char* name) {
     return t.size(0) <= 1 ? t.size(1) : t.stride(0);
 }
 
+// Tensors without storage of their own (FakeTensor, under torch.compile and
+// torch.export, and other subclasses that take every call themselves) have nothing that
+// a kernel could read.
+void check_ordinary(const Tensor& t, const char* name) {
+    TORCH_CHECK_TYPE(!t.key_set().has(c10::DispatchKey::Python), name,
+                     " must be an ordinary tensor, got a subclass without storage of its own; the losses at the vocabulary "
+                     "projection cannot be traced: call them through torch.compiler.disable");
+}
+
 // A tensor that the backward pass reads again. Saved-tensor hooks
 // (torch.autograd.graph.save_on_cpu, a checkpoint) may give back the same values in
 // another layout: the kernels go by the layout that is there now.
@@ -59,6 +68,7 @@ void check_saved(const Tensor& t, const char* name, at::IntArrayRef sizes, at::S
     TORCH_CHECK(t.defined() && t.sizes() == sizes && t.scalar_type() == type && t.device() == device, name,
                 " came back to the backward pass as another tensor than was saved: expected ", sizes, " ", type, " on ",
                 device);
+    check_ordinary(t, name);
 }
 Tensor as_saved(const Tensor& t, const char* name, at::IntArrayRef sizes, at::ScalarType type, at::Device device) {
     check_saved(t, name, sizes, type, device);
@@ -88,7 +98,11 @@ Problem unpack(const c10::IValue& v) {
     return p;
 }
 
-Tensor workspace(int64_t bytes, const Tensor& like) { return at::empty({bytes}, like.options().dtype(at::kByte)); }
+Tensor workspace(int64_t bytes, const Tensor& like) {
+    Tensor ws = at::empty({bytes}, like.options().dtype(at::kByte));
+    check_ordinary(ws, "the workspace");
+    return ws;
+}
 
 int64_t align_up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
@@ -103,6 +117,9 @@ Tensor forward_pass(Problem& p, const Tensor& hidden, const Tensor& weight, cons
     const bool per_row = reduction == B200_VL_NONE;
     const auto f32 = hidden.options().dtype(at::kFloat);
     if (rows == 0) return per_row ? at::empty({0}, f32) : at::zeros({}, f32);
+    const c10::cuda::CUDAGuard guard(hidden.device());
+    Tensor loss = per_row ? at::empty({rows}, f32) : at::empty({}, f32);
+    check_ordinary(loss, "the result");
     B200VocabLossDesc& d = p.desc;
     d.rows = rows;
     d.vocab = weight.size(0);
@@ -119,11 +136,9 @@ Tensor forward_pass(Problem& p, const Tensor& hidden, const Tensor& weight, cons
         d.teacher_dtype = teacher->scalar_type() == at::kFloat ? static_cast<int64_t>(B200_VL_F32)
                                                                : operand_code(teacher->scalar_type());
     }
-    const c10::cuda::CUDAGuard guard(hidden.device());
     check_rc(g_api.info(&d, at::cuda::getCurrentDeviceProperties()->multiProcessorCount, &p.info),
              "b200_vocab_loss_info");
     const int64_t kept = rows * (1 + (teacher ? d.top : 1)), behind = align_up(p.info.workspace_forward, 256);
-    Tensor loss = per_row ? at::empty({rows}, f32) : at::empty({}, f32);
     if (saved != nullptr) *saved = at::empty({kept}, f32);
     Tensor ws = workspace(saved != nullptr ? p.info.workspace_forward : behind + kept * 4, hidden);
     uint8_t* base = ws.mutable_data_ptr<uint8_t>();
@@ -183,6 +198,7 @@ struct VocabLoss : public torch::autograd::Function<VocabLoss> {
         const Tensor kept = as_saved(saved[4], "a result of the forward pass", {d.rows * (1 + std::max<int64_t>(d.top, 1))},
                                      at::kFloat, device);
         const float* lse = kept.const_data_ptr<float>();
+        check_ordinary(grads[0], "the gradient of the loss");
         const Tensor grad = grads[0].to(at::kFloat).contiguous();
         if (want_h) dh = at::empty(hidden.sizes(), hidden.options());
         if (want_w) dw = at::empty(weight.sizes(), weight.options());
@@ -206,6 +222,10 @@ bool is_index(at::ScalarType t) { return t == at::kInt || t == at::kLong; }
 Tensor vocab_loss(const Tensor& hidden, const Tensor& weight, const Tensor& index, const std::optional<Tensor>& teacher,
                   int64_t ignore_index, int64_t reduction, double temperature) {
     TORCH_CHECK(g_api.forward != nullptr, "the entry points of libb200gemm.so are not bound");
+    check_ordinary(hidden, "hidden");
+    check_ordinary(weight, "weight");
+    check_ordinary(index, teacher ? "teacher_index" : "target");
+    if (teacher) check_ordinary(*teacher, "teacher_logits");
     TORCH_CHECK_VALUE(is_operand(hidden.scalar_type()), "hidden must be bfloat16 or float16, got ", hidden.scalar_type());
     TORCH_CHECK_VALUE(weight.scalar_type() == hidden.scalar_type(), "weight must be ", hidden.scalar_type(),
                       " like hidden, got ", weight.scalar_type());
