@@ -287,6 +287,13 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return y;
 }
 
+// The smaller one; NaN where either is.
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float y;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+
 // The reference point of a sum of exponentials: the maximum, or 0 where it is
 // infinite (all terms are then 0, or one is infinite, without a NaN from
 // inf - inf).
@@ -1075,8 +1082,11 @@ vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constan
                     tmem_ld_wait();
                     const int x = col0 + c * 64;
                     const int left = p.n - x;
+                    // At most 1: where z / tau has no digits left behind the point, its
+                    // difference from lse may come out above 0, and half precision holds no
+                    // more than 2 in G's scale. NaN stays NaN.
                     auto grad = [&](uint32_t z) {
-                        return rg.x * exp2_approx(fmaf(__uint_as_float(z), p.c2, rg.y));
+                        return rg.x * exp2_approx(min_nan(fmaf(__uint_as_float(z), p.c2, rg.y), 0.0f));
                     };
                     if (left < 64) {
                         // Columns beyond the piece are zeros of the product that contracts
