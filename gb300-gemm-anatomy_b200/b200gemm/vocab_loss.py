@@ -36,15 +36,18 @@ _REDUCTION_CODE = {"none": _lib.VL_NONE, "mean": _lib.VL_MEAN, "sum": _lib.VL_SU
 
 
 def policy(rows: int, vocab: int, hidden: int, *, top: int = 0, dtype=torch.bfloat16,
-           sm_count: int = 148) -> dict:
+           reduction: str = "mean", sm_count: int = 148) -> dict:
     """The host's choices for a call (b200_vocab_loss_info), computed without a device: tile
     shape, pieces of the vocabulary, runs of the contraction, workspace bytes, launches.
-    ``top=0`` is the cross entropy."""
+    ``top=0`` is the cross entropy. In half precision reduction "none" takes two launches and a
+    copy of hidden more (the weights of rows)."""
     lib = _lib.load()
     if dtype not in _OPERAND_CODE:
         raise ValueError(f"dtype must be bfloat16 or float16, got {dtype}")
+    if reduction not in _REDUCTION_CODE:
+        raise ValueError(f"reduction must be one of {sorted(_REDUCTION_CODE)}, got {reduction!r}")
     desc = _lib.VocabLossDesc(rows, vocab, hidden, hidden, hidden, _OPERAND_CODE[dtype], top, 8, top, top,
-                              _lib.VL_F32, IGNORE_INDEX, _lib.VL_MEAN, 1.0)
+                              _lib.VL_F32, IGNORE_INDEX, _REDUCTION_CODE[reduction], 1.0)
     info = _lib.VocabLossInfo()
     _lib.check(lib.b200_vocab_loss_info(ctypes.byref(desc), sm_count, ctypes.byref(info)),
                "b200_vocab_loss_info", lib)
